@@ -1,0 +1,490 @@
+"""The training operators around the stone attention, timed and compared.
+
+Three operators of one training step: the ragged attention with a learned bias
+by the pair's relative position (``fused_attention_relative``), the dropout of
+the residual branches (``residual_dropout``) and the log probabilities of the
+moves played, with the policy's entropy and its best alternatives
+(``policy_log_probs``).  ``listed`` names the cases, ``draw`` one more of their
+ranges, ``prepare`` makes a case's inputs, ``run`` one pass (through the
+framework's operators where ``own`` is set, else in elementary torch
+operations in fp32), ``exact`` the definition in float64, ``work`` the bytes
+and operations a pass cannot do without.
+"""
+
+import math
+
+import numpy as np
+import torch
+
+own = False
+
+DEV = "cuda:0"
+DTYPES = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
+SIZE = {"bf16": 2, "f16": 2, "f32": 4}
+
+
+def listed():
+    return [
+        # one opening position at a search leaf: a handful of stones after the
+        # four latent rows, the forward alone; launch latency
+        {"name": "relative_leaf_1_f16", "kind": "relative", "positions": 1, "lo": 13, "hi": 13, "heads": 4, "hd": 32,
+         "dtype": "f16", "board": "hex", "reach": 12, "far": True, "train": False},
+        # a leaf batch of the evaluator at the production head layout
+        {"name": "relative_leaf_512_bf16", "kind": "relative", "positions": 512, "lo": 44, "hi": 124, "heads": 4,
+         "hd": 32, "dtype": "bf16", "board": "hex", "reach": 12, "far": True, "train": False},
+        # one block's attention of a training batch, forward and backward; the
+        # stones further than the reach masked out by their bucket
+        {"name": "relative_train_192_bf16", "kind": "relative", "positions": 192, "lo": 44, "hi": 124, "heads": 4,
+         "hd": 32, "dtype": "bf16", "board": "hex", "reach": 12, "far": False, "train": True},
+        # long games in another head layout, odd lengths
+        {"name": "relative_train_16_long_f16", "kind": "relative", "positions": 16, "lo": 511, "hi": 1021, "heads": 8,
+         "hd": 16, "dtype": "f16", "board": "hex", "reach": 24, "far": True, "train": True},
+        # sequences of tokens in one line, buckets by the logarithm of the distance
+        {"name": "relative_train_line_bf16", "kind": "relative", "positions": 2, "lo": 2049, "hi": 4096, "heads": 8,
+         "hd": 64, "dtype": "bf16", "board": "line", "reach": 128, "far": True, "train": True},
+        # the root of one search: 16 candidates of one position's legal moves
+        {"name": "policy_root_1_f32", "kind": "policy", "positions": 1, "lo": 271, "hi": 271, "moves": 1, "top": 16,
+         "dtype": "f32", "train": False},
+        # the policy loss of a training batch over its legal moves, with its gradient
+        {"name": "policy_train_512_f32", "kind": "policy", "positions": 512, "lo": 180, "hi": 1200, "moves": 2,
+         "top": 8, "dtype": "f32", "train": True},
+        # a vocabulary of tokens, the logits as the projection leaves them
+        {"name": "policy_train_64_vocabulary_bf16", "kind": "policy", "positions": 64, "lo": 131072, "hi": 131072,
+         "moves": 1, "top": 4, "dtype": "bf16", "train": True},
+        # one residual branch of a small batch: a launch each way
+        {"name": "dropout_24_f32", "kind": "dropout", "rows": 24 * 61, "width": 128, "x": "f32", "residual": "f32",
+         "p": 0.1, "train": True},
+        # the same at a training batch, mixed precision: bf16 branch onto the fp32 stream
+        {"name": "dropout_512_mixed", "kind": "dropout", "rows": 512 * 124, "width": 128, "x": "bf16",
+         "residual": "f32", "p": 0.1, "train": True},
+        # the window rows of a large batch, an odd width, no residual
+        {"name": "dropout_windows_bf16", "kind": "dropout", "rows": 131071, "width": 255, "x": "bf16",
+         "residual": "", "p": 0.25, "train": True},
+    ]
+
+
+def draw(rng):
+    def log(lo, hi):
+        return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+    kind = rng.choice(["relative", "relative", "relative", "policy", "policy", "dropout"])
+    if kind == "relative":
+        heads, hd = rng.choice([(4, 32), (4, 32), (8, 16), (8, 32), (2, 64), (8, 64)])
+        hi = log(1, 4096)
+        lo = rng.randint(max(1, hi // 3), hi)
+        # the pairs of a drawn case: no more than a quarter of the longest listed one's
+        most = min(512, max(1, (1 << 27) // (4 * heads * hd // 32 * hi * hi)))
+        board = rng.choice(["hex", "hex", "line"])
+        return {"kind": kind, "positions": log(1, most), "lo": lo, "hi": hi, "heads": heads, "hd": hd,
+                "dtype": rng.choice(["bf16", "f16"]), "board": board,
+                "reach": rng.choice([3, 8, 12, 24]) if board == "hex" else rng.choice([16, 128, 511]),
+                "far": rng.random() < 0.7, "train": rng.random() < 0.6}
+    if kind == "policy":
+        hi = log(1, 262144)
+        lo = rng.randint(max(1, hi // 4), hi)
+        return {"kind": kind, "positions": log(1, min(1024, max(1, (1 << 23) // hi))), "lo": lo, "hi": hi,
+                "moves": rng.choice([1, 1, 2, 5]), "top": rng.choice([0, 1, 4, 8, 16, 32]),
+                "dtype": rng.choice(["f32", "bf16", "f16"]), "train": rng.random() < 0.7}
+    return {"kind": kind, "rows": log(1, 100000), "width": rng.choice([1, 7, 64, 127, 128, 128, 255, 256]),
+            "x": rng.choice(["bf16", "f16", "f32"]), "residual": rng.choice(["", "bf16", "f16", "f32", "f32"]),
+            "p": rng.choice([0.05, 0.1, 0.25, 0.5]), "train": rng.random() < 0.7}
+
+
+# ----------------------------------------------------------------- inputs
+
+
+def _lengths(case):
+    """The case's lengths (their order follows the seed, their sum does not)."""
+    rng = np.random.default_rng([7, case["positions"], case["lo"], case["hi"]])
+    lens = rng.integers(case["lo"], case["hi"] + 1, case["positions"])
+    lens[0] = case["hi"]
+    return lens
+
+
+def _hex_buckets(reach):
+    """(2 reach + 3, 2 reach + 3) bucket of every clipped displacement: 0 the
+    same cell, 1 .. reach along an axis by distance, reach + 1 .. 2 reach off
+    the axes, 2 reach + 1 further than the reach; two more for the latents."""
+    d = np.arange(-reach - 1, reach + 2)
+    dq, dr = d[:, None], d[None, :]
+    dist = np.maximum(np.maximum(abs(dq), abs(dr)), abs(dq + dr))
+    axis = (dq == 0) | (dr == 0) | (dq + dr == 0)
+    out = np.where(axis, dist, reach + dist)
+    return np.where(dist > reach, 2 * reach + 1, out).astype(np.int32), 2 * reach + 4
+
+
+def _line_buckets(reach):
+    """(2 reach + 1, 1): 16 buckets a side, the near ones a distance each, the
+    rest by the logarithm of the distance up to the reach."""
+    d = np.arange(-reach, reach + 1)
+    far = 8 + np.floor(np.log(np.maximum(abs(d), 8) / 8) / math.log(max(reach, 9) / 8) * 7.999).astype(np.int64)
+    side = np.where(abs(d) < 8, abs(d), np.minimum(far, 15))
+    return np.where(d > 0, 16 + side, side).astype(np.int32)[:, None], 32
+
+
+def prepare(case, seed):
+    gen = torch.Generator(device=DEV)
+    gen.manual_seed(seed)
+
+    def rows(*shape):
+        return torch.randn(shape, generator=gen, device=DEV)
+
+    kind, order = case["kind"], np.random.default_rng([13, seed])
+    if kind == "relative":
+        lens = order.permutation(_lengths(case))
+        p, t, a, d = case["positions"], int(lens.max()), case["heads"], case["hd"]
+        # (P, A, T, D) views of (P, T, A, D) storage, as the projections leave them
+        q, k, v, grad = (rows(p, t, a, d).to(DTYPES[case["dtype"]]).transpose(1, 2) for _ in range(4))
+        coords = np.zeros((p, t, 2), np.int32)
+        if case["board"] == "hex":
+            # stones spread around the opening, as far as their number needs
+            latents, (buckets, n_buckets) = 4, _hex_buckets(case["reach"])
+            spread = 0.55 * np.sqrt(lens)[:, None, None]
+            coords[:, latents:] = np.rint(order.standard_normal((p, max(t - latents, 0), 2)) * spread)
+        else:
+            latents, (buckets, n_buckets) = 0, _line_buckets(case["reach"])
+            coords[:, :, 0] = np.arange(t)
+        bias = 0.5 * rows(a, n_buckets)
+        if not case["far"]:  # the furthest bucket is closed
+            bias[:, n_buckets - 3 if latents else n_buckets - 1] = -math.inf
+        leaves = [x.requires_grad_(case["train"]) for x in (q, k, v, bias)]
+        return {"kind": kind, "train": case["train"], "leaves": leaves, "grad": grad, "latents": latents,
+                "coords": torch.from_numpy(coords).to(DEV), "buckets": torch.from_numpy(buckets).to(DEV),
+                "lens": torch.from_numpy(lens.astype(np.int32)).to(DEV)}
+    if kind == "policy":
+        lens = order.permutation(_lengths(case))
+        offsets = np.concatenate([[0], np.cumsum(lens)])
+        moves = order.integers(0, lens[:, None], (case["positions"], case["moves"]))
+        moves[:, 1:][order.random(moves[:, 1:].shape) < 0.3] = -1  # fewer moves played than the table holds
+        logits = (2.0 * rows(int(offsets[-1]))).to(DTYPES[case["dtype"]]).requires_grad_(case["train"])
+        p = case["positions"]
+        return {"kind": kind, "train": case["train"], "logits": logits, "top": case["top"],
+                "offsets": torch.from_numpy(offsets).to(DEV), "moves": torch.from_numpy(moves).to(DEV),
+                "grads": [rows(p, case["moves"]), 0.01 * rows(p), 0.1 * rows(p), rows(p, case["top"])]}
+    x = rows(case["rows"], case["width"]).to(DTYPES[case["x"]]).requires_grad_(case["train"])
+    res, out_dtype = None, DTYPES[case["x"]]
+    if case["residual"]:
+        out_dtype = DTYPES[case["residual"]]
+        res = rows(case["rows"], case["width"]).to(out_dtype).requires_grad_(case["train"])
+    return {"kind": kind, "train": case["train"], "x": x, "residual": res, "p": case["p"], "salt": 5,
+            "rng": torch.tensor([0x1234567 * (seed + 1), 11 + seed], dtype=torch.int64, device=DEV),
+            "grad": rows(case["rows"], case["width"]).to(out_dtype)}
+
+
+# ----------------------------------------------------------------- one pass
+
+
+def run(st):
+    return (_own if own else _plain)[st["kind"]](st)
+
+
+def _own_relative(st):
+    import mantisnet
+
+    q, k, v, bias = st["leaves"]
+    out, lse = torch.ops.mantisnet.fused_attention_relative(q, k, v, bias, st["coords"], st["buckets"], st["lens"],
+                                                            st["latents"])
+    if not st["train"]:
+        return {"out": out, "lse": lse}
+    grads = torch.autograd.grad(out, st["leaves"], st["grad"])
+    return {"out": out.detach(), "lse": lse, **dict(zip(("dq", "dk", "dv", "dbias"), grads))}
+
+
+POLICY = ("log_probs", "entropy", "lse", "top_log_probs", "top_moves")
+
+
+def _own_policy(st):
+    import mantisnet
+
+    out = torch.ops.mantisnet.policy_log_probs(st["logits"], st["offsets"], st["moves"], st["top"])
+    res = {name: x.detach() for name, x in zip(POLICY, out)}
+    if st["train"]:
+        res["dlogits"] = torch.autograd.grad(out[:4], st["logits"], st["grads"])[0]
+    return res
+
+
+def _own_dropout(st):
+    import mantisnet
+
+    x, residual = st["x"], st["residual"]
+    out = torch.ops.mantisnet.residual_dropout(x, residual, st["rng"], st["p"], st["salt"])
+    if not st["train"]:
+        return {"out": out}
+    leaves = [x] if residual is None else [x, residual]
+    return {"out": out.detach(), **dict(zip(("dx", "dresidual"), torch.autograd.grad(out, leaves, st["grad"])))}
+
+
+def _pair_buckets(coords, buckets, latents, n_buckets):
+    """(P, T, T) bucket of every pair (query, key)."""
+    delta = coords[:, None, :, :] - coords[:, :, None, :]
+    hq, hr = (buckets.shape[0] - 1) // 2, (buckets.shape[1] - 1) // 2
+    pair = buckets.long()[delta[..., 0].clamp(-hq, hq) + hq, delta[..., 1].clamp(-hr, hr) + hr]
+    if latents:
+        pair[:, :latents, :] = n_buckets - 1
+        pair[:, :, :latents] = n_buckets - 2
+    return pair
+
+
+@torch.no_grad()
+def _plain_relative(st):
+    q, k, v, bias = (x.float() for x in st["leaves"])
+    p, a, t, d = q.shape
+    n_buckets = bias.shape[1]
+    pair = _pair_buckets(st["coords"], st["buckets"], st["latents"], n_buckets)
+    valid = torch.arange(t, device=q.device) < st["lens"][:, None]
+    live = valid[:, None, :, None]
+    keys = valid[:, None, None, :]
+    scale = 1.0 / math.sqrt(d)
+    s = torch.matmul(q, k.transpose(2, 3).contiguous()) * scale
+    for h in range(a):
+        s[:, h] += bias[h][pair]
+    s = torch.where(keys, s, -math.inf)
+    m = s.amax(3, keepdim=True)
+    m = torch.where(m == -math.inf, 0.0, m)
+    e = torch.exp(s - m)
+    total = e.sum(3, keepdim=True)
+    probs = torch.where(live & (total != 0), e / total, 0.0)
+    del e, s
+    out = torch.matmul(probs, torch.where(live, v, 0.0))
+    lse = torch.where(live, m + torch.log(total), 0.0)[..., 0]
+    dtype = st["leaves"][0].dtype
+    res = {"out": out.to(dtype), "lse": lse}
+    if not st["train"]:
+        return res
+    go = torch.where(live, st["grad"].float(), 0.0)
+    dv = torch.matmul(probs.transpose(2, 3).contiguous(), go)
+    dp = torch.matmul(go, v.transpose(2, 3).contiguous())
+    dp = torch.where(keys, dp, 0.0)
+    ds = probs * (dp - (probs * dp).sum(3, keepdim=True))
+    dq = torch.matmul(ds, torch.where(live, k, 0.0)) * scale
+    dk = torch.matmul(ds.transpose(2, 3).contiguous(), torch.where(live, q, 0.0)) * scale
+    # the bias gradient: the sum of ds over the pairs of each bucket
+    dbias = torch.stack([torch.where((pair == b)[:, None], ds, 0.0).sum((0, 2, 3), dtype=torch.float64)
+                         for b in range(n_buckets)], 1).float()
+    res.update(dq=dq.to(dtype), dk=dk.to(dtype), dv=dv.to(dtype), dbias=dbias)
+    return res
+
+
+def _padded(offsets):
+    """(P, longest) flat index and whether the run reaches it."""
+    lens = offsets[1:] - offsets[:-1]
+    at = torch.arange(int(lens.max()), device=offsets.device)
+    inside = at < lens[:, None]
+    return torch.where(inside, offsets[:-1, None] + at, 0), inside
+
+
+@torch.no_grad()
+def _plain_policy(st):
+    flat, inside = _padded(st["offsets"])
+    raw = st["logits"].float()
+    x = torch.where(inside, raw[flat], -math.inf)
+    m = x.amax(1, keepdim=True)
+    e = torch.exp(x - m)
+    total = e.sum(1, keepdim=True)
+    lse = m + torch.log(total)
+    logp = x - lse
+    probs = e / total
+    entropy = -torch.where(probs > 0, probs * logp, 0.0).sum(1)
+    played = st["moves"] >= 0
+    chosen = torch.where(played, logp.gather(1, st["moves"].clamp(min=0)), 0.0)
+    at = torch.arange(x.shape[1], device=x.device)
+    left, tops, vals = x.clone(), [], []
+    for _ in range(st["top"]):  # the largest left, the lowest index among equals
+        best = left.amax(1, keepdim=True)
+        idx = torch.where((left == best) & (left > -math.inf), at, x.shape[1]).amin(1, keepdim=True)
+        there = idx < x.shape[1]
+        tops.append(torch.where(there, idx, -1))
+        vals.append(torch.where(there, best - lse, -math.inf))
+        left.scatter_(1, idx.clamp(max=x.shape[1] - 1), -math.inf)
+    empty = x.new_empty((x.shape[0], 0))
+    top_moves = torch.cat(tops, 1) if tops else empty.long()
+    res = {"log_probs": chosen, "entropy": entropy, "lse": lse[:, 0],
+           "top_log_probs": torch.cat(vals, 1) if vals else empty, "top_moves": top_moves}
+    if st["train"]:
+        g_log, g_ent, g_lse, g_top = st["grads"]
+        g_log = torch.where(played, g_log, 0.0)
+        g_top = torch.where(top_moves >= 0, g_top, 0.0)
+        common = (g_lse - g_log.sum(1) - g_top.sum(1))[:, None]
+        dx = probs * (common - g_ent[:, None] * torch.where(probs > 0, logp + entropy[:, None], 0.0))
+        dx.scatter_add_(1, st["moves"].clamp(min=0), g_log)
+        dx.scatter_add_(1, top_moves.clamp(min=0), g_top)
+        res["dlogits"] = dx[inside].to(st["logits"].dtype)
+    return res
+
+
+def _mul_hi_lo(a, const):
+    """High and low words of the 32 x 32 bit product, in int64."""
+    lo = (a * const) & 0xFFFFFFFF  # (wraps modulo 2^64: its low words stay)
+    hi = (((a * (const & 0xFFFF)) >> 16) + a * (const >> 16)) >> 16
+    return hi, lo
+
+
+def _random_words(n, rng, salt):
+    """The first n 32-bit words of the stream (Salmon et al. 2011, Philox4x32
+    with ten rounds): element i takes word i % 4 of counter
+    (i / 4 low, i / 4 high, step, salt) under the key of the seed."""
+    mask = 0xFFFFFFFF
+    c0 = torch.arange((n + 3) // 4, device=rng.device)
+    c = [c0 & mask, c0 >> 32, (rng[1] & mask).expand_as(c0), torch.full_like(c0, salt & mask)]
+    k0, k1 = rng[0] & mask, (rng[0] >> 32) & mask
+    for _ in range(10):
+        h0, l0 = _mul_hi_lo(c[0], 0xD2511F53)
+        h1, l1 = _mul_hi_lo(c[2], 0xCD9E8D57)
+        c = [h1 ^ c[1] ^ k0, l1, h0 ^ c[3] ^ k1, l0]
+        k0, k1 = (k0 + 0x9E3779B9) & mask, (k1 + 0xBB67AE85) & mask
+    return torch.stack(c, 1).reshape(-1)[:n]
+
+
+@torch.no_grad()
+def _plain_dropout(st):
+    x, residual, p = st["x"], st["residual"], st["p"]
+    keep = (_random_words(x.numel(), st["rng"], st["salt"]) >= round(p * 2**32)).view(x.shape)
+    y = torch.where(keep, x.float() * (1.0 / (1.0 - p)), 0.0)
+    out = y.to(x.dtype) if residual is None else (residual.float() + y).to(residual.dtype)
+    res = {"out": out}
+    if st["train"]:
+        res["dx"] = torch.where(keep, st["grad"].float() * (1.0 / (1.0 - p)), 0.0).to(x.dtype)
+        if residual is not None:
+            res["dresidual"] = st["grad"]
+    return res
+
+
+_own = {"relative": _own_relative, "policy": _own_policy, "dropout": _own_dropout}
+_plain = {"relative": _plain_relative, "policy": _plain_policy, "dropout": _plain_dropout}
+
+
+# ----------------------------------------------------------------- the definition in float64
+
+
+def exact(case, seed):
+    st = prepare(case, seed)
+    return {"relative": _exact_relative, "policy": _exact_policy, "dropout": _exact_dropout}[st["kind"]](st)
+
+
+def _exact_relative(st):
+    """Position by position and head by head, autograd's gradient of the formula."""
+    q, k, v, bias = (x.detach().double() for x in st["leaves"])
+    p, a, t, d = q.shape
+    names = ["out", "lse"] + (["dq", "dk", "dv", "dbias"] if st["train"] else [])
+    res = {"out": torch.zeros_like(q), "lse": q.new_zeros(p, a, t), "dq": torch.zeros_like(q),
+           "dk": torch.zeros_like(q), "dv": torch.zeros_like(q), "dbias": torch.zeros_like(bias)}
+    half = [(n - 1) // 2 for n in st["buckets"].shape]
+    table = st["buckets"].long()
+    for i, n in enumerate(st["lens"].tolist()):
+        c = st["coords"][i, :n].long()
+        dq = (c[None, :, 0] - c[:, None, 0]).clamp(-half[0], half[0]) + half[0]
+        dr = (c[None, :, 1] - c[:, None, 1]).clamp(-half[1], half[1]) + half[1]
+        pair = table[dq, dr]
+        rows = torch.arange(n, device=q.device)
+        pair = torch.where(rows[:, None] < st["latents"], bias.shape[1] - 1, pair)
+        pair = torch.where(rows[None, :] < st["latents"], bias.shape[1] - 2, pair)
+        flat = pair.reshape(-1)
+        for h in range(a):
+            qq, kk, vv = (x[i, h, :n] for x in (q, k, v))
+            s = qq @ kk.t() / math.sqrt(d) + bias[h].index_select(0, flat).view(n, n)
+            top = s.amax(1, keepdim=True)
+            top = torch.where(top == -math.inf, torch.zeros_like(top), top)
+            w = torch.exp(s - top)
+            z = w.sum(1, keepdim=True)
+            w = torch.where(z > 0, w / z, torch.zeros_like(w))
+            o = w @ vv
+            res["out"][i, h, :n], res["lse"][i, h, :n] = o, (top + torch.log(z))[:, 0]
+            if st["train"]:
+                g = st["grad"][i, h, :n].double()
+                dw = g @ vv.t()
+                ds = w * (dw - (w * dw).sum(1, keepdim=True))
+                res["dv"][i, h, :n] = w.t() @ g
+                res["dq"][i, h, :n] = ds @ kk / math.sqrt(d)
+                res["dk"][i, h, :n] = ds.t() @ qq / math.sqrt(d)
+                res["dbias"][h] += torch.bincount(flat, ds.reshape(-1), minlength=bias.shape[1])
+    return {name: res[name] for name in names}
+
+
+def _exact_policy(st):
+    """Run by run on the host."""
+    logits = st["logits"].detach().double().cpu().numpy()
+    offsets, moves = st["offsets"].cpu().numpy(), st["moves"].cpu().numpy()
+    grads = [g.double().cpu().numpy() for g in st["grads"]]
+    p, k = len(offsets) - 1, st["top"]
+    out = {"log_probs": np.zeros(moves.shape), "entropy": np.zeros(p), "lse": np.zeros(p),
+           "top_log_probs": np.full((p, k), -np.inf), "top_moves": np.full((p, k), -1, np.int64)}
+    d = np.zeros_like(logits)
+    for i in range(p):
+        x = logits[offsets[i]:offsets[i + 1]]
+        top = x.max()
+        lse = top + np.log(np.exp(x - top).sum())
+        logp = x - lse
+        pr = np.exp(logp)
+        out["lse"][i], out["entropy"][i] = lse, -(pr * logp).sum()
+        best = np.argsort(-x, kind="stable")[:k]
+        out["top_moves"][i, :len(best)], out["top_log_probs"][i, :len(best)] = best, logp[best]
+        dx = pr * (grads[2][i] - grads[1][i] * (logp + out["entropy"][i]))
+        for j, move in enumerate(moves[i]):
+            if move >= 0:
+                out["log_probs"][i, j] = logp[move]
+                dx -= grads[0][i, j] * pr
+                dx[move] += grads[0][i, j]
+        for j, move in enumerate(best):
+            dx -= grads[3][i, j] * pr
+            dx[move] += grads[3][i, j]
+        d[offsets[i]:offsets[i + 1]] = dx
+    if st["train"]:
+        out["dlogits"] = d
+    return {name: torch.from_numpy(x) for name, x in out.items()}
+
+
+def _exact_dropout(st):
+    """The generator in unsigned host arithmetic, the sums in float64."""
+    x = st["x"].detach().double().cpu().numpy()
+    seed, step = (int(w) for w in st["rng"].tolist())
+    word = np.uint64(0xFFFFFFFF)
+    n4 = (x.size + 3) // 4
+    a, b = np.arange(n4, dtype=np.uint64), np.zeros(n4, np.uint64)
+    c, e = np.full(n4, step & 0xFFFFFFFF, np.uint64), np.full(n4, st["salt"] & 0xFFFFFFFF, np.uint64)
+    k0, k1 = seed & 0xFFFFFFFF, (seed >> 32) & 0xFFFFFFFF
+    for _ in range(10):
+        first, second = a * np.uint64(0xD2511F53), c * np.uint64(0xCD9E8D57)
+        a, b, c, e = ((second >> np.uint64(32)) ^ b ^ np.uint64(k0), second & word,
+                      (first >> np.uint64(32)) ^ e ^ np.uint64(k1), first & word)
+        k0, k1 = (k0 + 0x9E3779B9) & 0xFFFFFFFF, (k1 + 0xBB67AE85) & 0xFFFFFFFF
+    keep = (np.stack([a, b, c, e], 1).reshape(-1)[:x.size] >= np.uint64(round(st["p"] * 2**32))).reshape(x.shape)
+    out = np.where(keep, x / (1.0 - st["p"]), 0.0)
+    if st["residual"] is not None:
+        out = out + st["residual"].detach().double().cpu().numpy()
+    res = {"out": out}
+    if st["train"]:
+        grad = st["grad"].double().cpu().numpy()
+        res["dx"] = np.where(keep, grad / (1.0 - st["p"]), 0.0)
+        if st["residual"] is not None:
+            res["dresidual"] = grad
+    return {name: torch.from_numpy(y) for name, y in res.items()}
+
+
+# ----------------------------------------------------------------- what a pass cannot do without
+
+
+def work(case):
+    kind, train = case["kind"], case["train"]
+    if kind == "relative":
+        lens = _lengths(case)
+        p, t = case["positions"], int(lens.max())
+        live, pairs = int(lens.sum()), int((lens * lens).sum())
+        row = case["heads"] * case["hd"] * SIZE[case["dtype"]]
+        # live rows of q, k, v in, every row of out, lse; the gradient in and three out
+        nbytes = 3 * live * row + p * t * (row + 4 * case["heads"]) + 8 * live
+        flops = 4 * pairs * case["heads"] * case["hd"]
+        if train:
+            nbytes += live * row + 3 * p * t * row
+            flops += 10 * pairs * case["heads"] * case["hd"]
+        return {"bytes": nbytes, "flops": flops}
+    if kind == "policy":
+        n, p = int(_lengths(case).sum()), case["positions"]
+        small = p * (8 + 8 * case["moves"] + 4 * case["moves"] + 8 + 12 * case["top"])
+        if train:
+            small += p * (4 * case["moves"] + 8 + 4 * case["top"])
+        return {"bytes": n * SIZE[case["dtype"]] * (2 if train else 1) + small, "flops": n * (12 if train else 6)}
+    n = case["rows"] * case["width"]
+    res = SIZE[case["residual"]] if case["residual"] else 0
+    out = res or SIZE[case["x"]]
+    # (the residual's gradient is the incoming one)
+    return {"bytes": n * (SIZE[case["x"]] + res + out + (out + SIZE[case["x"]] if train else 0)), "flops": 3 * n}
