@@ -182,8 +182,8 @@ def _own_relative(st):
     import mantisnet
 
     q, k, v, bias = st["leaves"]
-    out, lse = torch.ops.mantisnet.fused_attention_relative(q, k, v, bias, st["coords"], st["buckets"], st["lens"],
-                                                            st["latents"])
+    out, lse, _stats = torch.ops.mantisnet.fused_attention_relative(q, k, v, bias, st["coords"], st["buckets"],
+                                                                    st["lens"], st["latents"])
     if not st["train"]:
         return {"out": out, "lse": lse}
     grads = torch.autograd.grad(out, st["leaves"], st["grad"])
