@@ -1,0 +1,364 @@
+// Ragged attention with a learned bias by relative position, on 16-bit MFMA
+// for gfx950.  For the live rows i and keys j < L of a position and head:
+//   s_ij = q_i . k_j / sqrt(hd) + bias[bucket(i, j)],  out_i = softmax_j(s_ij) v_j,
+//   lse_i = log sum_j exp s_ij
+// A live row whose every key has bias -inf gives zeros and lse -inf; rows past L
+// give zeros and lse 0.
+//
+// One workgroup serves an item (position, head, query tile of 4 kSub 16 rows); each
+// of its four wavefronts owns kSub 16-query sub-tiles and the keys stream
+// through LDS in 64-key chunks, double-buffered, the next one's rows in
+// registers meanwhile.  The transposed products S^T = K Q^T and O^T += V^T P^T keep a
+// lane on one query, and a score fragment is the next product's B operand as it
+// stands.  The bias is the score product's C operand (relative_bias.hpp), so
+// adding it costs the lookup alone.
+//
+// Softmax: p = exp2(c (s - m)), c = log2(e) / sqrt(hd), over the raw scores
+// (bias * sqrt(hd) included), in fp32 and with the difference first, so a row
+// of scores at the type's lowest value is still uniform; m moves only when a
+// score passes it by more than 8 in log2 units.  The probabilities enter the value product rounded to
+// 16 bits (relative 2^-9 or 2^-12 of each, as their output rounds once more);
+// the output is divided by the sum of the rounded ones, so a row of one key
+// is that key's value, and lse is the log of the unrounded fp32 sum.
+#include <type_traits>
+
+#include "mfma.hpp"
+#include "relative_bias.hpp"
+
+namespace mantis {
+namespace {
+
+constexpr int kWaves = 4;
+constexpr int kKChunk = 64;
+constexpr int kVtPitch = kKChunk + 8;  // 16-bit elements per staged V^T row
+constexpr float kLazyLog2 = 8.f;       // probabilities up to 2^8 before the reference point moves
+constexpr int kXcds = 8;
+
+struct Operand {  // (P, A, T, hd): base and element strides
+  const uint16_t* p;
+  int64_t sp, sa, st;
+};
+
+template <bool kHalf, int HD, int kSub>
+__global__ void __launch_bounds__(256)
+relative_attention_kernel(Operand q, Operand k, Operand v, Relative rel, const int32_t* __restrict__ seq_lens,
+                          int heads, int64_t T, uint16_t* __restrict__ out, int64_t osp, int64_t osa, int64_t ost,
+                          float* __restrict__ lse, float2* __restrict__ stats, float c_log2, float root_hd, int64_t n_items) {
+  constexpr int kQTile = kWaves * 16 * kSub;
+  constexpr int kKPitch = HD + 8;              // 16-bit elements per staged K row
+  constexpr int kKs = HD < 32 ? 1 : HD / 32;   // K steps of the score product
+  constexpr int kDt = HD / 16;                 // 16-dim output tiles
+  constexpr int kPieces = kKChunk * HD / 8;    // 16-byte pieces of a chunk's K (or V) rows
+  constexpr int kPer = kPieces < 256 ? 1 : kPieces / 256;
+  extern __shared__ float table[];  // the head's bias per displacement
+  __shared__ __attribute__((aligned(16))) uint16_t sk[2][kKChunk * kKPitch];
+  __shared__ __attribute__((aligned(16))) uint16_t svt[2][HD * kVtPitch];
+  __shared__ __attribute__((aligned(16))) uint32_t sc[2][kKChunk];
+  // consecutive items on one XCD share the position's rows in its L2 (the
+  // grid is a multiple of kXcds, workgroups go round-robin over the XCDs)
+  const int64_t item = int64_t(blockIdx.x % kXcds) * (gridDim.x / kXcds) + blockIdx.x / kXcds;
+  if (item >= n_items) return;
+  const int64_t n_qt = (T + kQTile - 1) / kQTile;
+  const int64_t pa = item / n_qt, qt = item % n_qt;
+  const int64_t p = pa / heads, a = pa % heads;
+  int64_t L = seq_lens[p];
+  L = L < 0 ? 0 : (L > T ? T : L);
+  const int64_t q0 = qt * kQTile;
+  uint16_t* op = out + p * osp + a * osa;
+  float* lp = lse + (p * heads + a) * T;
+  float2* sp = stats + (p * heads + a) * T;
+
+  if (q0 >= L) {  // a tile past the live rows
+    for (int i = threadIdx.x; i < kQTile * (HD / 8); i += 256) {
+      const int64_t row = q0 + i / (HD / 8);
+      const int c = (i % (HD / 8)) * 8;
+      if (row < T) {
+        *reinterpret_cast<uint4*>(op + row * ost + c) = make_uint4(0u, 0u, 0u, 0u);
+        if (c == 0) {
+          lp[row] = 0.f;
+          sp[row] = make_float2(0.f, INFINITY);
+        }
+      }
+    }
+    return;
+  }
+
+  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+  const int l16 = lane % 16, g = lane / 16;
+  using FR = Frag<kHalf>;
+  // rows through buffer descriptors over the live rows: one at or past L reads
+  // zeros without a memory access
+  const i32x4_t qrs = rows_rsrc(q.p + p * q.sp + a * q.sa, uint32_t(q.st * 2), uint32_t(L));
+  const i32x4_t krs = rows_rsrc(k.p + p * k.sp + a * k.sa, uint32_t(k.st * 2), uint32_t(L));
+  const i32x4_t vrs = rows_rsrc(v.p + p * v.sp + a * v.sa, uint32_t(v.st * 2), uint32_t(L));
+  // the K slots of a score step: dims 32 ks + 8 g .. +7 (HD = 16: lanes g >= 2 hold zeros on both sides)
+  auto kdim = [&](int ks) { return HD < 32 ? 8 * (g & 1) : 32 * ks + 8 * g; };
+  const bool upper = HD < 32 && g >= 2;
+  typename FR::vec qf[kSub][kKs];
+  int64_t qrow[kSub];
+#pragma unroll
+  for (int j = 0; j < kSub; ++j) {
+    qrow[j] = q0 + (wave * kSub + j) * 16 + l16;
+#pragma unroll
+    for (int ks = 0; ks < kKs; ++ks) {
+      uint4 u = row_load16(qrs, int32_t(qrow[j]), 2 * kdim(ks));
+      if (upper) u = make_uint4(0u, 0u, 0u, 0u);
+      qf[j][ks] = FR::cast(u);
+    }
+  }
+
+  // staging role of this thread: kPer 16-byte pieces of the chunk's K and V rows, a row's coordinates
+  const bool stager = int(threadIdx.x) < kPieces;
+  uint4 kreg[kPer], vreg[kPer];
+  uint32_t creg = 0u;
+  auto fetch = [&](int64_t kb) {
+#pragma unroll
+    for (int r = 0; r < kPer; ++r) {
+      const int i = int(threadIdx.x) + 256 * r;
+      const int32_t row = stager ? int32_t(kb) + i / (HD / 8) : -1;
+      kreg[r] = row_load16(krs, row, 16 * (i % (HD / 8)));
+      vreg[r] = row_load16(vrs, row, 16 * (i % (HD / 8)));
+    }
+    if (threadIdx.x < kKChunk) creg = coords_of(rel, p, T, kb + threadIdx.x, L);
+  };
+  auto stage = [&](int buf) {
+    if (threadIdx.x < kKChunk) sc[buf][threadIdx.x] = creg;
+    if (!stager) return;
+#pragma unroll
+    for (int r = 0; r < kPer; ++r) {
+      const int i = int(threadIdx.x) + 256 * r;
+      const int st_key = i / (HD / 8), st_d = 8 * (i % (HD / 8));
+      *reinterpret_cast<uint4*>(&sk[buf][st_key * kKPitch + st_d]) = kreg[r];
+      const uint32_t w[4] = {vreg[r].x, vreg[r].y, vreg[r].z, vreg[r].w};
+      uint16_t* col = &svt[buf][st_d * kVtPitch + st_key];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        col[(2 * e) * kVtPitch] = uint16_t(w[e] & 0xffffu);
+        col[(2 * e + 1) * kVtPitch] = uint16_t(w[e] >> 16);
+      }
+    }
+  };
+  fetch(0);
+  uint32_t qc[kSub];
+#pragma unroll
+  for (int j = 0; j < kSub; ++j) qc[j] = coords_of(rel, p, T, qrow[j], L);
+  stage_bias(rel, a, root_hd, table);
+  Side<true> side[kSub] = {Side<true>(rel, qc[0], qrow[0] < rel.n_latents),
+                           Side<true>(rel, qc[kSub - 1], qrow[kSub - 1] < rel.n_latents)};
+
+  // per sub-tile: the exponent's reference point (raw-score units), O^T tiles,
+  // the rounded probabilities' sum (a product with an all-ones A operand, every
+  // row of it) and this lane's share of the unrounded sum
+  float m[kSub], thr[kSub], lreal[kSub];
+  const float lazy_raw = kLazyLog2 / c_log2;
+  f32x4_t o[kSub][kDt], lsum[kSub];
+#pragma unroll
+  for (int j = 0; j < kSub; ++j) {
+    m[j] = thr[j] = -INFINITY;
+    lreal[j] = 0.f;
+    lsum[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int dt = 0; dt < kDt; ++dt) o[j][dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
+  const uint32_t one2 = FR::pack_unit(1.f, 1.f);
+  const typename FR::vec ones = FR::cast(make_uint4(one2, one2, one2, one2));
+
+  // one chunk for the first kNJ sub-tiles (those with a live query)
+  auto chunk = [&](auto nj, auto masked, int buf, int64_t kb, bool more) {
+    constexpr int kNJ = decltype(nj)::value;
+    if (more) fetch(kb + kKChunk);
+    if constexpr (kNJ > 0) {
+      f32x4_t s[kNJ][4];
+#pragma unroll
+      for (int tt = 0; tt < 4; ++tt) {
+        const uint4 kc = *reinterpret_cast<const uint4*>(&sc[buf][16 * tt + 4 * g]);
+        const uint32_t kcs[4] = {kc.x, kc.y, kc.z, kc.w};
+#pragma unroll
+        for (int j = 0; j < kNJ; ++j)
+#pragma unroll
+          for (int t = 0; t < 4; ++t) s[j][tt][t] = entry(table, side[j].at(kcs[t]));
+      }
+      if (kb < rel.n_latents) {  // uniform
+        const int64_t lat = rel.n_latents - kb - 4 * g;
+        const float b = entry(table, side[0].latent_other);
+#pragma unroll
+        for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int j = 0; j < kNJ; ++j) s[j][tt][t] = 16 * tt + t < lat ? b : s[j][tt][t];
+      }
+      if constexpr (decltype(masked)::value) {
+        const int lim = int(L - kb) - 4 * g;
+#pragma unroll
+        for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int j = 0; j < kNJ; ++j) s[j][tt][t] = 16 * tt + t < lim ? s[j][tt][t] : -INFINITY;
+      }
+#pragma unroll
+      for (int tt = 0; tt < 4; ++tt) {
+#pragma unroll
+        for (int ks = 0; ks < kKs; ++ks) {
+          uint4 ku = *reinterpret_cast<const uint4*>(&sk[buf][(16 * tt + l16) * kKPitch + kdim(ks)]);
+          if (upper) ku = make_uint4(0u, 0u, 0u, 0u);
+          const typename FR::vec kf = FR::cast(ku);
+#pragma unroll
+          for (int j = 0; j < kNJ; ++j) s[j][tt] = mfma16x16x32(kf, qf[j][ks], s[j][tt]);
+        }
+      }
+      typename FR::vec pf[kNJ][2];
+#pragma unroll
+      for (int j = 0; j < kNJ; ++j) {
+        float lmax = s[j][0][0];
+#pragma unroll
+        for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+          for (int t = 0; t < 4; ++t) lmax = fmaxf(lmax, s[j][tt][t]);
+        if (__builtin_amdgcn_ballot_w64(lmax > thr[j])) {  // wavefront-uniform
+          const float cmax = max_xor32(max_xor16(fmaxf(m[j], lmax)));
+          // (a row without a finite score keeps m = -inf and its zero sums)
+          const float alpha = m[j] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m[j] - cmax) * c_log2);
+          m[j] = cmax;
+          thr[j] = cmax + lazy_raw;
+          lreal[j] *= alpha;
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            lsum[j][t] *= alpha;
+#pragma unroll
+            for (int dt = 0; dt < kDt; ++dt) o[j][dt][t] *= alpha;
+          }
+        }
+        const float m0 = m[j] == -INFINITY ? 0.f : m[j];
+        uint32_t pw[4][2];
+#pragma unroll
+        for (int tt = 0; tt < 4; ++tt) {
+          float pr[4];
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            pr[t] = __builtin_amdgcn_exp2f((s[j][tt][t] - m0) * c_log2);
+            lreal[j] += pr[t];
+          }
+          pw[tt][0] = FR::pack_unit(pr[0], pr[1]);
+          pw[tt][1] = FR::pack_unit(pr[2], pr[3]);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          pf[j][h] = FR::cast(make_uint4(pw[2 * h][0], pw[2 * h][1], pw[2 * h + 1][0], pw[2 * h + 1][1]));
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int dt = 0; dt < kDt; ++dt) {
+          const uint16_t* row = &svt[buf][(16 * dt + l16) * kVtPitch + 32 * h];
+          const uint2 lo = *reinterpret_cast<const uint2*>(row + 4 * g);
+          const uint2 hi = *reinterpret_cast<const uint2*>(row + 16 + 4 * g);
+          const typename FR::vec vf = FR::cast(make_uint4(lo.x, lo.y, hi.x, hi.y));
+#pragma unroll
+          for (int j = 0; j < kNJ; ++j) o[j][dt] = mfma16x16x32(vf, pf[j][h], o[j][dt]);
+        }
+#pragma unroll
+        for (int j = 0; j < kNJ; ++j) lsum[j] = mfma16x16x32(ones, pf[j][h], lsum[j]);
+      }
+    }
+    if (more) stage(buf ^ 1);
+    __syncthreads();
+  };
+
+  const int64_t n_chunks = (L + kKChunk - 1) / kKChunk;
+  auto run = [&](auto nj) {
+    constexpr std::true_type yes{};
+    constexpr std::false_type no{};
+    const int64_t last = n_chunks - 1;  // only the last chunk can hold padding keys
+    for (int64_t ch = 0; ch < last; ++ch) chunk(nj, no, int(ch & 1), ch * kKChunk, true);
+    chunk(nj, yes, int(last & 1), last * kKChunk, false);
+  };
+  stage(0);
+  __syncthreads();
+  const int64_t live_q = L - (q0 + wave * 16 * kSub);  // (wavefront-uniform)
+  if (live_q > 16 && kSub > 1) run(std::integral_constant<int, kSub>{});
+  else if (live_q > 0) run(std::integral_constant<int, 1>{});
+  else run(std::integral_constant<int, 0>{});
+#pragma unroll
+  for (int j = 0; j < kSub; ++j) {
+    const float lt = lsum[j][0], lr = sum_xor32(sum_xor16(lreal[j]));
+    if (qrow[j] < T) {
+      const bool live = qrow[j] < L;
+      const float inv = live && lt != 0.f ? 1.f / lt : 0.f;
+#pragma unroll
+      for (int dt = 0; dt < kDt; ++dt) {
+        uint2 w = make_uint2(0u, 0u);
+        if (live) {
+          w.x = FR::pack_unit(o[j][dt][0] * inv, o[j][dt][1] * inv);
+          w.y = FR::pack_unit(o[j][dt][2] * inv, o[j][dt][3] * inv);
+        }
+        *reinterpret_cast<uint2*>(op + qrow[j] * ost + 16 * dt + 4 * g) = w;
+      }
+      if (g == 0) {
+        const float m0 = m[j] == -INFINITY ? 0.f : m[j], log2l = log2f(lr);  // (an empty row's sum is 0)
+        // (a row of scores at the lowest finite value has that as its lse)
+        lp[qrow[j]] = !live ? 0.f : fabsf(m0) == kLargest ? m0 : fmaf(m0, 1.f / root_hd, log2l * 0.6931471805599453f);
+        sp[qrow[j]] = live && lr != 0.f ? make_float2(m0, log2l) : make_float2(0.f, INFINITY);
+      }
+    }
+  }
+}
+
+template <bool kHalf, int HD, int kSub>
+int32_t launch(const Operand& q, const Operand& k, const Operand& v, const Relative& rel, const int32_t* seq_lens,
+               int64_t n_pos, int heads, int64_t t, uint16_t* out, const int64_t* os, float* lse, float2* stats, hipStream_t st) {
+  constexpr int kQTile = kWaves * 16 * kSub;
+  const int64_t n_items = n_pos * heads * ((t + kQTile - 1) / kQTile);
+  const int64_t grid = (n_items + kXcds - 1) / kXcds * kXcds;
+  if (grid > 2147483647LL) return MANTIS_E_ARG;
+  const size_t lds = size_t(rel.nq * rel.nr + 2) * sizeof(float);
+  const float root = sqrtf(float(HD));
+  relative_attention_kernel<kHalf, HD, kSub><<<unsigned(grid), 256, lds, st>>>(
+      q, k, v, rel, seq_lens, heads, t, out, os[0], os[1], os[2], lse, stats, 1.4426950408889634f / root, root, n_items);
+  return launched();
+}
+
+}  // namespace
+}  // namespace mantis
+
+using namespace mantis;
+
+extern "C" int32_t mantis_relative_attention(const void* q, const int64_t* qs, const void* k, const int64_t* ks,
+                                             const void* v, const int64_t* vs, int32_t dtype, const float* bias,
+                                             int64_t n_buckets, const int32_t* coords, const int32_t* buckets,
+                                             int64_t nq, int64_t nr, int64_t n_latents, const int32_t* seq_lens,
+                                             int64_t n_pos, int32_t heads, int64_t t, int32_t hd, void* out,
+                                             const int64_t* os, float* lse, float* stats, int32_t* err_flag,
+                                             void* stream) {
+  if (n_pos == 0 || t == 0) return MANTIS_OK;
+  if (!q || !k || !v || !out || !lse || !stats || !seq_lens || !qs || !ks || !vs || !os) return MANTIS_E_ARG;
+  if ((hd != 16 && hd != 32 && hd != 64) || heads <= 0 || n_pos < 0 || t < 0 || t > 2147483647LL) return MANTIS_E_ARG;
+  if (dtype != MANTIS_BF16 && dtype != MANTIS_F16) return MANTIS_E_ARG;
+  if (nq > kMaxDisplacements || nr > kMaxDisplacements || n_buckets > kMaxBuckets) return MANTIS_E_ARG;
+  for (const int64_t* st : {qs, ks, vs, os}) {
+    if (st[3] != 1) return MANTIS_E_ARG;
+    if ((st[0] | st[1] | st[2]) % 8) return MANTIS_E_ARG;
+  }
+  // a position's q, k and v rows are read through buffer descriptors: a row
+  // pitch of hd to 8,191 elements and 32-bit byte offsets
+  for (const int64_t* st : {qs, ks, vs})
+    if (st[2] < hd || st[2] >= 8192 || t * st[2] * 2 > 2147483647LL) return MANTIS_E_ARG;
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !aligned16(stats)) return MANTIS_E_ARG;
+  const Relative rel{coords, buckets, bias, int(nq), int(nr), int(n_buckets), n_latents, err_flag};
+  if (!good_relative(rel, t)) return MANTIS_E_ARG;
+  auto operand = [](const void* ptr, const int64_t* st) {
+    return Operand{static_cast<const uint16_t*>(ptr), st[0], st[1], st[2]};
+  };
+  const Operand Q = operand(q, qs), K = operand(k, ks), V = operand(v, vs);
+  uint16_t* o = static_cast<uint16_t*>(out);
+  float2* sp = reinterpret_cast<float2*>(stats);
+  hipStream_t st = as_stream(stream);
+#define MANTIS_FWD(HD_)                                                                                     \
+  return dtype == MANTIS_F16 ? launch<true, HD_, 2>(Q, K, V, rel, seq_lens, n_pos, heads, t, o, os, lse, sp, st) \
+                             : launch<false, HD_, 2>(Q, K, V, rel, seq_lens, n_pos, heads, t, o, os, lse, sp, st)
+  if (hd == 16) MANTIS_FWD(16);
+  if (hd == 32) MANTIS_FWD(32);
+  MANTIS_FWD(64);
+#undef MANTIS_FWD
+}

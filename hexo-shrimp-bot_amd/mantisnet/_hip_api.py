@@ -148,6 +148,16 @@ SIGNATURES = {
     "mantis_stone_attention": ([vp, vp, vp, vp, vp, vp, i32, vp, i64, i32, i64, i32, vp, vp, vp, vp, vp], i32),
     "mantis_stone_attention_backward": ([vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, i32, vp, i64, i32, i64, i32, vp,
                                          vp, vp, vp, vp, vp, vp, vp], i32),
+    "mantis_relative_attention": ([vp, vp, vp, vp, vp, vp, i32, vp, i64, vp, vp, i64, i64, i64, vp, i64, i32, i64, i32,
+                                   vp, vp, vp, vp, vp, vp], i32),
+    "mantis_relative_attention_backward_workspace": ([i64, i32, i64, i64], i64),
+    "mantis_relative_attention_backward": ([vp, vp, vp, vp, vp, vp, vp, vp, vp, i32, vp, i64, vp, vp, i64, i64, i64, vp,
+                                            i64, i32, i64, i32, vp, i64, vp, vp, vp, vp, vp, vp, vp, vp, vp], i32),
+    "mantis_policy_log_probs_workspace": ([i64, i64, i32], i64),
+    "mantis_policy_log_probs": ([vp, i32, i64, vp, i64, i64, vp, i64, i32, vp, vp, vp, vp, vp, vp, vp, i64, vp, vp], i32),
+    "mantis_policy_log_probs_backward": ([vp, i32, i64, vp, i64, i64, vp, i64, i32, vp, vp, vp, vp, vp, vp, vp, vp, vp,
+                                          vp], i32),
+    "mantis_residual_dropout": ([vp, i32, vp, vp, i64, ctypes.c_double, i64, vp, i32, vp], i32),
     "mantis_latent_attend": ([vp, i32, i64, vp, i64, i64, vp, vp], i32),
     "mantis_stone_attention_schedule_len": ([i64, i32, i64], i64),
     "mantis_stone_attention_schedule": ([vp, i64, i32, i64, vp, vp], i32),

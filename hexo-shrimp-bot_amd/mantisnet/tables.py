@@ -144,3 +144,21 @@ def window_latent_layout(window_pos: Tensor, positions: int) -> tuple[Tensor, Te
     _check_range(window_pos, positions, "window_pos")
     order = _stable_order(window_pos)
     return ops.runs_to_ptr(window_pos.index_select(0, order), positions), order
+
+
+def relative_buckets(reach: int) -> tuple[Tensor, int]:
+    """(buckets, count) of the relative attention over hexagonal coordinates:
+    buckets (2 reach + 3, 2 reach + 3) int32 by the displacement (dq, dr) of
+    two stones, on the CPU, and the number of buckets with the latents' two.
+    Bucket 0 is the same cell, 1 .. reach a displacement along an axis by its
+    distance, reach + 2 .. 2 reach one off the axes (reach + distance; distance
+    1 is always on an axis, so reach + 1 stays unused), 2 reach + 1 everything
+    further than the reach; 2 reach + 2 and 2 reach + 3 are the latents'."""
+    if not 1 <= reach <= 30:
+        raise ValueError(f"reach must lie in [1, 30], got {reach}")
+    d = torch.arange(-reach - 1, reach + 2, dtype=torch.int32)
+    dq, dr = d[:, None], d[None, :]
+    dist = torch.maximum(torch.maximum(dq.abs(), dr.abs()), (dq + dr).abs())
+    on_axis = (dq == 0) | (dr == 0) | (dq + dr == 0)
+    near = torch.where(on_axis, dist, reach + dist)
+    return torch.where(dist > reach, 2 * reach + 1, near).to(torch.int32), 2 * reach + 4

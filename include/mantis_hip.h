@@ -7,7 +7,8 @@
  *    (NULL = the default stream); work is enqueued on that stream only;
  *  - tensors are dense row-major; index and CSR-pointer arrays are int64;
  *  - `dtype` arguments take MANTIS_F32, MANTIS_BF16 or MANTIS_F16 (fp16
- *    narrowing rounds to nearest even and saturates at +-65504);
+ *    narrowing rounds to nearest even and saturates at +-65504, unless an entry
+ *    point says that it overflows);
  *  - CSR pointer arrays are clamped into [0, n_entries] on the device, so a
  *    corrupted pointer can only shorten a run, never leave the entry arrays;
  *  - every index is bounds-checked on the device: an out-of-range index is
@@ -823,6 +824,52 @@ int32_t mantis_stone_attention_backward(const void* q, const int64_t* q_strides,
                                         void* stream);
 
 /*
+ * Ragged attention with a learned bias by the pair's relative position (no
+ * counterpart in the reference, which reads a batch's stone coordinates
+ * nowhere):
+ *   s_ij = q_i . k_j / sqrt(hd) + bias[a, bucket(i, j)],  j < seq_lens[p]
+ *   out_i = softmax_j(s_ij) v_j,  lse_i = log sum_j exp s_ij
+ * bucket(i, j) = n_buckets - 2 if j < n_latents, else n_buckets - 1 if
+ * i < n_latents, else buckets[clamp(coords_j - coords_i)]: `buckets` (nq, nr)
+ * int32, both odd, nq * nr <= 4096, its middle entry the zero displacement,
+ * indexed by the displacement's two components clamped to +-(nq - 1) / 2 and
+ * +-(nr - 1) / 2.  bias (heads, n_buckets) fp32, n_buckets <= 384; coords
+ * (P, T, 2) int32 within int16 (latent and pad rows unread).  A bias may be
+ * -inf: a live row all of whose keys have it gives zeros and lse -inf (a finite
+ * bias past 3.4e38 / sqrt(hd) counts as the lowest or largest finite score).  Rows at
+ * or past seq_lens[p] give zeros and lse 0.  A bucket outside [0, n_buckets)
+ * counts as bias 0 without a gradient and, as a coordinate outside int16, sets
+ * MANTIS_FLAG_INDEX.  q/k/v/out as in mantis_stone_attention (a position's
+ * rows within 2^31 bytes), fp16 outputs past +-65504 infinite; lse
+ * (P, heads, T) and stats (P, heads, T, 2) fp32, the latter what the backward
+ * reads (the row's reference score and the log2 of its sum).
+ */
+int32_t mantis_relative_attention(const void* q, const int64_t* q_strides, const void* k,
+                                  const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                                  int32_t dtype, const float* bias, int64_t n_buckets, const int32_t* coords,
+                                  const int32_t* buckets, int64_t nq, int64_t nr, int64_t n_latents,
+                                  const int32_t* seq_lens, int64_t n_pos, int32_t heads, int64_t t, int32_t hd,
+                                  void* out, const int64_t* out_strides, float* lse, float* stats,
+                                  int32_t* err_flag, void* stream);
+
+/*
+ * Backward of mantis_relative_attention for the same inputs, given its stats
+ * and grad_out (dtype and shape of q): dq, dk and dv in `dtype` (fp16 past
+ * +-65504 infinite), dbias (heads, n_buckets) fp32, the sum of the score
+ * gradients over the pairs of each bucket.  fp32 sums in a fixed order (two
+ * calls agree bitwise); rows and keys at or past seq_lens[p] get zeros.
+ * workspace: mantis_relative_attention_backward_workspace bytes, 16-byte aligned.
+ */
+int64_t mantis_relative_attention_backward_workspace(int64_t n_pos, int32_t heads, int64_t t, int64_t n_buckets);
+int32_t mantis_relative_attention_backward(
+    const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+    const int64_t* v_strides, const void* grad_out, const int64_t* grad_out_strides, const float* stats,
+    int32_t dtype, const float* bias, int64_t n_buckets, const int32_t* coords, const int32_t* buckets, int64_t nq,
+    int64_t nr, int64_t n_latents, const int32_t* seq_lens, int64_t n_pos, int32_t heads, int64_t t, int32_t hd,
+    void* workspace, int64_t workspace_bytes, void* dq, const int64_t* dq_strides, void* dk,
+    const int64_t* dk_strides, void* dv, const int64_t* dv_strides, float* dbias, int32_t* err_flag, void* stream);
+
+/*
  * Work order for mantis_stone_attention over these seq_lens: its items
  * (position, head, 128-query tile) by key-chunk count descending, tiles past
  * each live prefix last, written to `schedule` (a device array of
@@ -1184,6 +1231,64 @@ int64_t mantis_leaf_workspace(const mantis_leaf_batch* batch, int64_t n_blocks);
 int32_t mantis_leaf_forward(const mantis_leaf_model* model, const mantis_leaf_batch* batch,
                             const mantis_leaf_out* out, float mass_floor, void* workspace, int64_t workspace_bytes,
                             int32_t* noncanonical, int32_t* err_flag, uint32_t* tile_counters, void* stream);
+
+/*
+ * Log probabilities of chosen moves, entropy and best alternatives of every
+ * position's policy, over its run of logits [offsets[p], offsets[p + 1]) (the
+ * legal rows; no counterpart in the reference, whose policy loss composes
+ * torch operations).  logits: n entries of `dtype` (MANTIS_F32, MANTIS_F16 or
+ * MANTIS_BF16), `stride` elements apart (a column of rows).  moves
+ * (P, n_moves) int64: indices within the run, -1 for none (n_moves <= 1024);
+ * top <= 64.  All fp32:
+ *   lse[p] = log sum exp x,  log_probs[p, g] = x[moves[p, g]] - lse[p] (0 for -1),
+ *   entropy[p] = -sum softmax(x) log softmax(x),
+ *   top_moves[p, k] / top_log_probs[p, k] = the run's entries by x descending,
+ *   then index ascending, among those above -inf (-1 and -inf past them),
+ *   norm[p] = (maximum of x, log sum exp(x - maximum)), what the backward reads.
+ * A run that is empty or -inf throughout: lse -inf, entropy 0, log_probs -inf,
+ * no alternatives; one that holds a NaN or +inf: NaN, no alternatives.  A move
+ * outside [-1, run) sets MANTIS_FLAG_INDEX and counts as -1; offsets that
+ * descend, leave [0, n] or span 2^31 entries set MANTIS_FLAG_ORDER and count
+ * as an empty run.  workspace: mantis_policy_log_probs_workspace bytes (0: NULL).
+ */
+int64_t mantis_policy_log_probs_workspace(int64_t n_pos, int64_t n, int32_t top);
+int32_t mantis_policy_log_probs(const void* logits, int32_t dtype, int64_t stride, const int64_t* offsets,
+                                int64_t n_pos, int64_t n, const int64_t* moves, int64_t n_moves, int32_t top,
+                                float* log_probs, float* entropy, float* lse, float* top_log_probs,
+                                int64_t* top_moves, float* norm, void* workspace, int64_t workspace_bytes,
+                                int32_t* err_flag, void* stream);
+
+/*
+ * Its gradient, from the gradients of log_probs, entropy, lse and
+ * top_log_probs (each fp32 or NULL: zero):
+ *   grad_logits_i = p_i (g_lse - sum_g G_g - sum_k K_k - g_entropy (log p_i + entropy))
+ *                   + the G_g with moves[g] = i + the K_k with top_moves[k] = i
+ * n dense entries of `dtype` (rounded once; an fp16 overflow is infinite);
+ * zeros for runs without a weight and for entries outside every run.  The
+ * order of the sums is fixed.
+ */
+int32_t mantis_policy_log_probs_backward(const void* logits, int32_t dtype, int64_t stride, const int64_t* offsets,
+                                         int64_t n_pos, int64_t n, const int64_t* moves, int64_t n_moves,
+                                         int32_t top, const int64_t* top_moves, const float* entropy,
+                                         const float* norm, const float* grad_log_probs, const float* grad_entropy,
+                                         const float* grad_lse, const float* grad_top, void* grad_logits,
+                                         int32_t* err_flag, void* stream);
+
+/*
+ * Dropout of a residual branch (the trunk blocks' x + drop(f(x)),
+ * python/mantisnet/mantisnet/model.py:263-380) with a mask that is drawn in
+ * place and never stored:
+ *   out[i] = residual[i] + (w_i >= round(p 2^32) ? x[i] / (1 - p) : 0)
+ * with residual of out_dtype, or NULL for 0.  w_i is word i % 4 of Philox4x32
+ * with ten rounds (Salmon et al. 2011) at the counter (i / 4 low, i / 4 high,
+ * step, salt) under the key seed, rng = (seed, step) two int64 on the device
+ * (step modulo 2^32), salt in [0, 2^32).  p in [0, 1]; 1 drops everything.
+ * x, residual and out hold n dense entries of MANTIS_F32, MANTIS_F16 or
+ * MANTIS_BF16.  With the incoming gradient as x and no residual it is its own
+ * backward.
+ */
+int32_t mantis_residual_dropout(const void* x, int32_t x_dtype, const void* residual, const int64_t* rng, int64_t n,
+                                double p, int64_t salt, void* out, int32_t out_dtype, void* stream);
 
 #ifdef __cplusplus
 }
