@@ -7,23 +7,32 @@
 //   dv_j = sum_i p_ij go_i,  dbias[a, b] = sum of ds_ij over the pairs of bucket b.
 //
 // Two passes, each a workgroup per (position, head, 64 rows), 16 rows per
-// wavefront, the other side's rows in 64-row chunks through LDS:
+// wavefront, the other side's rows in 64-row chunks through LDS, two buffers:
 //   query-major  S^T = K Q^T and dP^T = V dO^T, then dQ^T += K^T dS^T and the buckets' sums
 //   key-major    S = Q K^T and dP = dO V^T, then dV^T += dO^T P, dK^T += Q^T dS
+// Both keep a lane on one row of its own side, so a score fragment is the next
+// product's B operand as it stands, and read the transposed A operand from the
+// same row-major LDS rows (the transposing 64-bit LDS read of gfx950).
 // The query pass goes over the keys twice: delta first, from the fp32 products
 // (the 16-bit output's rounding would stay in every ds of its row, and in the
-// bias gradient's long sums), then ds; the rows of one chunk stay in
-// registers and LDS in between.
+// bias gradient's long sums), then ds.  Up to two chunks of keys stay in LDS in
+// between, and their p and dp in registers.
+//
+// Precision: scores and dp are exact products of 16-bit rows summed in fp32.
+// The probabilities and ds enter their products as two 16-bit parts, hi + lo:
+// bf16 beside bf16 rows (16 significant bits), beside fp16 rows fp16 parts of the
+// value times a power of two that follows the largest of its column (22
+// bits of that one).  What is cut is 2^-17 of a term, under the 2^-9 or 2^-12
+// that the outputs round.  (fp32 MFMAs with widened rows: MEASURED.)
 //
 // The bias gradient: every lane adds its ds to its own column of the
 // workgroup's LDS table (a row of 64 lanes per bucket and wavefront: no two
-// lanes meet, no bank is asked twice), or, where that table does not fit, the
-// four lane groups in turn to 16 columns.  The columns join in a fixed order into the
-// workgroup's partial sums, those of a head in a second launch.  Every sum is
-// fp32 in a fixed order: two calls agree bitwise.
-//
-// The probabilities and ds are fp32 and enter their products, with the rows
-// widened, as fp32 MFMA operands.
+// lanes meet, no bank is asked twice), four entries read, added and written
+// at a time; where that table does not fit, the four lane groups in turn to 16
+// columns.  (LDS float atomics instead: 2.5 cycles per lane, half of the whole
+// pass.)  The columns join in a fixed order into the workgroup's partial sums, those
+// of a head in a second launch.  Every sum is fp32 in a fixed order: two calls
+// agree bitwise.
 #include "attention_rows.hpp"
 #include "relative_bias.hpp"
 
@@ -31,12 +40,8 @@ namespace mantis {
 namespace {
 
 constexpr int kBwdWaves = 4;
+constexpr int kXcds = 8;
 constexpr size_t kLdsBytes = 160 * 1024;
-
-// fp32 add to LDS, no value back
-__device__ __forceinline__ void lds_add(float* p, float x) {
-  __hip_atomic_fetch_add(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-}
 
 // Dynamic LDS: the bias table, then (query pass) the bucket table and the columns.
 __host__ __device__ constexpr size_t table_bytes(int n_disp) { return (size_t(n_disp + 2) * 4 + 15) / 16 * 16; }
@@ -45,22 +50,183 @@ __host__ __device__ constexpr size_t column_bytes(int n_buckets, int columns) {
   return size_t(kBwdWaves) * (n_buckets + 1) * columns * 4;  // (a row for the pairs of no bucket)
 }
 
+// 64 rows of one operand: kPer 16-byte pieces per thread, in registers and then
+// in LDS at kPitch; rows at or past the descriptor's count are zeros.
+template <int HD>
+struct RowTile {
+  static constexpr int kPitch = HD + 8;           // 16-bit elements
+  static constexpr int kPieces = kTile * HD / 8;  // 16-byte pieces
+  static constexpr int kPer = kPieces < 256 ? 1 : kPieces / 256;
+  uint4 reg[kPer];
+  __device__ __forceinline__ void fetch(i32x4_t rows, int32_t first) {
+#pragma unroll
+    for (int r = 0; r < kPer; ++r) {
+      const int i = int(threadIdx.x) + 256 * r;
+      reg[r] = row_load16(rows, i < kPieces ? first + i / (HD / 8) : -1, 16 * (i % (HD / 8)));
+    }
+  }
+  __device__ __forceinline__ void stage(uint16_t* s) const {
+#pragma unroll
+    for (int r = 0; r < kPer; ++r) {
+      const int i = int(threadIdx.x) + 256 * r;
+      if (i < kPieces) *reinterpret_cast<uint4*>(s + (i / (HD / 8)) * kPitch + 8 * (i % (HD / 8))) = reg[r];
+    }
+  }
+};
+
+__device__ __forceinline__ i32x4_t rows_of(const Rows& r, int64_t pos, int64_t a, int64_t L) {
+  return rows_rsrc(r.at(pos, a), uint32_t(r.st * 2), uint32_t(L));
+}
+
+// this lane's row as the B fragments of a product over dims (HD = 16: lanes g >= 2 hold zeros)
+template <bool kHalf, int HD>
+__device__ __forceinline__ void row_frags(i32x4_t rows, int64_t row, int g, uint4 (&u)[Geom<kHalf, HD>::kKs]) {
+  using G = Geom<kHalf, HD>;
+#pragma unroll
+  for (int ks = 0; ks < G::kKs; ++ks) {
+    u[ks] = row_load16(rows, int32_t(row), 2 * G::kdim(ks, g));
+    if (HD < 32 && g >= 2) u[ks] = make_uint4(0u, 0u, 0u, 0u);
+  }
+}
+
+// the A fragment (16 dims x 32 rows) of the transposed rows 32 h .. of a tile,
+// dims 16 dt .., its K slots the rows 4 g + t and 16 + 4 g + t: the transposing
+// read gives lane i of 16 the i-th of the 16 dims of four rows whose 8-byte
+// pieces the 16 lanes name
+typedef short lds_s16x4_t __attribute__((ext_vector_type(4)));
+template <int HD>
+__device__ __forceinline__ uint4 transposed_frag(const uint16_t* s, int h, int dt, int l16, int g) {
+  using Shared = __attribute__((address_space(3))) lds_s16x4_t;
+  const uint16_t* at = s + (32 * h + 4 * g + l16 / 4) * RowTile<HD>::kPitch + 16 * dt + 4 * (l16 % 4);
+  const lds_s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Shared*)at);
+  const lds_s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Shared*)(at + 16 * RowTile<HD>::kPitch));
+  const uint2 a = __builtin_bit_cast(uint2, lo), b = __builtin_bit_cast(uint2, hi);
+  return make_uint4(a.x, a.y, b.x, b.y);
+}
+
+// two fp32 values as their packed 16-bit parts: hi rounded, lo what is left
+template <bool kHalf>
+__device__ __forceinline__ void parts(float a, float b, uint32_t& hi, uint32_t& lo) {
+  hi = Frag<kHalf>::pack_unit(a, b);
+  if constexpr (kHalf) {
+    const f16x2_t h = __builtin_bit_cast(f16x2_t, hi);
+    lo = Frag<true>::pack_unit(a - float(h[0]), b - float(h[1]));
+  } else {
+    lo = Frag<false>::pack_unit(a - __uint_as_float(hi << 16), b - __uint_as_float(hi & 0xffff0000u));
+  }
+}
+
+// acc (HD dims x this lane's row) += transposed rows . x for the staged rows
+// below n, x the 16 fp32 values of this lane (rows 16 tt + 4 g + t; zeros from n on)
+template <bool kHalf, int HD>
+__device__ __forceinline__ void accumulate_parts(const uint16_t* s, int n, int l16, int g, const f32x4_t (&x)[4],
+                                                 f32x4_t (&acc)[Geom<kHalf, HD>::kDt]) {
+  using FR = Frag<kHalf>;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    if (32 * h >= n) break;  // uniform
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      parts<kHalf>(x[2 * h + i / 2][2 * (i % 2)], x[2 * h + i / 2][2 * (i % 2) + 1], hi[i], lo[i]);
+    const typename FR::vec bh = FR::cast(make_uint4(hi[0], hi[1], hi[2], hi[3]));
+    const typename FR::vec bl = FR::cast(make_uint4(lo[0], lo[1], lo[2], lo[3]));
+#pragma unroll
+    for (int dt = 0; dt < Geom<kHalf, HD>::kDt; ++dt) {
+      const typename FR::vec a = FR::cast(transposed_frag<HD>(s, h, dt, l16, g));
+      acc[dt] = mfma16x16x32(a, bh, acc[dt]);
+      acc[dt] = mfma16x16x32(a, bl, acc[dt]);
+    }
+  }
+}
+
+// The power of two that a column's fp16 parts are scaled by: the largest value
+// met so far lands in [2^13, 2^15].  bf16 parts need none.
+template <bool kHalf>
+struct ColumnScale {
+  float s = kHalf ? 0x1p126f : 1.f;
+  // scales x, and acc when the scale moves; the four lanes of a column agree
+  template <int kDt>
+  __device__ __forceinline__ void apply(f32x4_t (&x)[4], f32x4_t (&acc)[kDt]) {
+    if constexpr (kHalf) {
+      float m = 0.f;
+#pragma unroll
+      for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) m = fmaxf(m, fabsf(x[tt][t]));
+      m = max_xor32(max_xor16(m));
+      const bool over = m * s > 32768.f;
+      if (__builtin_amdgcn_ballot_w64(over)) {  // wavefront-uniform
+        const int e = 267 - int(__float_as_uint(m) >> 23);  // 2^13 over m's power of two
+        const float next = over ? __uint_as_float(uint32_t(e < 1 ? 1 : e > 253 ? 253 : e) << 23) : s;
+        const float ratio = next / s;
+        s = next;
+#pragma unroll
+        for (int dt = 0; dt < kDt; ++dt)
+#pragma unroll
+          for (int t = 0; t < 4; ++t) acc[dt][t] *= ratio;
+      }
+#pragma unroll
+      for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) x[tt][t] *= s;
+    }
+  }
+};
+
+// table offsets of this lane's pairs with the 64 staged rows of the other side
+template <bool kQuery>
+__device__ __forceinline__ void pair_offsets(const Side<kQuery>& side, const Relative& rel, const uint32_t* sc,
+                                             int64_t first, int g, int (&at)[4][4]) {
+#pragma unroll
+  for (int tt = 0; tt < 4; ++tt) {
+    const uint4 c = *reinterpret_cast<const uint4*>(&sc[16 * tt + 4 * g]);
+    const uint32_t cs[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+    for (int t = 0; t < 4; ++t) at[tt][t] = side.at(cs[t]);
+  }
+  if (first < rel.n_latents) {  // uniform
+    const int64_t lat = rel.n_latents - first - 4 * g;
+#pragma unroll
+    for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+      for (int t = 0; t < 4; ++t) at[tt][t] = 16 * tt + t < lat ? side.latent_other : at[tt][t];
+  }
+}
+
+// four adds of a lane to its own LDS words, all read before the first is
+// written: words named twice take the sum so far
+__device__ __forceinline__ void add4(char* base, const int (&at)[4], const float (&x)[4]) {
+  float old[4];
+#pragma unroll
+  for (int t = 0; t < 4; ++t) old[t] = *reinterpret_cast<const float*>(base + at[t]);
+  const float x1 = x[1] + (at[1] == at[0] ? x[0] : 0.f);
+  const float x2 = x[2] + (at[2] == at[1] ? x1 : at[2] == at[0] ? x[0] : 0.f);
+  const float x3 = x[3] + (at[3] == at[2] ? x2 : at[3] == at[1] ? x1 : at[3] == at[0] ? x[0] : 0.f);
+  *reinterpret_cast<float*>(base + at[0]) = old[0] + x[0];
+  *reinterpret_cast<float*>(base + at[1]) = old[1] + x1;
+  *reinterpret_cast<float*>(base + at[2]) = old[2] + x2;
+  *reinterpret_cast<float*>(base + at[3]) = old[3] + x3;
+}
+
 template <bool kHalf, int HD, int kColumns>
 __global__ void __launch_bounds__(256)
 relative_bwd_q_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int32_t* __restrict__ seq_lens, int heads,
-                      int64_t T, const float2* __restrict__ stats, float scale, float root_hd,
+                      int64_t T, int64_t n_items, const float2* __restrict__ stats, float scale, float root_hd,
                       float* __restrict__ delta, RowsOut dq, float* __restrict__ partial) {
   using G = Geom<kHalf, HD>;
-  __shared__ __attribute__((aligned(16))) uint16_t sk[kTile * G::kPitch], sv[kTile * G::kPitch];
-  __shared__ __attribute__((aligned(16))) uint16_t skt[HD * kTPitch];
-  __shared__ __attribute__((aligned(16))) uint32_t sc[kTile];
+  using Tile = RowTile<HD>;
+  __shared__ __attribute__((aligned(16))) uint16_t sk[2][kTile * Tile::kPitch], sv[2][kTile * Tile::kPitch];
+  __shared__ __attribute__((aligned(16))) uint32_t sc[2][kTile];
   extern __shared__ __attribute__((aligned(16))) char dynamic[];
+  const int64_t item = int64_t(blockIdx.x % kXcds) * (gridDim.x / kXcds) + blockIdx.x / kXcds;
+  if (item >= n_items) return;
   const int n_disp = rel.nq * rel.nr;
   float* table = reinterpret_cast<float*>(dynamic);
   uint16_t* bucket = reinterpret_cast<uint16_t*>(dynamic + table_bytes(n_disp));
   float* columns = reinterpret_cast<float*>(dynamic + table_bytes(n_disp) + bucket_bytes(n_disp));
   const int64_t n_tiles = (T + kTile - 1) / kTile;
-  const int64_t pa = blockIdx.x / n_tiles, tile = blockIdx.x % n_tiles;
+  const int64_t pa = item / n_tiles, tile = item % n_tiles;
   const int64_t pos = pa / heads, a = pa % heads;
   int64_t L = seq_lens[pos];
   L = L < 0 ? 0 : (L > T ? T : L);
@@ -69,190 +235,220 @@ relative_bwd_q_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int32
   const bool live = i < L;
   const int n_rows = rel.n_buckets + 1;
   // partial sums: (head, position, tile, bucket)
-  float* part = partial + ((a * (gridDim.x / n_tiles / heads) + pos) * n_tiles + tile) * rel.n_buckets;
+  float* part = partial + ((a * (n_items / n_tiles / heads) + pos) * n_tiles + tile) * rel.n_buckets;
+  f32x4_t acc[G::kDt];
+#pragma unroll
+  for (int dt = 0; dt < G::kDt; ++dt) acc[dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   if (tile * kTile >= L) {  // no live row
     if (i < T) {
-      const f32x4_t zero[G::kDt] = {};
-      store_row<kHalf, HD, true>(dq.row(pos, a, i), g, zero, 0.f, false);
+      store_row<kHalf, HD, true>(dq.row(pos, a, i), g, acc, 0.f, false);
       if (g == 0) delta[pa * T + i] = 0.f;
     }
     for (int b = threadIdx.x; b < rel.n_buckets; b += 256) part[b] = 0.f;
     return;
   }
+  const i32x4_t krs = rows_of(k, pos, a, L), vrs = rows_of(v, pos, a, L);
+  Tile ck, cv;
+  uint32_t cc = 0u;
+  auto fetch = [&](int64_t kb) {
+    ck.fetch(krs, int32_t(kb));
+    cv.fetch(vrs, int32_t(kb));
+    if (threadIdx.x < kTile) cc = coords_of(rel, pos, T, kb + threadIdx.x, L);
+  };
+  auto stage = [&](int buf) {
+    ck.stage(sk[buf]);
+    cv.stage(sv[buf]);
+    if (threadIdx.x < kTile) sc[buf][threadIdx.x] = cc;
+  };
+  fetch(0);
   uint4 qf[G::kKs], gf[G::kKs];
-  load_frags<kHalf, HD>(q.at(pos, a) + i * q.st, live, g, qf);
-  load_frags<kHalf, HD>(go.at(pos, a) + i * go.st, live, g, gf);
+  row_frags<kHalf, HD>(rows_of(q, pos, a, L), i, g, qf);
+  row_frags<kHalf, HD>(rows_of(go, pos, a, L), i, g, gf);
   const float2 st = live ? stats[pa * T + i] : make_float2(0.f, INFINITY);
   const Side<true> side(rel, coords_of(rel, pos, T, i, L), i < rel.n_latents);
   stage_bias(rel, a, root_hd, table);
   for (int d = threadIdx.x; d < n_disp + 2; d += 256) bucket[d] = uint16_t(bucket_of(rel, d));
-  for (int c = threadIdx.x; c < kBwdWaves * n_rows * kColumns; c += 256) columns[c] = 0.f;
-  float* column = columns + wave * n_rows * kColumns + lane % kColumns;
+  for (int c = threadIdx.x; c < kBwdWaves * n_rows * kColumns / 4; c += 256)
+    reinterpret_cast<float4*>(columns)[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+  // this lane's column; a dead query's pairs all go to the row of no bucket
+  char* column = reinterpret_cast<char*>(columns + wave * n_rows * kColumns + lane % kColumns);
+  const int row_bytes = live ? kColumns * 4 : 0;
+  if (!live) column += rel.n_buckets * kColumns * 4;
+  stage(0);
+  const int64_t n_chunks = (L + kTile - 1) / kTile;
+  if (n_chunks > 1) fetch(kTile);
+  __syncthreads();
 
-  f32x4_t acc[G::kDt];
-#pragma unroll
-  for (int dt = 0; dt < G::kDt; ++dt) acc[dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  const uint16_t* kp = k.at(pos, a);
-  const uint16_t* vp = v.at(pos, a);
-  Chunk<kHalf, HD> ck, cv;
-  uint32_t cc = 0u;
-  auto fetch = [&](int64_t kb) {
-    ck.fetch(kp, k.st, kb, L);
-    cv.fetch(vp, v.st, kb, L);
-    if (threadIdx.x < kTile) cc = coords_of(rel, pos, T, kb + threadIdx.x, L);
-  };
-  auto stage = [&](bool transposed) {
-    __syncthreads();  // the last chunk's readers are done
-    ck.stage_rows(sk);
-    if (transposed) ck.stage_transposed(skt);
-    cv.stage_rows(sv);
-    if (threadIdx.x < kTile) sc[threadIdx.x] = cc;
-    __syncthreads();
-  };
   const float c_log2 = scale * kLog2e;
-  int at[4][4];  // the pairs' table entries, as byte offsets
-  // p and dp of the staged chunk's keys for this lane's query, zeros at or past L
-  auto pairs = [&](int64_t kb, int n, float (&p)[4][4], f32x4_t (&dp)[4]) {
-    const int lim = n - 4 * g;  // keys 16 tt + t below it are live
-    f32x4_t s[4];
+  auto rows_in = [&](int64_t c) { return int(L - c * kTile < kTile ? L - c * kTile : kTile); };
+  // p and dp of this lane's query with chunk c's keys, zeros past the last one
+  auto pairs = [&](int buf, int64_t c, const int (&at)[4][4], f32x4_t (&p)[4], f32x4_t (&dp)[4]) {
+    const int n = rows_in(c);
 #pragma unroll
-    for (int tt = 0; tt < 4; ++tt) {
-      const uint4 kc = *reinterpret_cast<const uint4*>(&sc[16 * tt + 4 * g]);
-      const uint32_t kcs[4] = {kc.x, kc.y, kc.z, kc.w};
+    for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
-      for (int t = 0; t < 4; ++t) at[tt][t] = side.at(kcs[t]);
-    }
-    if (kb < rel.n_latents) {  // uniform
-      const int64_t lat = rel.n_latents - kb - 4 * g;
+      for (int t = 0; t < 4; ++t) p[tt][t] = entry(table, at[tt][t]);
+    products_onto<kHalf, HD>(sk[buf], n, l16, g, qf, p);
+    products<kHalf, HD>(sv[buf], n, l16, g, gf, dp);
+#pragma unroll
+    for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+      for (int t = 0; t < 4; ++t) p[tt][t] = __builtin_amdgcn_exp2f(fmaf(p[tt][t] - st.x, c_log2, -st.y));
+    if (n < kTile) {  // uniform
+      const int lim = n - 4 * g;
 #pragma unroll
       for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
-        for (int t = 0; t < 4; ++t) at[tt][t] = 16 * tt + t < lat ? side.latent_other : at[tt][t];
+        for (int t = 0; t < 4; ++t) {
+          p[tt][t] = 16 * tt + t < lim ? p[tt][t] : 0.f;
+          dp[tt][t] = 16 * tt + t < lim ? dp[tt][t] : 0.f;
+        }
     }
-#pragma unroll
-    for (int tt = 0; tt < 4; ++tt)
-#pragma unroll
-      for (int t = 0; t < 4; ++t) s[tt][t] = entry(table, at[tt][t]);
-    products_onto<kHalf, HD>(sk, n, l16, g, qf, s);
-    products<kHalf, HD>(sv, n, l16, g, gf, dp);
-#pragma unroll
-    for (int tt = 0; tt < 4; ++tt)
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const bool in = 16 * tt + t < lim;
-        p[tt][t] = in ? __builtin_amdgcn_exp2f(fmaf(s[tt][t] - st.x, c_log2, -st.y)) : 0.f;
-        dp[tt][t] = in ? dp[tt][t] : 0.f;
-      }
   };
   float dl = 0.f;
-  auto sum_delta = [&](const float (&p)[4][4], const f32x4_t (&dp)[4]) {
+  // (a chunk's terms among themselves first: fewer roundings of the long sum)
+  auto sum_delta = [&](const f32x4_t (&p)[4], const f32x4_t (&dp)[4]) {
+    float sum = 0.f;
 #pragma unroll
     for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
-      for (int t = 0; t < 4; ++t) dl = fmaf(p[tt][t], dp[tt][t], dl);
+      for (int t = 0; t < 4; ++t) sum = fmaf(p[tt][t], dp[tt][t], sum);
+    dl += sum;
   };
-  auto spread = [&](int n, const float (&p)[4][4], const f32x4_t (&dp)[4]) {
-    const int lim = n - 4 * g;
-    float ds[4][4];
+  ColumnScale<kHalf> cs;
+  auto spread = [&](int buf, int64_t c, const int (&at)[4][4], f32x4_t (&p)[4], const f32x4_t (&dp)[4]) {
+    const int n = rows_in(c);
 #pragma unroll
-    for (int tt = 0; tt < 4; ++tt)
+    for (int tt = 0; tt < 4; ++tt) {
+      if (16 * tt >= n) break;  // uniform
+      int to[4];
+      float x[4];
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        ds[tt][t] = p[tt][t] * (dp[tt][t] - dl);
-        const bool in = live && 16 * tt + t < lim;
-        float* to = column + (in ? int(bucket[at[tt][t] / 4]) : rel.n_buckets) * kColumns;
-        if constexpr (kColumns == 64) {
-          lds_add(to, ds[tt][t]);
-        } else {
+        p[tt][t] *= dp[tt][t] - dl;
+        x[t] = p[tt][t];
+        to[t] = int(bucket[at[tt][t] / 4]) * row_bytes;
+      }
+      if (n < kTile) {  // uniform: a key past the last one adds nothing, whatever delta is
 #pragma unroll
-          for (int turn = 0; turn < 4; ++turn)
-            if (g == turn) lds_add(to, ds[tt][t]);
+        for (int t = 0; t < 4; ++t) p[tt][t] = x[t] = 16 * tt + t < n - 4 * g ? x[t] : 0.f;
+      }
+      if constexpr (kColumns == 64) {
+        add4(column, to, x);
+      } else {
+#pragma unroll
+        for (int turn = 0; turn < 4; ++turn) {
+          if (g == turn) add4(column, to, x);
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (the next group reads what this one wrote)
         }
       }
-    accumulate<kHalf, HD>(skt, n, l16, g, ds, acc);
+    }
+    cs.apply(p, acc);
+    accumulate_parts<kHalf, HD>(sk[buf], n, l16, g, p, acc);
   };
-  float p[4][4];
-  f32x4_t dp[4];
-  fetch(0);
-  if (L <= kTile) {
-    stage(true);
-    if (first < L) {  // wavefront-uniform: a live row here
-      pairs(0, int(L), p, dp);
+  int at[4][4];
+  f32x4_t p[4], dp[4];
+  const bool working = first < L;  // wavefront-uniform: a live row here
+  if (n_chunks <= 2) {
+    f32x4_t p1[4], dp1[4];
+    if (working) {
+      pair_offsets(side, rel, sc[0], 0, g, at);
+      pairs(0, 0, at, p, dp);
       sum_delta(p, dp);
+    }
+    if (n_chunks == 2) {
+      stage(1);
+      __syncthreads();
+      if (working) {
+        int at1[4][4];
+        pair_offsets(side, rel, sc[1], kTile, g, at1);
+        pairs(1, 1, at1, p1, dp1);
+        sum_delta(p1, dp1);
+      }
+    }
+    if (working) {
       dl = sum_xor32(sum_xor16(dl));
-      spread(int(L), p, dp);
+      spread(0, 0, at, p, dp);
+      if (n_chunks == 2) {
+        pair_offsets(side, rel, sc[1], kTile, g, at);
+        spread(1, 1, at, p1, dp1);
+      }
     }
   } else {
-    for (int64_t kb = 0; kb < L; kb += kTile) {
-      stage(false);
-      fetch(kb + kTile < L ? kb + kTile : 0);
-      if (first >= L) continue;
-      pairs(kb, int(L - kb < kTile ? L - kb : kTile), p, dp);
-      sum_delta(p, dp);
-    }
-    dl = sum_xor32(sum_xor16(dl));
-    for (int64_t kb = 0; kb < L; kb += kTile) {
-      stage(true);
-      if (kb + kTile < L) fetch(kb + kTile);
-      if (first >= L) continue;
-      const int n = int(L - kb < kTile ? L - kb : kTile);
-      pairs(kb, n, p, dp);
-      spread(n, p, dp);
+    // step s: chunk s % n_chunks in buffer s % 2; the first n_chunks for delta
+    for (int64_t s = 0, c = 0; s < 2 * n_chunks; ++s, c = c + 1 < n_chunks ? c + 1 : 0) {
+      const int buf = int(s & 1);
+      if (working) {
+        pair_offsets(side, rel, sc[buf], c * kTile, g, at);
+        pairs(buf, c, at, p, dp);
+        if (s < n_chunks) sum_delta(p, dp);
+        else spread(buf, c, at, p, dp);
+        if (s == n_chunks - 1) dl = sum_xor32(sum_xor16(dl));
+      }
+      if (s + 1 < 2 * n_chunks) {
+        stage(buf ^ 1);  // (its readers met the barrier of the step before)
+        if (s + 2 < 2 * n_chunks) fetch((s + 2) % n_chunks * kTile);
+      }
+      __syncthreads();
     }
   }
   if (i < T) {
-    store_row<kHalf, HD, true>(dq.row(pos, a, i), g, acc, scale, live);
+    store_row<kHalf, HD, true>(dq.row(pos, a, i), g, acc, scale / cs.s, live);
     if (g == 0) delta[pa * T + i] = live ? dl : 0.f;
   }
   __syncthreads();
-  // the columns of a bucket, from the bucket's own on so that the threads meet other banks
-  for (int b = threadIdx.x; b < rel.n_buckets; b += 256) {
+  // eight threads to a bucket's columns, starting apart so that they meet other
+  // banks; the shuffles join them
+  for (int b0 = 0; b0 < rel.n_buckets; b0 += 32) {
+    const int b = b0 + int(threadIdx.x) / 8, eighth = threadIdx.x % 8;
     float sum = 0.f;
-    for (int w = 0; w < kBwdWaves; ++w)
-      for (int c = 0; c < kColumns; ++c) sum += columns[(w * n_rows + b) * kColumns + (c + b) % kColumns];
-    part[b] = sum;
+    if (b < rel.n_buckets)
+      for (int w = 0; w < kBwdWaves; ++w)
+#pragma unroll
+        for (int c = 0; c < kColumns / 8; ++c)
+          sum += columns[(w * n_rows + b) * kColumns + (8 * c + eighth + 8 * (int(threadIdx.x) / 8)) % kColumns];
+    sum += __shfl_xor(sum, 1);
+    sum += __shfl_xor(sum, 2);
+    sum += __shfl_xor(sum, 4);
+    if (b < rel.n_buckets && eighth == 0) part[b] = sum;
   }
 }
 
 template <bool kHalf, int HD>
 __global__ void __launch_bounds__(256)
 relative_bwd_kv_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int32_t* __restrict__ seq_lens, int heads,
-                       int64_t T, const float2* __restrict__ stats, float scale, float root_hd,
+                       int64_t T, int64_t n_items, const float2* __restrict__ stats, float scale, float root_hd,
                        const float* __restrict__ delta, RowsOut dk, RowsOut dv) {
   using G = Geom<kHalf, HD>;
-  __shared__ __attribute__((aligned(16))) uint16_t sq[kTile * G::kPitch], sg[kTile * G::kPitch];
-  __shared__ __attribute__((aligned(16))) uint16_t sqt[HD * kTPitch], sgt[HD * kTPitch];
-  __shared__ __attribute__((aligned(16))) float sm[kTile], sl[kTile], sd[kTile];
-  __shared__ __attribute__((aligned(16))) uint32_t sc[kTile];
+  using Tile = RowTile<HD>;
+  __shared__ __attribute__((aligned(16))) uint16_t sq[2][kTile * Tile::kPitch], sg[2][kTile * Tile::kPitch];
+  __shared__ __attribute__((aligned(16))) float sm[2][kTile], sl[2][kTile], sd[2][kTile];
+  __shared__ __attribute__((aligned(16))) uint32_t sc[2][kTile];
   extern __shared__ __attribute__((aligned(16))) char dynamic[];
+  const int64_t item = int64_t(blockIdx.x % kXcds) * (gridDim.x / kXcds) + blockIdx.x / kXcds;
+  if (item >= n_items) return;
   float* table = reinterpret_cast<float*>(dynamic);
   const int64_t n_tiles = (T + kTile - 1) / kTile;
-  const int64_t pa = blockIdx.x / n_tiles, tile = blockIdx.x % n_tiles;
+  const int64_t pa = item / n_tiles, tile = item % n_tiles;
   const int64_t pos = pa / heads, a = pa % heads;
   int64_t L = seq_lens[pos];
   L = L < 0 ? 0 : (L > T ? T : L);
   const int lane = threadIdx.x % 64, l16 = lane % 16, g = lane / 16;
   const int64_t first = tile * kTile + 16 * (threadIdx.x / 64), j = first + l16;
   const bool live = j < L;
+  constexpr float kPScale = kHalf ? 0x1p14f : 1.f;  // (probabilities are at most 1)
   f32x4_t ak[G::kDt], av[G::kDt];
 #pragma unroll
   for (int dt = 0; dt < G::kDt; ++dt) ak[dt] = av[dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  ColumnScale<kHalf> cs;
   if (tile * kTile < L) {  // workgroup-uniform
-    uint4 kf[G::kKs], vf[G::kKs];
-    load_frags<kHalf, HD>(k.at(pos, a) + j * k.st, live, g, kf);
-    load_frags<kHalf, HD>(v.at(pos, a) + j * v.st, live, g, vf);
-    const bool latent = j < rel.n_latents;
-    const Side<false> side(rel, coords_of(rel, pos, T, j, L), latent);
-    stage_bias(rel, a, root_hd, table);
-    const uint16_t* qp = q.at(pos, a);
-    const uint16_t* gp = go.at(pos, a);
-    const float c_log2 = scale * kLog2e;
-    Chunk<kHalf, HD> cq, cg;
+    const i32x4_t qrs = rows_of(q, pos, a, L), grs = rows_of(go, pos, a, L);
+    Tile cq, cg;
     float rm = 0.f, rl = INFINITY, rd = 0.f;
     uint32_t cc = 0u;
     auto fetch = [&](int64_t qb) {
-      cq.fetch(qp, q.st, qb, L);
-      cg.fetch(gp, go.st, qb, L);
+      cq.fetch(qrs, int32_t(qb));
+      cg.fetch(grs, int32_t(qb));
       if (threadIdx.x < kTile) {
         const int64_t i = qb + threadIdx.x;
         const bool in = i < L;
@@ -262,68 +458,78 @@ relative_bwd_kv_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int3
         cc = coords_of(rel, pos, T, i, L);
       }
     };
-    fetch(0);
-    for (int64_t qb = 0; qb < L; qb += kTile) {
-      __syncthreads();
-      cq.stage_rows(sq);
-      cq.stage_transposed(sqt);
-      cg.stage_rows(sg);
-      cg.stage_transposed(sgt);
+    auto stage = [&](int buf) {
+      cq.stage(sq[buf]);
+      cg.stage(sg[buf]);
       if (threadIdx.x < kTile) {
-        sm[threadIdx.x] = rm;
-        sl[threadIdx.x] = rl;
-        sd[threadIdx.x] = rd;
-        sc[threadIdx.x] = cc;
+        sm[buf][threadIdx.x] = rm;
+        sl[buf][threadIdx.x] = rl;
+        sd[buf][threadIdx.x] = rd;
+        sc[buf][threadIdx.x] = cc;
       }
-      __syncthreads();
-      if (qb + kTile < L) fetch(qb + kTile);
-      if (first >= L) continue;  // wavefront-uniform
-      const int n = int(L - qb < kTile ? L - qb : kTile);
-      f32x4_t s[4], dp[4];
-      int at[4][4];
-#pragma unroll
-      for (int tt = 0; tt < 4; ++tt) {
-        const uint4 qc = *reinterpret_cast<const uint4*>(&sc[16 * tt + 4 * g]);
-        const uint32_t qcs[4] = {qc.x, qc.y, qc.z, qc.w};
-#pragma unroll
-        for (int t = 0; t < 4; ++t) at[tt][t] = side.at(qcs[t]);
-      }
-      if (qb < rel.n_latents) {  // uniform (a latent key's pairs keep its own entry)
-        const int64_t lat = rel.n_latents - qb - 4 * g;
+    };
+    fetch(0);
+    uint4 kf[G::kKs], vf[G::kKs];
+    row_frags<kHalf, HD>(rows_of(k, pos, a, L), j, g, kf);
+    row_frags<kHalf, HD>(rows_of(v, pos, a, L), j, g, vf);
+    const Side<false> side(rel, coords_of(rel, pos, T, j, L), j < rel.n_latents);
+    stage_bias(rel, a, root_hd, table);
+    const float c_log2 = scale * kLog2e;
+    stage(0);
+    if (kTile < L) fetch(kTile);
+    __syncthreads();
+    for (int64_t qb = 0; qb < L; qb += kTile) {
+      const int buf = int(qb / kTile & 1);
+      if (first < L) {  // wavefront-uniform
+        const int n = int(L - qb < kTile ? L - qb : kTile);
+        f32x4_t p[4], ds[4];
+        int at[4][4];
+        pair_offsets(side, rel, sc[buf], qb, g, at);  // (a latent key's pairs keep its own entry)
 #pragma unroll
         for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
-          for (int t = 0; t < 4; ++t) at[tt][t] = 16 * tt + t < lat ? side.latent_other : at[tt][t];
-      }
+          for (int t = 0; t < 4; ++t) p[tt][t] = entry(table, at[tt][t]);
+        products_onto<kHalf, HD>(sq[buf], n, l16, g, kf, p);
+        products<kHalf, HD>(sg[buf], n, l16, g, vf, ds);
 #pragma unroll
-      for (int tt = 0; tt < 4; ++tt)
+        for (int tt = 0; tt < 4; ++tt) {
+          const f32x4_t m4 = *reinterpret_cast<const f32x4_t*>(&sm[buf][16 * tt + 4 * g]);
+          const f32x4_t l4 = *reinterpret_cast<const f32x4_t*>(&sl[buf][16 * tt + 4 * g]);
+          const f32x4_t d4 = *reinterpret_cast<const f32x4_t*>(&sd[buf][16 * tt + 4 * g]);
 #pragma unroll
-        for (int t = 0; t < 4; ++t) s[tt][t] = entry(table, at[tt][t]);
-      products_onto<kHalf, HD>(sq, n, l16, g, kf, s);
-      products<kHalf, HD>(sg, n, l16, g, vf, dp);
-      const int lim = n - 4 * g;  // queries 16 tt + t below it are live
-      float p[4][4], ds[4][4];
-#pragma unroll
-      for (int tt = 0; tt < 4; ++tt) {
-        const float4 m4 = *reinterpret_cast<const float4*>(&sm[16 * tt + 4 * g]);
-        const float4 l4 = *reinterpret_cast<const float4*>(&sl[16 * tt + 4 * g]);
-        const float4 d4 = *reinterpret_cast<const float4*>(&sd[16 * tt + 4 * g]);
-        const float mv[4] = {m4.x, m4.y, m4.z, m4.w}, lv[4] = {l4.x, l4.y, l4.z, l4.w},
-                    dv4[4] = {d4.x, d4.y, d4.z, d4.w};
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          const float e = __builtin_amdgcn_exp2f(fmaf(s[tt][t] - mv[t], c_log2, -lv[t]));
-          p[tt][t] = 16 * tt + t < lim ? e : 0.f;
-          ds[tt][t] = 16 * tt + t < lim ? e * (dp[tt][t] - dv4[t]) : 0.f;
+          for (int t = 0; t < 4; ++t) {
+            p[tt][t] = __builtin_amdgcn_exp2f(fmaf(p[tt][t] - m4[t], c_log2, -l4[t]));
+            ds[tt][t] = p[tt][t] * (ds[tt][t] - d4[t]);
+          }
         }
+        if (n < kTile) {  // uniform
+          const int lim = n - 4 * g;  // queries 16 tt + t below it are live
+#pragma unroll
+          for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+              p[tt][t] = 16 * tt + t < lim ? p[tt][t] : 0.f;
+              ds[tt][t] = 16 * tt + t < lim ? ds[tt][t] : 0.f;
+            }
+        }
+        if constexpr (kHalf) {
+#pragma unroll
+          for (int tt = 0; tt < 4; ++tt) p[tt] *= kPScale;
+        }
+        accumulate_parts<kHalf, HD>(sg[buf], n, l16, g, p, av);
+        cs.apply(ds, ak);
+        accumulate_parts<kHalf, HD>(sq[buf], n, l16, g, ds, ak);
       }
-      accumulate<kHalf, HD>(sgt, n, l16, g, p, av);
-      accumulate<kHalf, HD>(sqt, n, l16, g, ds, ak);
+      if (qb + kTile < L) {
+        stage(buf ^ 1);  // (its readers met the barrier of the chunk before)
+        if (qb + 2 * kTile < L) fetch(qb + 2 * kTile);
+      }
+      __syncthreads();
     }
   }
   if (j < T) {
-    store_row<kHalf, HD, true>(dk.row(pos, a, j), g, ak, scale, live);
-    store_row<kHalf, HD, true>(dv.row(pos, a, j), g, av, 1.f, live);
+    store_row<kHalf, HD, true>(dk.row(pos, a, j), g, ak, scale / cs.s, live);
+    store_row<kHalf, HD, true>(dv.row(pos, a, j), g, av, 1.f / kPScale, live);
   }
 }
 
@@ -345,7 +551,7 @@ relative_bias_sum_kernel(const float* __restrict__ partial, int64_t n_parts, int
 
 template <bool kHalf, int HD>
 constexpr size_t static_lds() {
-  return size_t(2 * kTile * Geom<kHalf, HD>::kPitch + HD * kTPitch) * 2 + kTile * 4;
+  return size_t(4 * kTile * RowTile<HD>::kPitch) * 2 + 2 * kTile * 4;  // (of the query pass)
 }
 
 // the dynamic LDS that a kernel may ask for, set once per kernel and device
@@ -366,7 +572,8 @@ template <bool kHalf, int HD>
 int32_t launch(const Rows& q, const Rows& k, const Rows& v, const Rows& go, const Relative& rel,
                const int32_t* seq_lens, int64_t n_pos, int heads, int64_t t, const float2* stats, float* delta,
                float* partial, const RowsOut& dq, const RowsOut& dk, const RowsOut& dv, float* dbias, hipStream_t st) {
-  const int64_t n_tiles = (t + kTile - 1) / kTile, grid = n_pos * heads * n_tiles;
+  const int64_t n_tiles = (t + kTile - 1) / kTile, n_items = n_pos * heads * n_tiles;
+  const int64_t grid = (n_items + kXcds - 1) / kXcds * kXcds;
   if (grid > 2147483647LL) return MANTIS_E_ARG;
   const float root = sqrtf(float(HD)), scale = 1.f / root;
   const int n_disp = rel.nq * rel.nr;
@@ -379,10 +586,10 @@ int32_t launch(const Rows& q, const Rows& k, const Rows& v, const Rows& go, cons
   if (!(fits ? allow_lds<relative_bwd_q_kernel<kHalf, HD, 64>>(most)
              : allow_lds<relative_bwd_q_kernel<kHalf, HD, 16>>(most)))
     return MANTIS_E_LAUNCH;
-  first<<<unsigned(grid), 256, fits ? wide : narrow, st>>>(q, k, v, go, rel, seq_lens, heads, t, stats, scale, root,
-                                                           delta, dq, partial);
+  first<<<unsigned(grid), 256, fits ? wide : narrow, st>>>(q, k, v, go, rel, seq_lens, heads, t, n_items, stats, scale,
+                                                           root, delta, dq, partial);
   relative_bwd_kv_kernel<kHalf, HD><<<unsigned(grid), 256, table_bytes(n_disp), st>>>(
-      q, k, v, go, rel, seq_lens, heads, t, stats, scale, root, delta, dk, dv);
+      q, k, v, go, rel, seq_lens, heads, t, n_items, stats, scale, root, delta, dk, dv);
   relative_bias_sum_kernel<<<unsigned(heads * rel.n_buckets), 256, 0, st>>>(partial, n_pos * n_tiles, rel.n_buckets,
                                                                            dbias);
   return launched();
@@ -417,6 +624,8 @@ extern "C" int32_t mantis_relative_attention_backward(
     if (st[3] != 1) return MANTIS_E_ARG;
     if ((st[0] | st[1] | st[2]) % 8) return MANTIS_E_ARG;
   }
+  for (const int64_t* st : {qs, ks, vs, gs})  // (buffer descriptors, as in the forward)
+    if (st[2] < hd || st[2] >= 8192 || t * st[2] * 2 > 2147483647LL) return MANTIS_E_ARG;
   for (const void* ptr : {q, k, v, grad_out, static_cast<const void*>(dq), static_cast<const void*>(dk),
                           static_cast<const void*>(dv), static_cast<const void*>(stats),
                           static_cast<const void*>(workspace)})
