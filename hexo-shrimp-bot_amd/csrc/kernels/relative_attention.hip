@@ -32,7 +32,6 @@ constexpr int kWaves = 4;
 constexpr int kKChunk = 64;
 constexpr int kVtPitch = kKChunk + 8;  // 16-bit elements per staged V^T row
 constexpr float kLazyLog2 = 8.f;       // probabilities up to 2^8 before the reference point moves
-constexpr int kXcds = 8;
 
 struct Operand {  // (P, A, T, hd): base and element strides
   const uint16_t* p;
@@ -43,7 +42,7 @@ template <bool kHalf, int HD, int kSub>
 __global__ void __launch_bounds__(256)
 relative_attention_kernel(Operand q, Operand k, Operand v, Relative rel, const int32_t* __restrict__ seq_lens,
                           int heads, int64_t T, uint16_t* __restrict__ out, int64_t osp, int64_t osa, int64_t ost,
-                          float* __restrict__ lse, float2* __restrict__ stats, float c_log2, float root_hd, int64_t n_items) {
+                          float* __restrict__ lse, float2* __restrict__ stats, float c_log2, float root_hd, int64_t n_pa) {
   constexpr int kQTile = kWaves * 16 * kSub;
   constexpr int kKPitch = HD + 8;              // 16-bit elements per staged K row
   constexpr int kKs = HD < 32 ? 1 : HD / 32;   // K steps of the score product
@@ -54,13 +53,10 @@ relative_attention_kernel(Operand q, Operand k, Operand v, Relative rel, const i
   __shared__ __attribute__((aligned(16))) uint16_t sk[2][kKChunk * kKPitch];
   __shared__ __attribute__((aligned(16))) uint16_t svt[2][HD * kVtPitch];
   __shared__ __attribute__((aligned(16))) uint32_t sc[2][kKChunk];
-  // consecutive items on one XCD share the position's rows in its L2 (the
-  // grid is a multiple of kXcds, workgroups go round-robin over the XCDs)
-  const int64_t item = int64_t(blockIdx.x % kXcds) * (gridDim.x / kXcds) + blockIdx.x / kXcds;
-  if (item >= n_items) return;
   const int64_t n_qt = (T + kQTile - 1) / kQTile;
-  const int64_t pa = item / n_qt, qt = item % n_qt;
-  const int64_t p = pa / heads, a = pa % heads;
+  const Item item = item_of(n_pa, heads, n_qt);
+  if (item.pa >= n_pa) return;
+  const int64_t pa = item.pa, qt = item.tile, p = pa / heads, a = pa % heads;
   int64_t L = seq_lens[p];
   L = L < 0 ? 0 : (L > T ? T : L);
   const int64_t q0 = qt * kQTile;
@@ -143,8 +139,9 @@ relative_attention_kernel(Operand q, Operand k, Operand v, Relative rel, const i
 #pragma unroll
   for (int j = 0; j < kSub; ++j) qc[j] = coords_of(rel, p, T, qrow[j], L);
   stage_bias(rel, a, root_hd, table);
-  Side<true> side[kSub] = {Side<true>(rel, qc[0], qrow[0] < rel.n_latents),
-                           Side<true>(rel, qc[kSub - 1], qrow[kSub - 1] < rel.n_latents)};
+  const Side<true, 4> side[2] = {{rel, qc[0], qrow[0] < rel.n_latents},
+                                {rel, qc[kSub - 1], qrow[kSub - 1] < rel.n_latents}};
+  const int n_latents = int(rel.n_latents);
 
   // per sub-tile: the exponent's reference point (raw-score units), O^T tiles,
   // the rounded probabilities' sum (a product with an all-ones A operand, every
@@ -170,23 +167,13 @@ relative_attention_kernel(Operand q, Operand k, Operand v, Relative rel, const i
     if constexpr (kNJ > 0) {
       f32x4_t s[kNJ][4];
 #pragma unroll
-      for (int tt = 0; tt < 4; ++tt) {
-        const uint4 kc = *reinterpret_cast<const uint4*>(&sc[buf][16 * tt + 4 * g]);
-        const uint32_t kcs[4] = {kc.x, kc.y, kc.z, kc.w};
-#pragma unroll
-        for (int j = 0; j < kNJ; ++j)
-#pragma unroll
-          for (int t = 0; t < 4; ++t) s[j][tt][t] = entry(table, side[j].at(kcs[t]));
-      }
-      if (kb < rel.n_latents) {  // uniform
-        const int64_t lat = rel.n_latents - kb - 4 * g;
-        const float b = entry(table, side[0].latent_other);
+      for (int j = 0; j < kNJ; ++j) {
+        int at[4][4];
+        pair_offsets(side[j], n_latents, sc[buf], int(kb), g, at);
 #pragma unroll
         for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
-          for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int j = 0; j < kNJ; ++j) s[j][tt][t] = 16 * tt + t < lat ? b : s[j][tt][t];
+          for (int t = 0; t < 4; ++t) s[j][tt][t] = entry(table, at[tt][t]);
       }
       if constexpr (decltype(masked)::value) {
         const int lim = int(L - kb) - 4 * g;
@@ -309,13 +296,12 @@ template <bool kHalf, int HD, int kSub>
 int32_t launch(const Operand& q, const Operand& k, const Operand& v, const Relative& rel, const int32_t* seq_lens,
                int64_t n_pos, int heads, int64_t t, uint16_t* out, const int64_t* os, float* lse, float2* stats, hipStream_t st) {
   constexpr int kQTile = kWaves * 16 * kSub;
-  const int64_t n_items = n_pos * heads * ((t + kQTile - 1) / kQTile);
-  const int64_t grid = (n_items + kXcds - 1) / kXcds * kXcds;
+  const int64_t grid = item_grid(n_pos, heads, (t + kQTile - 1) / kQTile);
   if (grid > 2147483647LL) return MANTIS_E_ARG;
   const size_t lds = size_t(rel.nq * rel.nr + 2) * sizeof(float);
   const float root = sqrtf(float(HD));
   relative_attention_kernel<kHalf, HD, kSub><<<unsigned(grid), 256, lds, st>>>(
-      q, k, v, rel, seq_lens, heads, t, out, os[0], os[1], os[2], lse, stats, 1.4426950408889634f / root, root, n_items);
+      q, k, v, rel, seq_lens, heads, t, out, os[0], os[1], os[2], lse, stats, 1.4426950408889634f / root, root, n_pos * heads);
   return launched();
 }
 

@@ -33,6 +33,8 @@
 // pass.)  The columns join in a fixed order into the workgroup's partial sums, those
 // of a head in a second launch.  Every sum is fp32 in a fixed order: two calls
 // agree bitwise.
+#include <type_traits>
+
 #include "attention_rows.hpp"
 #include "relative_bias.hpp"
 
@@ -40,12 +42,13 @@ namespace mantis {
 namespace {
 
 constexpr int kBwdWaves = 4;
-constexpr int kXcds = 8;
 constexpr size_t kLdsBytes = 160 * 1024;
 
-// Dynamic LDS: the bias table, then (query pass) the bucket table and the columns.
-__host__ __device__ constexpr size_t table_bytes(int n_disp) { return (size_t(n_disp + 2) * 4 + 15) / 16 * 16; }
-__host__ __device__ constexpr size_t bucket_bytes(int n_disp) { return (size_t(n_disp + 2) * 2 + 15) / 16 * 16; }
+// Dynamic LDS: the table by displacement (the bias; in the query pass the bias and
+// the byte offset of the bucket's row of columns), then the query pass's columns.
+__host__ __device__ constexpr size_t table_bytes(int n_disp, int entry) {
+  return (size_t(n_disp + 2) * entry + 15) / 16 * 16;
+}
 __host__ __device__ constexpr size_t column_bytes(int n_buckets, int columns) {
   return size_t(kBwdWaves) * (n_buckets + 1) * columns * 4;  // (a row for the pairs of no bucket)
 }
@@ -174,29 +177,9 @@ struct ColumnScale {
   }
 };
 
-// table offsets of this lane's pairs with the 64 staged rows of the other side
-template <bool kQuery>
-__device__ __forceinline__ void pair_offsets(const Side<kQuery>& side, const Relative& rel, const uint32_t* sc,
-                                             int64_t first, int g, int (&at)[4][4]) {
-#pragma unroll
-  for (int tt = 0; tt < 4; ++tt) {
-    const uint4 c = *reinterpret_cast<const uint4*>(&sc[16 * tt + 4 * g]);
-    const uint32_t cs[4] = {c.x, c.y, c.z, c.w};
-#pragma unroll
-    for (int t = 0; t < 4; ++t) at[tt][t] = side.at(cs[t]);
-  }
-  if (first < rel.n_latents) {  // uniform
-    const int64_t lat = rel.n_latents - first - 4 * g;
-#pragma unroll
-    for (int tt = 0; tt < 4; ++tt)
-#pragma unroll
-      for (int t = 0; t < 4; ++t) at[tt][t] = 16 * tt + t < lat ? side.latent_other : at[tt][t];
-  }
-}
-
 // four adds of a lane to its own LDS words, all read before the first is
 // written: words named twice take the sum so far
-__device__ __forceinline__ void add4(char* base, const int (&at)[4], const float (&x)[4]) {
+__device__ __forceinline__ void add4(char* base, const uint32_t (&at)[4], const float (&x)[4]) {
   float old[4];
 #pragma unroll
   for (int t = 0; t < 4; ++t) old[t] = *reinterpret_cast<const float*>(base + at[t]);
@@ -212,22 +195,20 @@ __device__ __forceinline__ void add4(char* base, const int (&at)[4], const float
 template <bool kHalf, int HD, int kColumns>
 __global__ void __launch_bounds__(256)
 relative_bwd_q_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int32_t* __restrict__ seq_lens, int heads,
-                      int64_t T, int64_t n_items, const float2* __restrict__ stats, float scale, float root_hd,
+                      int64_t T, int64_t n_pa, const float2* __restrict__ stats, float scale, float root_hd,
                       float* __restrict__ delta, RowsOut dq, float* __restrict__ partial) {
   using G = Geom<kHalf, HD>;
   using Tile = RowTile<HD>;
   __shared__ __attribute__((aligned(16))) uint16_t sk[2][kTile * Tile::kPitch], sv[2][kTile * Tile::kPitch];
   __shared__ __attribute__((aligned(16))) uint32_t sc[2][kTile];
   extern __shared__ __attribute__((aligned(16))) char dynamic[];
-  const int64_t item = int64_t(blockIdx.x % kXcds) * (gridDim.x / kXcds) + blockIdx.x / kXcds;
-  if (item >= n_items) return;
-  const int n_disp = rel.nq * rel.nr;
-  float* table = reinterpret_cast<float*>(dynamic);
-  uint16_t* bucket = reinterpret_cast<uint16_t*>(dynamic + table_bytes(n_disp));
-  float* columns = reinterpret_cast<float*>(dynamic + table_bytes(n_disp) + bucket_bytes(n_disp));
   const int64_t n_tiles = (T + kTile - 1) / kTile;
-  const int64_t pa = item / n_tiles, tile = item % n_tiles;
-  const int64_t pos = pa / heads, a = pa % heads;
+  const Item item = item_of(n_pa, heads, n_tiles);
+  if (item.pa >= n_pa) return;
+  const int n_disp = rel.nq * rel.nr;
+  uint2* table = reinterpret_cast<uint2*>(dynamic);
+  float* columns = reinterpret_cast<float*>(dynamic + table_bytes(n_disp, 8));
+  const int64_t pa = item.pa, tile = item.tile, pos = pa / heads, a = pa % heads;
   int64_t L = seq_lens[pos];
   L = L < 0 ? 0 : (L > T ? T : L);
   const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, l16 = lane % 16, g = lane / 16;
@@ -235,7 +216,7 @@ relative_bwd_q_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int32
   const bool live = i < L;
   const int n_rows = rel.n_buckets + 1;
   // partial sums: (head, position, tile, bucket)
-  float* part = partial + ((a * (n_items / n_tiles / heads) + pos) * n_tiles + tile) * rel.n_buckets;
+  float* part_sums = partial + ((a * (n_pa / heads) + pos) * n_tiles + tile) * rel.n_buckets;
   f32x4_t acc[G::kDt];
 #pragma unroll
   for (int dt = 0; dt < G::kDt; ++dt) acc[dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -244,7 +225,7 @@ relative_bwd_q_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int32
       store_row<kHalf, HD, true>(dq.row(pos, a, i), g, acc, 0.f, false);
       if (g == 0) delta[pa * T + i] = 0.f;
     }
-    for (int b = threadIdx.x; b < rel.n_buckets; b += 256) part[b] = 0.f;
+    for (int b = threadIdx.x; b < rel.n_buckets; b += 256) part_sums[b] = 0.f;
     return;
   }
   const i32x4_t krs = rows_of(k, pos, a, L), vrs = rows_of(v, pos, a, L);
@@ -265,45 +246,44 @@ relative_bwd_q_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int32
   row_frags<kHalf, HD>(rows_of(q, pos, a, L), i, g, qf);
   row_frags<kHalf, HD>(rows_of(go, pos, a, L), i, g, gf);
   const float2 st = live ? stats[pa * T + i] : make_float2(0.f, INFINITY);
-  const Side<true> side(rel, coords_of(rel, pos, T, i, L), i < rel.n_latents);
-  stage_bias(rel, a, root_hd, table);
-  for (int d = threadIdx.x; d < n_disp + 2; d += 256) bucket[d] = uint16_t(bucket_of(rel, d));
+  const Side<true, 8> side(rel, coords_of(rel, pos, T, i, L), i < rel.n_latents);
+  const int n_latents = int(rel.n_latents);
+  for (int d = threadIdx.x; d < n_disp + 2; d += 256) {
+    const int b = bucket_of(rel, d);
+    const float x = b < rel.n_buckets ? raw_bias(rel.bias[a * rel.n_buckets + b], root_hd) : 0.f;
+    table[d] = make_uint2(__float_as_uint(x), uint32_t(b) * kColumns * 4);
+  }
   for (int c = threadIdx.x; c < kBwdWaves * n_rows * kColumns / 4; c += 256)
     reinterpret_cast<float4*>(columns)[c] = make_float4(0.f, 0.f, 0.f, 0.f);
-  // this lane's column; a dead query's pairs all go to the row of no bucket
+  // this lane's column (the lanes of a dead query spoil only their own, which no sum takes)
   char* column = reinterpret_cast<char*>(columns + wave * n_rows * kColumns + lane % kColumns);
-  const int row_bytes = live ? kColumns * 4 : 0;
-  if (!live) column += rel.n_buckets * kColumns * 4;
   stage(0);
   const int64_t n_chunks = (L + kTile - 1) / kTile;
   if (n_chunks > 1) fetch(kTile);
   __syncthreads();
 
   const float c_log2 = scale * kLog2e;
-  auto rows_in = [&](int64_t c) { return int(L - c * kTile < kTile ? L - c * kTile : kTile); };
-  // p and dp of this lane's query with chunk c's keys, zeros past the last one
-  auto pairs = [&](int buf, int64_t c, const int (&at)[4][4], f32x4_t (&p)[4], f32x4_t (&dp)[4]) {
-    const int n = rows_in(c);
+  constexpr std::true_type full{};
+  constexpr std::false_type part{};
+  // p and dp of this lane's query with chunk c's keys, zeros past the n-th (a full chunk has no branch)
+  auto pairs = [&](auto whole, int buf, int64_t c, int n, f32x4_t (&p)[4], f32x4_t (&dp)[4]) {
+    constexpr bool kWhole = decltype(whole)::value;
+    int at[4][4];
+    pair_offsets(side, n_latents, sc[buf], int(c * kTile), g, at);
 #pragma unroll
     for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
       for (int t = 0; t < 4; ++t) p[tt][t] = entry(table, at[tt][t]);
-    products_onto<kHalf, HD>(sk[buf], n, l16, g, qf, p);
-    products<kHalf, HD>(sv[buf], n, l16, g, gf, dp);
+    products_onto<kHalf, HD>(sk[buf], kWhole ? kTile : n, l16, g, qf, p);
+    products<kHalf, HD>(sv[buf], kWhole ? kTile : n, l16, g, gf, dp);
 #pragma unroll
     for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
-      for (int t = 0; t < 4; ++t) p[tt][t] = __builtin_amdgcn_exp2f(fmaf(p[tt][t] - st.x, c_log2, -st.y));
-    if (n < kTile) {  // uniform
-      const int lim = n - 4 * g;
-#pragma unroll
-      for (int tt = 0; tt < 4; ++tt)
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          p[tt][t] = 16 * tt + t < lim ? p[tt][t] : 0.f;
-          dp[tt][t] = 16 * tt + t < lim ? dp[tt][t] : 0.f;
-        }
-    }
+      for (int t = 0; t < 4; ++t) {
+        const bool in = kWhole || 16 * tt + t < n - 4 * g;
+        p[tt][t] = in ? __builtin_amdgcn_exp2f(fmaf(p[tt][t] - st.x, c_log2, -st.y)) : 0.f;
+        dp[tt][t] = in ? dp[tt][t] : 0.f;
+      }
   };
   float dl = 0.f;
   // (a chunk's terms among themselves first: fewer roundings of the long sum)
@@ -316,73 +296,71 @@ relative_bwd_q_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int32
     dl += sum;
   };
   ColumnScale<kHalf> cs;
-  auto spread = [&](int buf, int64_t c, const int (&at)[4][4], f32x4_t (&p)[4], const f32x4_t (&dp)[4]) {
-    const int n = rows_in(c);
+  // ds (in p's place) into the buckets' sums and dq
+  auto spread = [&](auto whole, int buf, int64_t c, int n, f32x4_t (&p)[4], const f32x4_t (&dp)[4]) {
+    constexpr bool kWhole = decltype(whole)::value;
+    int at[4][4];
+    pair_offsets(side, n_latents, sc[buf], int(c * kTile), g, at);
 #pragma unroll
     for (int tt = 0; tt < 4; ++tt) {
-      if (16 * tt >= n) break;  // uniform
-      int to[4];
+      if (!kWhole && 16 * tt >= n) break;  // uniform
+      uint32_t to[4];
       float x[4];
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        p[tt][t] *= dp[tt][t] - dl;
-        x[t] = p[tt][t];
-        to[t] = int(bucket[at[tt][t] / 4]) * row_bytes;
-      }
-      if (n < kTile) {  // uniform: a key past the last one adds nothing, whatever delta is
-#pragma unroll
-        for (int t = 0; t < 4; ++t) p[tt][t] = x[t] = 16 * tt + t < n - 4 * g ? x[t] : 0.f;
+        to[t] = *reinterpret_cast<const uint32_t*>(dynamic + at[tt][t] + 4);
+        x[t] = p[tt][t] * (dp[tt][t] - dl);
+        // (a key past the last one adds nothing, whatever delta is)
+        if (!kWhole) x[t] = 16 * tt + t < n - 4 * g ? x[t] : 0.f;
+        if (kColumns < 16) x[t] = live ? x[t] : 0.f;  // (two queries share a column)
+        p[tt][t] = x[t];
       }
       if constexpr (kColumns == 64) {
         add4(column, to, x);
       } else {
 #pragma unroll
-        for (int turn = 0; turn < 4; ++turn) {
-          if (g == turn) add4(column, to, x);
+        for (int turn = 0; turn < 64 / kColumns; ++turn) {
+          if (lane / kColumns == turn) add4(column, to, x);
           __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (the next group reads what this one wrote)
         }
       }
     }
     cs.apply(p, acc);
-    accumulate_parts<kHalf, HD>(sk[buf], n, l16, g, p, acc);
+    accumulate_parts<kHalf, HD>(sk[buf], kWhole ? kTile : n, l16, g, p, acc);
   };
-  int at[4][4];
   f32x4_t p[4], dp[4];
   const bool working = first < L;  // wavefront-uniform: a live row here
-  if (n_chunks <= 2) {
+  const int tail = int(L - (n_chunks - 1) * kTile);  // rows of the last chunk
+  if (n_chunks == 1) {
+    if (working) {
+      pairs(part, 0, 0, tail, p, dp);
+      sum_delta(p, dp);
+      dl = sum_xor32(sum_xor16(dl));
+      spread(part, 0, 0, tail, p, dp);
+    }
+  } else if (n_chunks == 2) {
     f32x4_t p1[4], dp1[4];
     if (working) {
-      pair_offsets(side, rel, sc[0], 0, g, at);
-      pairs(0, 0, at, p, dp);
+      pairs(full, 0, 0, kTile, p, dp);
       sum_delta(p, dp);
     }
-    if (n_chunks == 2) {
-      stage(1);
-      __syncthreads();
-      if (working) {
-        int at1[4][4];
-        pair_offsets(side, rel, sc[1], kTile, g, at1);
-        pairs(1, 1, at1, p1, dp1);
-        sum_delta(p1, dp1);
-      }
-    }
+    stage(1);
+    __syncthreads();
     if (working) {
+      pairs(part, 1, 1, tail, p1, dp1);
+      sum_delta(p1, dp1);
       dl = sum_xor32(sum_xor16(dl));
-      spread(0, 0, at, p, dp);
-      if (n_chunks == 2) {
-        pair_offsets(side, rel, sc[1], kTile, g, at);
-        spread(1, 1, at, p1, dp1);
-      }
+      spread(full, 0, 0, kTile, p, dp);
+      spread(part, 1, 1, tail, p1, dp1);
     }
   } else {
     // step s: chunk s % n_chunks in buffer s % 2; the first n_chunks for delta
-    for (int64_t s = 0, c = 0; s < 2 * n_chunks; ++s, c = c + 1 < n_chunks ? c + 1 : 0) {
+    auto step = [&](auto whole, int64_t s, int64_t c, int n) {
       const int buf = int(s & 1);
       if (working) {
-        pair_offsets(side, rel, sc[buf], c * kTile, g, at);
-        pairs(buf, c, at, p, dp);
+        pairs(whole, buf, c, n, p, dp);
         if (s < n_chunks) sum_delta(p, dp);
-        else spread(buf, c, at, p, dp);
+        else spread(whole, buf, c, n, p, dp);
         if (s == n_chunks - 1) dl = sum_xor32(sum_xor16(dl));
       }
       if (s + 1 < 2 * n_chunks) {
@@ -390,6 +368,10 @@ relative_bwd_q_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int32
         if (s + 2 < 2 * n_chunks) fetch((s + 2) % n_chunks * kTile);
       }
       __syncthreads();
+    };
+    for (int64_t sweep = 0; sweep < 2 * n_chunks; sweep += n_chunks) {
+      for (int64_t c = 0; c + 1 < n_chunks; ++c) step(full, sweep + c, c, kTile);
+      step(part, sweep + n_chunks - 1, n_chunks - 1, tail);
     }
   }
   if (i < T) {
@@ -397,27 +379,31 @@ relative_bwd_q_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int32
     if (g == 0) delta[pa * T + i] = live ? dl : 0.f;
   }
   __syncthreads();
-  // eight threads to a bucket's columns, starting apart so that they meet other
-  // banks; the shuffles join them
+  // eight threads to a bucket's columns, each those of two queries in every
+  // lane group, the eight starting apart so that a wavefront's reads meet other banks
+  const int first_dead = L - tile * kTile < kTile ? int(L - tile * kTile) : kTile;  // queries of this workgroup
   for (int b0 = 0; b0 < rel.n_buckets; b0 += 32) {
     const int b = b0 + int(threadIdx.x) / 8, eighth = threadIdx.x % 8;
     float sum = 0.f;
     if (b < rel.n_buckets)
       for (int w = 0; w < kBwdWaves; ++w)
 #pragma unroll
-        for (int c = 0; c < kColumns / 8; ++c)
-          sum += columns[(w * n_rows + b) * kColumns + (8 * c + eighth + 8 * (int(threadIdx.x) / 8)) % kColumns];
+        for (int c = 0; c < kColumns / 8; ++c) {
+          const int col = (8 * c + eighth + 8 * (int(threadIdx.x) / 8)) % kColumns;
+          const float x = columns[(w * n_rows + b) * kColumns + col];
+          sum += 16 * w + col % 16 < first_dead ? x : 0.f;
+        }
     sum += __shfl_xor(sum, 1);
     sum += __shfl_xor(sum, 2);
     sum += __shfl_xor(sum, 4);
-    if (b < rel.n_buckets && eighth == 0) part[b] = sum;
+    if (b < rel.n_buckets && eighth == 0) part_sums[b] = sum;
   }
 }
 
 template <bool kHalf, int HD>
 __global__ void __launch_bounds__(256)
 relative_bwd_kv_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int32_t* __restrict__ seq_lens, int heads,
-                       int64_t T, int64_t n_items, const float2* __restrict__ stats, float scale, float root_hd,
+                       int64_t T, int64_t n_pa, const float2* __restrict__ stats, float scale, float root_hd,
                        const float* __restrict__ delta, RowsOut dk, RowsOut dv) {
   using G = Geom<kHalf, HD>;
   using Tile = RowTile<HD>;
@@ -425,12 +411,11 @@ relative_bwd_kv_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int3
   __shared__ __attribute__((aligned(16))) float sm[2][kTile], sl[2][kTile], sd[2][kTile];
   __shared__ __attribute__((aligned(16))) uint32_t sc[2][kTile];
   extern __shared__ __attribute__((aligned(16))) char dynamic[];
-  const int64_t item = int64_t(blockIdx.x % kXcds) * (gridDim.x / kXcds) + blockIdx.x / kXcds;
-  if (item >= n_items) return;
-  float* table = reinterpret_cast<float*>(dynamic);
   const int64_t n_tiles = (T + kTile - 1) / kTile;
-  const int64_t pa = item / n_tiles, tile = item % n_tiles;
-  const int64_t pos = pa / heads, a = pa % heads;
+  const Item item = item_of(n_pa, heads, n_tiles);
+  if (item.pa >= n_pa) return;
+  float* table = reinterpret_cast<float*>(dynamic);
+  const int64_t pa = item.pa, tile = item.tile, pos = pa / heads, a = pa % heads;
   int64_t L = seq_lens[pos];
   L = L < 0 ? 0 : (L > T ? T : L);
   const int lane = threadIdx.x % 64, l16 = lane % 16, g = lane / 16;
@@ -472,25 +457,26 @@ relative_bwd_kv_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int3
     uint4 kf[G::kKs], vf[G::kKs];
     row_frags<kHalf, HD>(rows_of(k, pos, a, L), j, g, kf);
     row_frags<kHalf, HD>(rows_of(v, pos, a, L), j, g, vf);
-    const Side<false> side(rel, coords_of(rel, pos, T, j, L), j < rel.n_latents);
+    const Side<false, 4> side(rel, coords_of(rel, pos, T, j, L), j < rel.n_latents);
+    const int n_latents = int(rel.n_latents);
     stage_bias(rel, a, root_hd, table);
     const float c_log2 = scale * kLog2e;
     stage(0);
     if (kTile < L) fetch(kTile);
     __syncthreads();
-    for (int64_t qb = 0; qb < L; qb += kTile) {
+    auto chunk = [&](auto whole, int64_t qb, int n) {
+      constexpr bool kWhole = decltype(whole)::value;  // (a full chunk has no branch)
       const int buf = int(qb / kTile & 1);
       if (first < L) {  // wavefront-uniform
-        const int n = int(L - qb < kTile ? L - qb : kTile);
         f32x4_t p[4], ds[4];
         int at[4][4];
-        pair_offsets(side, rel, sc[buf], qb, g, at);  // (a latent key's pairs keep its own entry)
+        pair_offsets(side, n_latents, sc[buf], int(qb), g, at);  // (a latent key's pairs keep its own entry)
 #pragma unroll
         for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
           for (int t = 0; t < 4; ++t) p[tt][t] = entry(table, at[tt][t]);
-        products_onto<kHalf, HD>(sq[buf], n, l16, g, kf, p);
-        products<kHalf, HD>(sg[buf], n, l16, g, vf, ds);
+        products_onto<kHalf, HD>(sq[buf], kWhole ? kTile : n, l16, g, kf, p);
+        products<kHalf, HD>(sg[buf], kWhole ? kTile : n, l16, g, vf, ds);
 #pragma unroll
         for (int tt = 0; tt < 4; ++tt) {
           const f32x4_t m4 = *reinterpret_cast<const f32x4_t*>(&sm[buf][16 * tt + 4 * g]);
@@ -498,34 +484,28 @@ relative_bwd_kv_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int3
           const f32x4_t d4 = *reinterpret_cast<const f32x4_t*>(&sd[buf][16 * tt + 4 * g]);
 #pragma unroll
           for (int t = 0; t < 4; ++t) {
-            p[tt][t] = __builtin_amdgcn_exp2f(fmaf(p[tt][t] - m4[t], c_log2, -l4[t]));
-            ds[tt][t] = p[tt][t] * (ds[tt][t] - d4[t]);
+            const bool in = kWhole || 16 * tt + t < n - 4 * g;
+            p[tt][t] = in ? __builtin_amdgcn_exp2f(fmaf(p[tt][t] - m4[t], c_log2, -l4[t])) : 0.f;
+            ds[tt][t] = in ? p[tt][t] * (ds[tt][t] - d4[t]) : 0.f;
           }
-        }
-        if (n < kTile) {  // uniform
-          const int lim = n - 4 * g;  // queries 16 tt + t below it are live
-#pragma unroll
-          for (int tt = 0; tt < 4; ++tt)
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-              p[tt][t] = 16 * tt + t < lim ? p[tt][t] : 0.f;
-              ds[tt][t] = 16 * tt + t < lim ? ds[tt][t] : 0.f;
-            }
         }
         if constexpr (kHalf) {
 #pragma unroll
           for (int tt = 0; tt < 4; ++tt) p[tt] *= kPScale;
         }
-        accumulate_parts<kHalf, HD>(sg[buf], n, l16, g, p, av);
+        accumulate_parts<kHalf, HD>(sg[buf], kWhole ? kTile : n, l16, g, p, av);
         cs.apply(ds, ak);
-        accumulate_parts<kHalf, HD>(sq[buf], n, l16, g, ds, ak);
+        accumulate_parts<kHalf, HD>(sq[buf], kWhole ? kTile : n, l16, g, ds, ak);
       }
       if (qb + kTile < L) {
         stage(buf ^ 1);  // (its readers met the barrier of the chunk before)
         if (qb + 2 * kTile < L) fetch(qb + 2 * kTile);
       }
       __syncthreads();
-    }
+    };
+    const int64_t last = (L - 1) / kTile * kTile;
+    for (int64_t qb = 0; qb < last; qb += kTile) chunk(std::true_type{}, qb, kTile);
+    chunk(std::false_type{}, last, int(L - last));
   }
   if (j < T) {
     store_row<kHalf, HD, true>(dk.row(pos, a, j), g, ak, scale / cs.s, live);
@@ -572,24 +552,34 @@ template <bool kHalf, int HD>
 int32_t launch(const Rows& q, const Rows& k, const Rows& v, const Rows& go, const Relative& rel,
                const int32_t* seq_lens, int64_t n_pos, int heads, int64_t t, const float2* stats, float* delta,
                float* partial, const RowsOut& dq, const RowsOut& dk, const RowsOut& dv, float* dbias, hipStream_t st) {
-  const int64_t n_tiles = (t + kTile - 1) / kTile, n_items = n_pos * heads * n_tiles;
-  const int64_t grid = (n_items + kXcds - 1) / kXcds * kXcds;
+  const int64_t n_tiles = (t + kTile - 1) / kTile, n_pa = n_pos * heads;
+  const int64_t grid = item_grid(n_pos, heads, n_tiles);
   if (grid > 2147483647LL) return MANTIS_E_ARG;
   const float root = sqrtf(float(HD)), scale = 1.f / root;
   const int n_disp = rel.nq * rel.nr;
-  const size_t tables = table_bytes(n_disp) + bucket_bytes(n_disp);
-  const size_t wide = tables + column_bytes(rel.n_buckets, 64), narrow = tables + column_bytes(rel.n_buckets, 16);
-  const bool fits = static_lds<kHalf, HD>() + wide <= kLdsBytes;
-  if (!fits && static_lds<kHalf, HD>() + narrow > kLdsBytes) return MANTIS_E_ARG;
-  auto first = fits ? relative_bwd_q_kernel<kHalf, HD, 64> : relative_bwd_q_kernel<kHalf, HD, 16>;
-  constexpr size_t most = kLdsBytes - static_lds<kHalf, HD>();
-  if (!(fits ? allow_lds<relative_bwd_q_kernel<kHalf, HD, 64>>(most)
-             : allow_lds<relative_bwd_q_kernel<kHalf, HD, 16>>(most)))
-    return MANTIS_E_LAUNCH;
-  first<<<unsigned(grid), 256, fits ? wide : narrow, st>>>(q, k, v, go, rel, seq_lens, heads, t, n_items, stats, scale,
-                                                           root, delta, dq, partial);
-  relative_bwd_kv_kernel<kHalf, HD><<<unsigned(grid), 256, table_bytes(n_disp), st>>>(
-      q, k, v, go, rel, seq_lens, heads, t, n_items, stats, scale, root, delta, dk, dv);
+  // Columns per wavefront: 64 unless that table keeps workgroups off the CU that the
+  // registers would allow (three, with 64 dims two), then 32 or 16 with the lane
+  // groups in turn.  24 to 28 KB of 64 columns a wavefront against 32 and 16: MEASURED2
+  constexpr size_t fixed = static_lds<kHalf, HD>(), share = kLdsBytes / (HD == 64 ? 2 : 3);
+  auto total = [&](int columns) { return fixed + table_bytes(n_disp, 8) + column_bytes(rel.n_buckets, columns); };
+  const int columns = total(64) <= share ? 64 : total(32) <= share ? 32 : total(16) <= kLdsBytes ? 16 : 8;
+  if (total(columns) > kLdsBytes) return MANTIS_E_ARG;
+  auto query_pass = [&](auto kernel, bool allowed) {
+    if (!allowed) return false;
+    kernel<<<unsigned(grid), 256, total(columns) - fixed, st>>>(q, k, v, go, rel, seq_lens, heads, t, n_pa, stats,
+                                                                scale, root, delta, dq, partial);
+    return true;
+  };
+#define MANTIS_QUERY_PASS(C) \
+  query_pass(relative_bwd_q_kernel<kHalf, HD, C>, allow_lds<relative_bwd_q_kernel<kHalf, HD, C>>(kLdsBytes - fixed))
+  const bool queued = columns == 64   ? MANTIS_QUERY_PASS(64)
+                      : columns == 32 ? MANTIS_QUERY_PASS(32)
+                      : columns == 16 ? MANTIS_QUERY_PASS(16)
+                                      : MANTIS_QUERY_PASS(8);
+#undef MANTIS_QUERY_PASS
+  if (!queued) return MANTIS_E_LAUNCH;
+  relative_bwd_kv_kernel<kHalf, HD><<<unsigned(grid), 256, table_bytes(n_disp, 4), st>>>(
+      q, k, v, go, rel, seq_lens, heads, t, n_pa, stats, scale, root, delta, dk, dv);
   relative_bias_sum_kernel<<<unsigned(heads * rel.n_buckets), 256, 0, st>>>(partial, n_pos * n_tiles, rel.n_buckets,
                                                                            dbias);
   return launched();

@@ -7,9 +7,10 @@
 // key's pairs take bucket B - 2, the other pairs of a latent query B - 1.  A
 // workgroup serves one head and holds its bias per displacement in LDS, in
 // raw-score units (bias * sqrt(hd)), where it is the C operand of the score
-// product.  Coordinates are packed as two int16 halves, so an entry's address
-// is a saturating subtraction, two clamps and one two-way dot product:
-// four instructions and one LDS read per pair.
+// product.  Coordinates are packed as two int16 halves and one side carries
+// the half extents, so an entry's address is a saturating subtraction, two
+// clamps and two 16-bit multiply-adds: five instructions and one LDS read per
+// pair.  (A two-way dot product for the last two needs wait states after it.)
 #pragma once
 
 #include "common.hpp"
@@ -17,6 +18,7 @@
 namespace mantis {
 namespace {
 
+constexpr int kXcds = 8;
 constexpr int kMaxDisplacements = 4096;  // entries of a bucket table
 constexpr int kMaxBuckets = 384;
 
@@ -31,9 +33,12 @@ struct Relative {
 
 typedef short s16x2_t __attribute__((ext_vector_type(2)));
 
-// c in int16 as the low half, r as the high one; outside of int16 the flag and the nearest
+constexpr int kMaxCoord = 30000;  // with a half extent of at most 2,047 a sum stays in int16
+
+// c as the low half, r as the high one; past kMaxCoord the flag and the nearest
 __device__ __forceinline__ uint32_t pack_coords(int32_t c, int32_t r, int32_t* flag) {
-  const int32_t cc = c < -32768 ? -32768 : c > 32767 ? 32767 : c, rr = r < -32768 ? -32768 : r > 32767 ? 32767 : r;
+  const int32_t cc = c < -kMaxCoord ? -kMaxCoord : c > kMaxCoord ? kMaxCoord : c;
+  const int32_t rr = r < -kMaxCoord ? -kMaxCoord : r > kMaxCoord ? kMaxCoord : r;
   if (cc != c || rr != r) raise_flag(flag, MANTIS_FLAG_INDEX);
   return uint32_t(uint16_t(cc)) | uint32_t(uint16_t(rr)) << 16;
 }
@@ -71,33 +76,84 @@ __device__ __forceinline__ void stage_bias(const Relative& rel, int64_t head, fl
   }
 }
 
-// This lane's side of its pairs: the byte offset of the entry of a pair with
-// the other side's packed coordinates (kQuery: this lane holds the query).
-template <bool kQuery>
+// This lane's side of its pairs: the byte offset of the table entry (kEntry
+// bytes each) of a pair with the other side's packed coordinates (kQuery: this
+// lane holds the query).  A latent row's pairs all have one entry, which its
+// clamps hold, whatever the displacement.
+template <bool kQuery, int kEntry>
 struct Side {
-  s16x2_t own, lo, hi, mult;
-  int base, latent_other;
+  s16x2_t own, lo, hi;
+  uint32_t row_bytes;  // of the table
+  int latent_other;    // the entry of a pair whose other side is a latent row
   __device__ __forceinline__ Side(const Relative& rel, uint32_t packed, bool latent) {
     const short hq = short((rel.nq - 1) / 2), hr = short((rel.nr - 1) / 2);
-    const int n = rel.nq * rel.nr;
-    own = __builtin_bit_cast(s16x2_t, packed);
-    lo = s16x2_t{short(-hq), short(-hr)};
-    hi = s16x2_t{hq, hr};
-    // a latent row's pairs all have one entry, whatever the displacement
-    mult = latent ? s16x2_t{0, 0} : s16x2_t{short(4 * rel.nr), 4};
-    base = latent ? 4 * (kQuery ? n + 1 : n) : 4 * (hq * rel.nr + hr);
-    // the entry of a pair whose other side is a latent row
-    latent_other = kQuery || latent ? 4 * n : 4 * (n + 1);
+    const s16x2_t half{hq, hr}, c = __builtin_bit_cast(s16x2_t, packed);
+    own = kQuery ? c - half : c + half;
+    lo = latent ? s16x2_t{short(rel.nq), short(kQuery ? 1 : 0)} : s16x2_t{0, 0};
+    hi = latent ? lo : s16x2_t{short(2 * hq), short(2 * hr)};
+    row_bytes = uint32_t(kEntry * rel.nr);
+    latent_other = kEntry * (rel.nq * rel.nr + (kQuery || latent ? 0 : 1));
   }
   __device__ __forceinline__ int at(uint32_t other) const {
     const s16x2_t o = __builtin_bit_cast(s16x2_t, other);
     s16x2_t d = kQuery ? __builtin_elementwise_sub_sat(o, own) : __builtin_elementwise_sub_sat(own, o);
     d = __builtin_elementwise_max(__builtin_elementwise_min(d, hi), lo);
-    return __builtin_amdgcn_sdot2(d, mult, base, false);
+    const uint32_t u = __builtin_bit_cast(uint32_t, d);
+    int r;
+    asm("v_mad_i32_i16 %0, %1, %2, 0 op_sel:[1,0,0,0]" : "=v"(r) : "v"(u), "n"(kEntry));  // (the high half)
+    asm("v_mad_i32_i16 %0, %1, %2, %3" : "=v"(r) : "v"(u), "s"(row_bytes), "v"(r));
+    return r;
   }
 };
-__device__ __forceinline__ float entry(const float* table, int byte_offset) {
-  return *reinterpret_cast<const float*>(reinterpret_cast<const char*>(table) + byte_offset);
+
+// table offsets of this lane's pairs with 64 rows of the other side, row 16 tt + 4 g + t
+// from `first` on, their packed coordinates in LDS
+template <bool kQuery, int kEntry>
+__device__ __forceinline__ void pair_offsets(const Side<kQuery, kEntry>& side, int n_latents, const uint32_t* sc,
+                                             int first, int g, int (&at)[4][4]) {
+#pragma unroll
+  for (int tt = 0; tt < 4; ++tt) {
+    const uint4 c = *reinterpret_cast<const uint4*>(&sc[16 * tt + 4 * g]);
+    const uint32_t cs[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+    for (int t = 0; t < 4; ++t) at[tt][t] = side.at(cs[t]);
+  }
+  if (first < n_latents) {  // uniform
+    asm volatile("");       // (a branch: most chunks hold no latent row)
+    const int lat = n_latents - first - 4 * g;
+#pragma unroll
+    for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+      for (int t = 0; t < 4; ++t) at[tt][t] = 16 * tt + t < lat ? side.latent_other : at[tt][t];
+  }
+}
+__device__ __forceinline__ float entry(const void* table, int byte_offset) {
+  return *reinterpret_cast<const float*>(static_cast<const char*>(table) + byte_offset);
+}
+
+// Work items (position and head, tile of rows) to workgroups, which the
+// dispatcher deals round-robin over the XCDs.  The unit that an XCD takes
+// whole is a position where there are many, so that the heads that share its
+// rows' cache lines share an L2, and a (position, head) where there are few,
+// so that a long position's work is spread.  (Two lines of 2,049-4,096 rows, 8
+// heads, against consecutive items on one XCD: the forward 198 -> 165 us, the
+// backward's passes 585 + 324 -> 508 + 285; 512 positions of 44-124 rows by
+// position 33 us, by head 35.)
+struct Item {
+  int64_t pa, tile;
+};
+constexpr int64_t kManyPositions = 64;
+__device__ __forceinline__ Item item_of(int64_t n_pa, int heads, int64_t n_tiles) {
+  const bool whole = n_pa / heads >= kManyPositions;
+  const uint32_t per = uint32_t(whole ? heads * n_tiles : n_tiles);  // (the grid fits 31 bits)
+  const uint32_t x = blockIdx.x % kXcds, i = blockIdx.x / kXcds, r = i % per;
+  const int64_t unit = int64_t(i / per) * kXcds + x;
+  return Item{whole ? unit * heads + r / uint32_t(n_tiles) : unit, int64_t(r % uint32_t(n_tiles))};
+}
+inline int64_t item_grid(int64_t n_pos, int heads, int64_t n_tiles) {
+  const bool whole = n_pos >= kManyPositions;
+  const int64_t units = whole ? n_pos : n_pos * heads, per = whole ? heads * n_tiles : n_tiles;
+  return (units + kXcds - 1) / kXcds * kXcds * per;
 }
 
 inline bool good_relative(const Relative& rel, int64_t t) {

@@ -834,11 +834,11 @@ int32_t mantis_stone_attention_backward(const void* q, const int64_t* q_strides,
  * int32, both odd, nq * nr <= 4096, its middle entry the zero displacement,
  * indexed by the displacement's two components clamped to +-(nq - 1) / 2 and
  * +-(nr - 1) / 2.  bias (heads, n_buckets) fp32, n_buckets <= 384; coords
- * (P, T, 2) int32 within int16 (latent and pad rows unread).  A bias may be
+ * (P, T, 2) int32 within +-30,000 (latent and pad rows unread).  A bias may be
  * -inf: a live row all of whose keys have it gives zeros and lse -inf (a finite
  * bias past 3.4e38 / sqrt(hd) counts as the lowest or largest finite score).  Rows at
  * or past seq_lens[p] give zeros and lse 0.  A bucket outside [0, n_buckets)
- * counts as bias 0 without a gradient and, as a coordinate outside int16, sets
+ * counts as bias 0 without a gradient and, as a coordinate outside that range, sets
  * MANTIS_FLAG_INDEX.  q/k/v/out as in mantis_stone_attention (a position's
  * rows within 2^31 bytes), fp16 outputs past +-65504 infinite; lse
  * (P, heads, T) and stats (P, heads, T, 2) fp32, the latter what the backward

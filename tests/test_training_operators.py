@@ -479,9 +479,9 @@ def test_relative_attention(device, lens, heads, d, dtype, kw):
 
 @gpu
 def test_relative_attention_far_coordinates_and_extents(device):
-    # clamped displacements past the table, int16's corners (a difference past int16 saturates)
+    # clamped displacements past the table, the coordinates' corners (a difference past int16 saturates)
     case = list(relative_case([50, 50], 2, 32, BF, 3, n_latents=0, table=(9, 5), device=device))
-    corners = torch.tensor([[-32768, 32767], [32767, -32768], [0, 0], [32767, 32767], [-32768, -32768]])
+    corners = torch.tensor([[-30000, 30000], [30000, -30000], [0, 0], [30000, 30000], [-30000, -30000]])
     case[4][0, :5] = corners.to(torch.int32).to(device)
     check_relative(case)
     ops.raise_on_device_error(device)
