@@ -2,6 +2,8 @@
 
 * ``libhexo_encoder.so`` — host C++ (g++), no GPU dependency;
 * ``libmantis_hip.so`` — HIP for gfx950 (hipcc --offload-arch=gfx950);
+* ``libmantis_torch.so`` — the training operators on torch's dispatcher, over
+  ``libmantis_hip.so`` (g++ against the installed torch's headers);
 * ``oracle/liboracle.so`` — the CPU oracle used by the tests (gcc).
 
 Every HIP object is compiled with packed-FP32 instruction selection disabled
@@ -64,13 +66,29 @@ def build_hip() -> Path:
     return out
 
 
+def build_operators() -> Path:
+    import torch  # (its headers and libraries)
+
+    home = Path(torch.__file__).resolve().parent
+    rocm = Path(os.environ.get("ROCM_PATH", "/opt/rocm"))
+    out = PKG / "libmantis_torch.so"
+    _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-Wno-sign-compare", "-Wno-unused-function",
+          "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+          f"-I{home}/include", f"-I{home}/include/torch/csrc/api/include", "-isystem", f"{rocm}/include",
+          "-o", str(out), str(CSRC / "dispatch" / "training_ops.cpp"),
+          f"-L{PKG}", "-lmantis_hip", "-Wl,-rpath,$ORIGIN",
+          f"-L{home}/lib", "-lc10", "-ltorch_cpu", "-ltorch", "-lc10_hip", "-ltorch_hip",
+          f"-L{rocm}/lib", "-lamdhip64"])
+    return out
+
+
 def build_oracle() -> Path:
     _run(["make", "-s", "-C", str(ROOT / "oracle")])
     return ROOT / "oracle" / "liboracle.so"
 
 
 def build_all() -> list[Path]:
-    return [build_encoder(), build_hip(), build_oracle()]
+    return [build_encoder(), build_hip(), build_operators(), build_oracle()]
 
 
 if __name__ == "__main__":

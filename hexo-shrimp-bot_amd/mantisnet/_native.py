@@ -1,11 +1,14 @@
-"""ctypes bindings for the two native libraries of this package.
+"""The native libraries of this package: two behind ctypes bindings, one on
+torch's dispatcher.
 
 * ``libhexo_encoder.so`` — host C++ rules subset + position encoder
   (``include/hexo_encoder.h``).
 * ``libmantis_hip.so`` — the HIP kernels for gfx950 behind a C ABI
   (``include/mantis_hip.h``).
+* ``libmantis_torch.so`` — the training operators over that ABI
+  (``csrc/dispatch/training_ops.cpp``).
 
-Both are built in-tree by ``__graft_entry__.build()``.  There is no fallback:
+All are built in-tree by ``__graft_entry__.build()``.  There is no fallback:
 a missing library raises ``RuntimeError`` naming the file, so a GPU run can
 never silently take another path.
 """
@@ -19,6 +22,7 @@ from pathlib import Path
 PKG_ROOT = Path(__file__).resolve().parents[1]
 ENCODER_LIB = PKG_ROOT / "libhexo_encoder.so"
 HIP_LIB = PKG_ROOT / "libmantis_hip.so"
+TORCH_LIB = PKG_ROOT / "libmantis_torch.so"
 
 _encoder = None
 _hip = None
@@ -34,12 +38,17 @@ class NativeError(RuntimeError):
     """A native entry point returned a nonzero status."""
 
 
-def _load(path: Path) -> ctypes.CDLL:
+def _built(path: Path) -> Path:
     if not path.exists():
         raise RuntimeError(
             f"{path.name} is not built at {path}; run __graft_entry__.build() "
             "(the MantisNet path has no fallback)"
         )
+    return path
+
+
+def _load(path: Path) -> ctypes.CDLL:
+    _built(path)
     return ctypes.CDLL(str(path), mode=os.RTLD_LOCAL)
 
 
@@ -95,6 +104,13 @@ def hip() -> ctypes.CDLL:
 
         _hip = _hip_api.bind(_load(HIP_LIB))
     return _hip
+
+
+def load_operators() -> None:
+    """Register the natively written operators (once per process)."""
+    import torch
+
+    torch.ops.load_library(str(_built(TORCH_LIB)))
 
 
 def check(status: int, err: ctypes.Array | None = None, what: str = "") -> None:

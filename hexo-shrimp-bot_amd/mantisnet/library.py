@@ -37,7 +37,7 @@ from __future__ import annotations
 import torch
 from torch import Tensor
 
-from . import ops, tables
+from . import _native, ops, tables
 
 _NS = "mantisnet"
 
@@ -589,153 +589,19 @@ def _(window_pos, positions):
 
 # ----------------------------------------------------------------- training around the stone attention
 
-# These operators carry their gradient as an autograd function on the
-# dispatcher's Autograd key instead of the decorator's generated one: the same
-# dispatch and tracing with 39 instead of 58 us of host time for a call and its
-# backward, which is most of the time of a small batch.
-_LIB = torch.library.Library(_NS, "FRAGMENT")
-
-
-def _define(schema: str, kernel, fake, autograd=None) -> None:
-    """Register an operator: its kernel (which refuses CPU tensors itself),
-    its fake and, given the autograd.Function, its gradient."""
-    name = schema[:schema.index("(")]
-    _LIB.define(schema)
-    _LIB.impl(name, kernel, "CompositeExplicitAutograd")
-    torch.library.register_fake(f"{_NS}::{name}", fake, lib=_LIB)
-    if autograd is None:
-        return
-
-    def differentiable(*args):
-        if torch.is_grad_enabled() and any(isinstance(a, Tensor) and a.requires_grad for a in args):
-            return autograd.apply(*args)
-        return _below(name)(*args)
-
-    _LIB.impl(name, differentiable, "Autograd")
-
-
-def _below(name: str):
-    """The operator without its Autograd key."""
-    op = getattr(getattr(torch.ops, _NS), name).default
-
-    def call(*args):
-        with torch._C._AutoDispatchBelowAutograd():
-            return op(*args)
-
-    return call
-
-
-class _RelativeAttention(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, bias, coords, buckets, seq_lens, n_latents):
-        out, lse, stats = _below("fused_attention_relative")(q, k, v, bias, coords, buckets, seq_lens, n_latents)
-        ctx.save_for_backward(q, k, v, bias, coords, buckets, seq_lens, stats)
-        ctx.n_latents = n_latents
-        ctx.mark_non_differentiable(lse, stats)
-        ctx.set_materialize_grads(False)
-        return out, lse, stats
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad_out, _grad_lse, _grad_stats):
-        q, k, v, bias, coords, buckets, seq_lens, stats = ctx.saved_tensors
-        if grad_out is None:
-            return (None,) * 8
-        grads = torch.ops.mantisnet.fused_attention_relative_backward(q, k, v, bias, coords, buckets, seq_lens,
-                                                                      ctx.n_latents, stats, grad_out)
-        return *grads, None, None, None, None
-
-
-# Ragged attention over each position's live prefix with a learned bias by the
-# two rows' relative position: bias (A, buckets), coords (P, T, 2) int32
-# (Batch.coords), buckets the displacement's bucket (tables.relative_buckets),
-# the first n_latents rows (Batch: 4) without coordinates.  Returns (out like
-# q, lse (P, A, T) fp32, stats for the backward); differentiable in q, k, v and bias.
-_define("fused_attention_relative(Tensor q, Tensor k, Tensor v, Tensor bias, Tensor coords, Tensor buckets, "
-        "Tensor seq_lens, int n_latents) -> (Tensor, Tensor, Tensor)",
-        ops.relative_attention,
-        lambda q, k, v, bias, coords, buckets, seq_lens, n_latents: (
-            torch.empty_like(q), q.new_empty(q.shape[:3], dtype=torch.float32),
-            q.new_empty((*q.shape[:3], 2), dtype=torch.float32)),
-        _RelativeAttention)
-
-# (dq, dk, dv, dbias) of fused_attention_relative; pad rows and keys get zero gradients.
-_define("fused_attention_relative_backward(Tensor q, Tensor k, Tensor v, Tensor bias, Tensor coords, Tensor buckets, "
-        "Tensor seq_lens, int n_latents, Tensor stats, Tensor grad_out) -> (Tensor, Tensor, Tensor, Tensor)",
-        ops.relative_attention_backward,
-        lambda q, k, v, bias, coords, buckets, seq_lens, n_latents, stats, grad_out: (
-            torch.empty_like(q), torch.empty_like(k), torch.empty_like(v),
-            torch.empty_like(bias, memory_format=torch.contiguous_format)))
-
-
-class _PolicyLogProbs(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, offsets, moves, top):
-        out = _below("policy_log_probs")(logits, offsets, moves, top)
-        _log_probs, entropy, _lse, _top_log_probs, top_moves, norm = out
-        ctx.save_for_backward(logits, offsets, moves, top_moves, entropy, norm)
-        ctx.mark_non_differentiable(top_moves, norm)
-        ctx.set_materialize_grads(False)
-        return out
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad_log_probs, grad_entropy, grad_lse, grad_top, _grad_moves, _grad_norm):
-        return torch.ops.mantisnet.policy_log_probs_backward(*ctx.saved_tensors, grad_log_probs, grad_entropy,
-                                                             grad_lse, grad_top), None, None, None
-
-
-# Over each position's run of logits (legal order): the log probabilities of
-# moves (P, G) (-1: none), the entropy, the log-sum-exp and the `top` best
-# moves with their log probabilities; norm for the backward.  Differentiable
-# in the logits through the first four.
-_define("policy_log_probs(Tensor logits, Tensor offsets, Tensor moves, int top) -> "
-        "(Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)",
-        ops.policy_log_probs,
-        lambda logits, offsets, moves, top: (
-            *(logits.new_empty(shape, dtype=torch.float32) for shape in (
-                moves.shape, moves.shape[:1], moves.shape[:1], (moves.shape[0], top))),
-            moves.new_empty((moves.shape[0], top)), logits.new_empty((moves.shape[0], 2), dtype=torch.float32)),
-        _PolicyLogProbs)
-
-# The logits' gradient of policy_log_probs (a missing gradient is zero).
-_define("policy_log_probs_backward(Tensor logits, Tensor offsets, Tensor moves, Tensor top_moves, Tensor entropy, "
-        "Tensor norm, Tensor? grad_log_probs, Tensor? grad_entropy, Tensor? grad_lse, Tensor? grad_top) -> Tensor",
-        ops.policy_log_probs_backward,
-        lambda logits, *rest: torch.empty_like(logits, memory_format=torch.contiguous_format))
-
-
-class _ResidualDropout(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, residual, rng, p, salt):
-        out = _below("residual_dropout")(x, residual, rng, p, salt)
-        ctx.save_for_backward(rng)  # (a step counted on before the backward is an error there)
-        ctx.call = p, salt, x.dtype
-        ctx.set_materialize_grads(False)
-        return out
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad_out):
-        if grad_out is None:
-            return (None,) * 5
-        dx = None
-        if ctx.needs_input_grad[0]:
-            dx = torch.ops.mantisnet.residual_dropout_backward(grad_out, *ctx.saved_tensors, *ctx.call)
-        return dx, grad_out if ctx.needs_input_grad[1] else None, None, None, None
-
-
-# residual + dropout(x) (residual None: dropout(x)) with a mask that is drawn
-# again in the backward: rng (2,) int64 = (seed, step), salt per branch.
-_define("residual_dropout(Tensor x, Tensor? residual, Tensor rng, float p, int salt) -> Tensor",
-        ops.residual_dropout,
-        lambda x, residual, rng, p, salt: x.new_empty(x.shape, dtype=(x if residual is None else residual).dtype),
-        _ResidualDropout)
-
-# x's gradient of residual_dropout, in `dtype`.
-_define("residual_dropout_backward(Tensor grad_out, Tensor rng, float p, int salt, ScalarType dtype) -> Tensor",
-        ops.residual_dropout_backward,
-        lambda grad_out, rng, p, salt, dtype: grad_out.new_empty(grad_out.shape, dtype=dtype))
+# fused_attention_relative, policy_log_probs, residual_dropout and their
+# backwards, registered natively (csrc/dispatch/training_ops.cpp): schemas,
+# kernels, fakes and gradients.
+#
+# fused_attention_relative(q, k, v, bias, coords, buckets, seq_lens, n_latents) -> (out, lse, stats):
+#   fused_attention with a learned bias by the two rows' relative position;
+#   differentiable in q, k, v and bias.
+# policy_log_probs(logits, offsets, moves, top) -> (log_probs, entropy, lse, top_log_probs, top_moves, norm):
+#   over each position's run of logits; differentiable in the logits through
+#   the first four.
+# residual_dropout(x, residual, rng, p, salt) -> out: residual + dropout(x), the
+#   mask drawn again in the backward; differentiable in x and residual.
+_native.load_operators()
 
 
 OPERATORS = (

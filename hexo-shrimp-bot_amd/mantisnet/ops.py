@@ -11,7 +11,6 @@ is no CPU or PyTorch fallback: a CPU tensor is refused.
 from __future__ import annotations
 
 import ctypes
-from contextlib import nullcontext
 from typing import NamedTuple
 
 import torch
@@ -167,7 +166,10 @@ def _flag_words(device: torch.device) -> Tensor:
     idx = device.index if device.index is not None else torch.cuda.current_device()
     f = _flags.get(idx)
     if f is None:
-        f = torch.zeros(2, dtype=torch.int32, device=device)
+        f = torch.ops.mantisnet.error_words(idx)  # (the dispatcher's operators may have made them)
+        if f is None:
+            f = torch.zeros(2, dtype=torch.int32, device=device)
+            torch.ops.mantisnet.set_error_words(f)
         _flags[idx] = f
     return f
 
@@ -207,7 +209,9 @@ def raise_on_bits(device: torch.device, bits: int) -> None:
 
 def raise_on_device_error(device: torch.device | None = None) -> None:
     """Raise if any kernel since the last check flagged bad indices."""
-    devs = [device] if device is not None else [torch.device("cuda", i) for i in list(_flags)]
+    devs = [device] if device is not None else [
+        torch.device("cuda", i) for i in range(torch.cuda.device_count())
+        if i in _flags or torch.ops.mantisnet.error_words(i) is not None]
     for d in devs:
         raise_on_bits(d, int(error_flag(d).item()))
 
@@ -1792,81 +1796,9 @@ def stone_attention(q: Tensor, k: Tensor, v: Tensor, seq_lens: Tensor, want_lse:
 
 # ----------------------------------------------------------------- relative attention, policy, dropout
 
-
-def _on_device(dev: torch.device):
-    """A guard that makes ``dev`` current where it is not: these operators
-    launch on their inputs' device, on its current stream."""
-    return nullcontext() if dev.index == _cur_device() else torch.cuda.device(dev)
-
-
-def _checked_flag(dev: torch.device) -> Tensor:
-    """The device's error flag; refuses to make it inside a graph capture,
-    where its memory would belong to the graph and be cleared by replays only."""
-    if dev.index not in _flags and torch.cuda.is_current_stream_capturing():
-        raise RuntimeError("the device's error flag does not exist yet: run the operator once before capturing it")
-    return error_flag(dev)
-
-
-def _row_strides(t: Tensor) -> tuple[int, int, int, int] | None:
-    """Element strides of a (P, A, T, D) operand as the row kernels take them
-    (a dimension of one entry has no stride of its own), or None where its
-    rows are not dense, aligned and within their descriptors."""
-    p, a, n, d = t.shape
-    sp, sa, st, sd = t.stride()
-    if p == 1:
-        sp = 0
-    if a == 1:
-        sa = 0
-    if n == 1:
-        st = d
-    if sd != 1 or (sp | sa | st) % 8 or t.data_ptr() % 16 or not d <= st < 8192 or n * st * 2 > 0x7FFFFFFF:
-        return None
-    return sp, sa, st, 1
-
-
-def _head_rows(t: Tensor) -> tuple[Tensor, ctypes.Array]:
-    """A (P, A, T, D) operand and its strides, copied where its rows have to be."""
-    strides = _row_strides(t)
-    if strides is None:
-        t = t.clone(memory_format=torch.contiguous_format)
-        strides = _row_strides(t)
-        if strides is None:
-            raise ValueError("a position's rows are past the kernel's 2 GiB")
-    return t, (ctypes.c_int64 * 4)(*strides)
-
-
-def _head_rows_like(t: Tensor) -> tuple[Tensor, ctypes.Array]:
-    """An empty operand in t's layout, or a contiguous one where that layout's rows are not the kernel's."""
-    y = torch.empty_like(t)
-    strides = _row_strides(y)
-    if strides is None:
-        y = torch.empty(t.shape, dtype=t.dtype, device=t.device)
-        strides = _row_strides(y)
-    return y, (ctypes.c_int64 * 4)(*strides)
-
-
-def _check_relative(q, k, v, bias, coords, buckets, seq_lens, n_latents) -> None:
-    if q.ndim != 4 or q.shape != k.shape or q.shape != v.shape:
-        raise ValueError("q, k and v must have the same (P, A, T, D) shape")
-    p, heads, t, hd = q.shape
-    if q.dtype not in (torch.float16, torch.bfloat16) or k.dtype != q.dtype or v.dtype != q.dtype:
-        raise ValueError("relative attention runs 16-bit MFMA: q, k and v must share float16 or bfloat16")
-    if hd not in (16, 32, 64):
-        raise ValueError("relative attention supports head_dim 16, 32 and 64")
-    if seq_lens.shape != (p,) or seq_lens.dtype != torch.int32:
-        raise ValueError("seq_lens must be int32 with shape (P,)")
-    if bias.ndim != 2 or bias.shape[0] != heads or not bias.is_floating_point():
-        raise ValueError("bias must be floating point with shape (heads, buckets)")
-    if not 1 <= bias.shape[1] <= 384:
-        raise ValueError("bias must hold 1 to 384 buckets")
-    if coords.shape != (p, t, 2) or coords.dtype != torch.int32:
-        raise ValueError("coords must be int32 with shape (P, T, 2)")
-    if buckets.ndim != 2 or buckets.dtype != torch.int32 or any(n % 2 == 0 for n in buckets.shape):
-        raise ValueError("buckets must be int32 with an odd number of rows and of columns")
-    if buckets.numel() > 4096:
-        raise ValueError("buckets must hold at most 4096 displacements")
-    if not 0 <= n_latents <= t or (n_latents and bias.shape[1] < 2):
-        raise ValueError("n_latents must lie in [0, T], with two buckets of their own")
+# Their argument checks, outputs and launches are the operators' own, on
+# torch's dispatcher (csrc/dispatch/training_ops.cpp); these name them beside
+# the others and let a trace see them.
 
 
 def relative_attention(q: Tensor, k: Tensor, v: Tensor, bias: Tensor, coords: Tensor, buckets: Tensor,
@@ -1877,32 +1809,11 @@ def relative_attention(q: Tensor, k: Tensor, v: Tensor, bias: Tensor, coords: Te
     ``Batch.coords`` holds them, buckets the displacement's bucket
     (``tables.relative_buckets``), the first n_latents rows without
     coordinates.  out has q's layout; lse (P, A, T) and stats (P, A, T, 2)
-    fp32, stats for the backward."""
-    dev = _on_gpu(q, k, v, bias, coords, buckets, seq_lens)
-    _check_relative(q, k, v, bias, coords, buckets, seq_lens, n_latents)
-    p, heads, t, hd = q.shape
-    (q, qs), (k, ks), (v, vs) = _head_rows(q), _head_rows(k), _head_rows(v)
-    out, os_ = _head_rows_like(q)
-    lse = torch.empty((p, heads, t), dtype=torch.float32, device=dev)
-    stats = torch.empty((p, heads, t, 2), dtype=torch.float32, device=dev)
-    if out.numel() == 0:
-        return out, lse, stats
-    bias, coords, buckets, seq_lens = bias.float().contiguous(), _i32x2(coords), buckets.contiguous(), seq_lens.contiguous()
+    fp32, stats for the backward.  Differentiable in q, k, v and bias."""
+    p, heads, t, hd = q.shape if q.ndim == 4 else (0, 0, 0, 0)
     nbytes = p * t * heads * (4 * hd * q.element_size() + 12)
-    with _on_device(dev):
-        _launch("relative_attention", nbytes, 0.0, lambda: _check(
-            _lib().mantis_relative_attention(
-                _ptr(q), qs, _ptr(k), ks, _ptr(v), vs, _dt(q), _ptr(bias), bias.shape[1], _ptr(coords), _ptr(buckets),
-                buckets.shape[0], buckets.shape[1], n_latents, _ptr(seq_lens), p, heads, t, hd, _ptr(out), os_,
-                _ptr(lse), _ptr(stats), _ptr(_checked_flag(dev)), _stream()),
-            "relative_attention"))
-    return out, lse, stats
-
-
-def _i32x2(coords: Tensor) -> Tensor:
-    """Contiguous coordinates whose pairs are 8-byte aligned."""
-    coords = coords.contiguous()
-    return coords if coords.data_ptr() % 8 == 0 else coords.clone()
+    return _launch("relative_attention", nbytes, 0.0, lambda: torch.ops.mantisnet.fused_attention_relative(
+        q, k, v, bias, coords, buckets, seq_lens, n_latents))
 
 
 def relative_attention_backward(q: Tensor, k: Tensor, v: Tensor, bias: Tensor, coords: Tensor, buckets: Tensor,
@@ -1910,51 +1821,11 @@ def relative_attention_backward(q: Tensor, k: Tensor, v: Tensor, bias: Tensor, c
                                 grad_out: Tensor) -> tuple[Tensor, Tensor, Tensor, Tensor]:
     """(dq, dk, dv, dbias) of relative_attention, given its stats: dq, dk and dv
     in q's dtype and their operand's layout, dbias in bias's dtype."""
-    dev = _on_gpu(q, k, v, bias, coords, buckets, seq_lens, stats, grad_out)
-    _check_relative(q, k, v, bias, coords, buckets, seq_lens, n_latents)
-    p, heads, t, hd = q.shape
-    if grad_out.shape != q.shape:
-        raise ValueError("grad_out must have q's shape")
-    if stats.shape != (p, heads, t, 2) or stats.dtype != torch.float32:
-        raise ValueError("stats must be the forward's (P, A, T, 2) fp32 statistics")
-    (q, qs), (k, ks), (v, vs), (go, gs) = (_head_rows(x) for x in (q, k, v, grad_out.to(q.dtype)))
-    (dq, dqs), (dk, dks), (dv, dvs) = (_head_rows_like(x) for x in (q, k, v))
-    if dq.numel() == 0:
-        return dq, dk, dv, torch.zeros_like(bias, memory_format=torch.contiguous_format)
-    bias32, coords, buckets = bias.float().contiguous(), _i32x2(coords), buckets.contiguous()
-    seq_lens, stats = seq_lens.contiguous(), stats.contiguous()
-    n_buckets = bias.shape[1]
-    dbias = torch.empty((heads, n_buckets), dtype=torch.float32, device=dev)
-    ws = _workspace(_lib().mantis_relative_attention_backward_workspace(p, heads, t, n_buckets), dev)
+    p, heads, t, hd = q.shape if q.ndim == 4 else (0, 0, 0, 0)
     nbytes = p * t * heads * (7 * hd * q.element_size() + 8)
-    with _on_device(dev):
-        _launch("relative_attention_backward", nbytes, 0.0, lambda: _check(
-            _lib().mantis_relative_attention_backward(
-                _ptr(q), qs, _ptr(k), ks, _ptr(v), vs, _ptr(go), gs, _ptr(stats), _dt(q), _ptr(bias32), n_buckets,
-                _ptr(coords), _ptr(buckets), buckets.shape[0], buckets.shape[1], n_latents, _ptr(seq_lens), p, heads,
-                t, hd, _ptr(ws), ws.numel(), _ptr(dq), dqs, _ptr(dk), dks, _ptr(dv), dvs, _ptr(dbias),
-                _ptr(_checked_flag(dev)), _stream()),
-            "relative_attention_backward"))
-    return dq, dk, dv, dbias.to(bias.dtype)
-
-
-def _check_policy(logits: Tensor, offsets: Tensor, moves: Tensor, top: int) -> tuple[Tensor, int, Tensor, Tensor]:
-    """(logits, stride, offsets, moves) as the kernels take them."""
-    if logits.ndim != 1:
-        raise ValueError("logits must be flat (N,)")
-    _dt(logits)
-    if offsets.ndim != 1 or offsets.numel() < 1:
-        raise ValueError("offsets must hold P + 1 entries")
-    if moves.ndim != 2 or moves.shape[0] != offsets.numel() - 1:
-        raise ValueError("moves must have shape (P, moves)")
-    if moves.shape[1] > 1024:
-        raise ValueError("at most 1024 moves of a position")
-    if not 0 <= top <= 64:
-        raise ValueError(f"top must lie in [0, 64], got {top}")
-    stride = logits.stride(0) if logits.numel() > 1 else 1
-    if stride < 1:
-        logits, stride = logits.contiguous(), 1
-    return logits, stride, _i64(offsets, "offsets"), _i64(moves, "moves")
+    return _launch("relative_attention_backward", nbytes, 0.0,
+                   lambda: torch.ops.mantisnet.fused_attention_relative_backward(
+                       q, k, v, bias, coords, buckets, seq_lens, n_latents, stats, grad_out))
 
 
 def policy_log_probs(logits: Tensor, offsets: Tensor, moves: Tensor,
@@ -1964,24 +1835,11 @@ def policy_log_probs(logits: Tensor, offsets: Tensor, moves: Tensor,
     run of logits (see mantis_policy_log_probs): logits (N,) fp32, fp16 or
     bf16 with any stride (``ModelOutput.policy_logits``), offsets
     ``Batch.legal_offsets``, moves (P, G) int64 indices in legal order, -1 for
-    none.  Everything else is fp32; norm is for the backward."""
-    dev = _on_gpu(logits, offsets, moves)
-    logits, stride, offsets, moves = _check_policy(logits, offsets, moves, top)
-    p, g, n = moves.shape[0], moves.shape[1], logits.numel()
-    new = lambda *shape: torch.empty(shape, dtype=torch.float32, device=dev)  # noqa: E731
-    log_probs, entropy, lse, top_log, norm = new(p, g), new(p), new(p), new(p, top), new(p, 2)
-    top_moves = torch.empty((p, top), dtype=torch.int64, device=dev)
-    if p:
-        need = _lib().mantis_policy_log_probs_workspace(p, n, top)
-        ws = _workspace(need, dev) if need else None
-        with _on_device(dev):
-            _launch("policy_log_probs", n * logits.element_size() + p * (12 * (g + top) + 24), 6 * n, lambda: _check(
-                _lib().mantis_policy_log_probs(
-                    _ptr(logits), _dt(logits), stride, _ptr(offsets), p, n, _ptr(moves), g, top, _ptr(log_probs),
-                    _ptr(entropy), _ptr(lse), _ptr(top_log), _ptr(top_moves), _ptr(norm), _ptr(ws), need,
-                    _ptr(_checked_flag(dev)), _stream()),
-                "policy_log_probs"))
-    return log_probs, entropy, lse, top_log, top_moves, norm
+    none.  Everything else is fp32; norm is for the backward.  Differentiable
+    in the logits through the first four."""
+    nbytes = logits.numel() * logits.element_size() + 12 * moves.numel() + offsets.numel() * (24 + 12 * top)
+    return _launch("policy_log_probs", nbytes, 6 * logits.numel(),
+                   lambda: torch.ops.mantisnet.policy_log_probs(logits, offsets, moves, top))
 
 
 def policy_log_probs_backward(logits: Tensor, offsets: Tensor, moves: Tensor, top_moves: Tensor, entropy: Tensor,
@@ -1990,57 +1848,10 @@ def policy_log_probs_backward(logits: Tensor, offsets: Tensor, moves: Tensor, to
     """The logits' gradient of policy_log_probs, (N,) in their dtype, from the
     gradients of its first four outputs (None: zero) and its top_moves,
     entropy and norm."""
-    dev = _on_gpu(logits, offsets, moves, top_moves, entropy, norm, grad_log_probs, grad_entropy, grad_lse, grad_top)
-    p, top = top_moves.shape
-    logits, stride, offsets, moves = _check_policy(logits, offsets, moves, top)
-    g, n = moves.shape[1], logits.numel()
-    if offsets.numel() != p + 1 or entropy.shape != (p,) or norm.shape != (p, 2):
-        raise ValueError("top_moves, entropy and norm must be the forward's")
-    if entropy.dtype != torch.float32 or norm.dtype != torch.float32:
-        raise ValueError("entropy and norm must be float32")
-    grads = []
-    for name, grad, shape in (("log_probs", grad_log_probs, (p, g)), ("entropy", grad_entropy, (p,)),
-                              ("lse", grad_lse, (p,)), ("top_log_probs", grad_top, (p, top))):
-        if grad is not None and grad.shape != shape:
-            raise ValueError(f"the gradient of {name} must have shape {shape}")
-        grads.append(None if grad is None else grad.float().contiguous())
-    top_moves, entropy, norm = _i64(top_moves, "top_moves"), entropy.contiguous(), norm.contiguous()
-    out = torch.empty(n, dtype=logits.dtype, device=dev)
-    if p == 0:
-        return out.zero_()
-    if n:
-        with _on_device(dev):
-            _launch("policy_log_probs_backward", 2 * n * logits.element_size(), 6 * n, lambda: _check(
-                _lib().mantis_policy_log_probs_backward(
-                    _ptr(logits), _dt(logits), stride, _ptr(offsets), p, n, _ptr(moves), g, top, _ptr(top_moves),
-                    _ptr(entropy), _ptr(norm), _ptr(grads[0]), _ptr(grads[1]), _ptr(grads[2]), _ptr(grads[3]),
-                    _ptr(out), _ptr(_checked_flag(dev)), _stream()),
-                "policy_log_probs_backward"))
-    return out
-
-
-def _check_dropout(x: Tensor, rng: Tensor, p: float, salt: int) -> None:
-    _dt(x)
-    if rng.shape != (2,) or rng.dtype != torch.int64:
-        raise ValueError("rng must hold two int64, (seed, step)")
-    if not 0.0 <= p <= 1.0:
-        raise ValueError(f"the dropout probability must lie in [0, 1], got {p}")
-    if not 0 <= salt < 1 << 32:
-        raise ValueError(f"salt must lie in [0, 2^32), got {salt}")
-
-
-def _dropout(x: Tensor, residual: Tensor | None, rng: Tensor, p: float, salt: int, out: Tensor) -> Tensor:
-    if out.numel():
-        dev = out.device
-        x, rng = x.contiguous(), rng.contiguous()
-        residual = None if residual is None else residual.contiguous()
-        nbytes = x.numel() * (x.element_size() + out.element_size() * (1 if residual is None else 2))
-        with _on_device(dev):
-            _launch("residual_dropout", nbytes, 2 * x.numel(), lambda: _check(
-                _lib().mantis_residual_dropout(_ptr(x), _dt(x), _ptr(residual), _ptr(rng), x.numel(), float(p), salt,
-                                               _ptr(out), _dt(out), _stream()),
-                "residual_dropout"))
-    return out
+    return _launch("policy_log_probs_backward", 2 * logits.numel() * logits.element_size(), 6 * logits.numel(),
+                   lambda: torch.ops.mantisnet.policy_log_probs_backward(
+                       logits, offsets, moves, top_moves, entropy, norm, grad_log_probs, grad_entropy, grad_lse,
+                       grad_top))
 
 
 def residual_dropout(x: Tensor, residual: Tensor | None, rng: Tensor, p: float, salt: int = 0) -> Tensor:
@@ -2048,25 +1859,18 @@ def residual_dropout(x: Tensor, residual: Tensor | None, rng: Tensor, p: float, 
     dtype (x's without one): an entry is kept, and scaled by 1 / (1 - p), with
     probability 1 - p, by the words of a counter-based generator at its
     row-major index (see mantis_residual_dropout).  rng: (seed, step) int64 on
-    the device, one step per training step; salt tells a step's branches apart."""
-    dev = _on_gpu(x, residual, rng)
-    _check_dropout(x, rng, p, salt)
-    if residual is not None:
-        _dt(residual)
-        if residual.shape != x.shape:
-            raise ValueError("x and residual must have one shape")
-    out = torch.empty(x.shape, dtype=x.dtype if residual is None else residual.dtype, device=dev)
-    return _dropout(x, residual, rng, p, salt, out)
+    the device, one step per training step; salt tells a step's branches
+    apart.  Differentiable in x and residual; the backward draws the mask again."""
+    nbytes = x.numel() * (2 * x.element_size() + (0 if residual is None else 2 * residual.element_size()))
+    return _launch("residual_dropout", nbytes, 2 * x.numel(),
+                   lambda: torch.ops.mantisnet.residual_dropout(x, residual, rng, p, salt))
 
 
 def residual_dropout_backward(grad_out: Tensor, rng: Tensor, p: float, salt: int, dtype: torch.dtype) -> Tensor:
     """x's gradient of residual_dropout in ``dtype``: the incoming gradient
     under the same mask (the residual's gradient is the incoming one)."""
-    dev = _on_gpu(grad_out, rng)
-    _check_dropout(grad_out, rng, p, salt)
-    out = torch.empty(grad_out.shape, dtype=dtype, device=dev)
-    _dt(out)
-    return _dropout(grad_out, None, rng, p, salt, out)
+    return _launch("residual_dropout_backward", 2 * grad_out.numel() * grad_out.element_size(), grad_out.numel(),
+                   lambda: torch.ops.mantisnet.residual_dropout_backward(grad_out, rng, p, salt, dtype))
 
 
 # ----------------------------------------------------------------- fused row GEMM

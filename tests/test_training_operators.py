@@ -341,19 +341,19 @@ def test_fakes_and_refusals():
                 {"buckets": new(65, 65, dtype=torch.int32)}, {"seq_lens": new(2, dtype=i64)},
                 {"seq_lens": new(3, dtype=torch.int32)}, {"n_latents": -1}, {"n_latents": 10}):
             with pytest.raises(ValueError):
-                ops._check_relative(*_fake_relative(**change))
+                OPS.fused_attention_relative(*_fake_relative(**change))
         good = (new(50), new(4, dtype=i64), new(3, 2, dtype=i64), 5)
         for at, bad in ((0, new(50, 1)), (0, new(50, dtype=torch.float64)), (0, new(50, dtype=i64)), (1, new(4)),
                         (1, new(0, dtype=i64)), (2, new(3, dtype=i64)), (2, new(2, 2, dtype=i64)), (2, new(3, 2)),
                         (2, new(3, 1025, dtype=i64)), (3, -1), (3, 65)):
             with pytest.raises(ValueError):
-                ops._check_policy(*(bad if i == at else x for i, x in enumerate(good)))
+                OPS.policy_log_probs(*(bad if i == at else x for i, x in enumerate(good)))
         for x, rng, p, salt in ((new(3, dtype=i64), new(2, dtype=i64), 0.1, 0), (new(3), new(3, dtype=i64), 0.1, 0),
                                 (new(3), new(2), 0.1, 0), (new(3), new(2, dtype=i64), -0.1, 0),
                                 (new(3), new(2, dtype=i64), 1.1, 0), (new(3), new(2, dtype=i64), math.nan, 0),
                                 (new(3), new(2, dtype=i64), 0.1, -1), (new(3), new(2, dtype=i64), 0.1, 1 << 32)):
             with pytest.raises(ValueError):
-                ops._check_dropout(x, rng, p, salt)
+                OPS.residual_dropout(x, None, rng, p, salt)
 
 
 def test_native_argument_checks():
