@@ -13,10 +13,11 @@
 //
 // Forward: one pass over the logits, each lane with its own running maximum,
 // sum and weighted sum in fp32, joined by shuffles and through LDS in a fixed
-// order.  The best entries of a wavefront are a sorted list across its lanes:
-// an entry that beats the last one is inserted by a ballot and a one-lane shift,
-// so the pass costs two comparisons per entry and about top * ln(n / top)
-// insertions.  One workgroup per run; long runs are cut into slices over
+// order.  The best entries of a wavefront are a list of 64-bit keys (value,
+// then index) sorted across its lanes, joined by VALU lane moves: entries that
+// beat the last one are inserted one by one where they are few, and sorted and
+// merged as 64 where they are many (a run's first), so the pass costs a
+// comparison per 16 bytes and about top * ln(n / top) insertions.  One workgroup per run; long runs are cut into slices over
 // several workgroups whose partial results a second launch joins.
 #include "common.hpp"
 
@@ -87,43 +88,108 @@ __device__ __forceinline__ State wave_join(State s) {
   return s;
 }
 
-// The best `top` entries of a wavefront: lane r holds the r-th.
+// The value of lane ^ X: VALU lane moves, no LDS round trip.
+template <int X>
+__device__ __forceinline__ uint32_t from_lane_xor(uint32_t x) {
+  constexpr int kDpp = X == 1 ? 0xB1 : X == 2 ? 0x4E : X == 3 ? 0x1B : X == 7 ? 0x141 : X == 15 ? 0x140 : 0;
+  if constexpr (kDpp != 0) {  // quad permutations, mirrored half rows and rows of 16
+    return uint32_t(__builtin_amdgcn_update_dpp(0, int(x), kDpp, 0xF, 0xF, false));
+  } else if constexpr (X == 4) {
+    return from_lane_xor<3>(from_lane_xor<7>(x));
+  } else if constexpr (X == 8) {
+    return from_lane_xor<7>(from_lane_xor<15>(x));
+  } else if constexpr (X == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    return threadIdx.x & 16 ? r[0] : r[1];
+  } else if constexpr (X == 32) {
+    const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return threadIdx.x & 32 ? r[0] : r[1];
+  } else {
+    static_assert(X == 31 || X == 63, "a butterfly or mirror distance");
+    return from_lane_xor<(X + 1) / 2>(from_lane_xor<X / 2>(x));
+  }
+}
+
+// An entry as one number: greater comes first (the value, then the lower
+// index); 0 is no entry.  NaN and -inf are none.
+__device__ __forceinline__ uint64_t key_of(float x, uint32_t at) {
+  const uint32_t u = __float_as_uint(x + 0.f);  // (-0 and 0 are one value)
+  const uint32_t up = u ^ (u >> 31 ? 0xFFFFFFFFu : 0x80000000u);
+  return x > -INFINITY ? uint64_t(up) << 32 | (0xFFFFFFFFu - at) : 0u;
+}
+__device__ __forceinline__ float value_of(uint64_t key) {
+  const uint32_t up = uint32_t(key >> 32);
+  return key ? __uint_as_float(up ^ (up >> 31 ? 0x80000000u : 0xFFFFFFFFu)) : -INFINITY;
+}
+__device__ __forceinline__ uint32_t index_of(uint64_t key) { return 0xFFFFFFFFu - uint32_t(key); }
+
+__device__ __forceinline__ uint64_t key_in_lane(uint64_t key, int lane) {
+  return uint64_t(__builtin_amdgcn_readlane(uint32_t(key >> 32), lane)) << 32 |
+         uint32_t(__builtin_amdgcn_readlane(uint32_t(key), lane));
+}
+
+// lane and lane ^ X: the greater key to the lower lane
+template <int X>
+__device__ __forceinline__ void exchange(uint64_t& key) {
+  const uint64_t other = uint64_t(from_lane_xor<X>(uint32_t(key >> 32))) << 32 | from_lane_xor<X>(uint32_t(key));
+  constexpr int kTop = X >= 32 ? 32 : X >= 16 ? 16 : X >= 8 ? 8 : X >= 4 ? 4 : X >= 2 ? 2 : 1;
+  if ((other > key) != bool(threadIdx.x & kTop)) key = other;
+}
+template <int X>
+__device__ __forceinline__ void exchanges_from(uint64_t& key) {  // X, X / 2, .. 1
+  exchange<X>(key);
+  if constexpr (X > 1) exchanges_from<X / 2>(key);
+}
+// 64 keys into descending lanes: bitonic, every merge opened by a mirrored exchange
+__device__ __forceinline__ void sort_keys(uint64_t& key) {
+  exchange<1>(key);
+  exchange<3>(key), exchanges_from<1>(key);
+  exchange<7>(key), exchanges_from<2>(key);
+  exchange<15>(key), exchanges_from<4>(key);
+  exchange<31>(key), exchanges_from<8>(key);
+  exchange<63>(key), exchanges_from<16>(key);
+}
+
+// The best entries of a wavefront, descending over its lanes; the first `top` count.
 struct Best {
-  float v;
-  uint32_t i;
-  float worst_v;  // the last one's, in every lane
-  uint32_t worst_i;
+  uint64_t key, worst;  // worst: the top-th, in every lane
+  float worst_v;
   __device__ __forceinline__ void clear() {
-    v = worst_v = -INFINITY;
-    i = worst_i = 0u;
+    key = worst = 0;
+    worst_v = -INFINITY;
   }
-  // whether (x, at) comes before the last one (-inf and NaN never do)
-  __device__ __forceinline__ bool wants(float x, uint32_t at) const {
-    return x > worst_v || (x == worst_v && at < worst_i);
+  __device__ __forceinline__ void settle(int top) {
+    worst = key_in_lane(key, top - 1);
+    worst_v = value_of(worst);
   }
-  // one candidate per lane; in lanes without one `want` is false
-  __device__ __forceinline__ void insert(float x, uint32_t at, bool want, int top) {
-    uint64_t left = __builtin_amdgcn_ballot_w64(want);
+  // one sorted list more: `reversed` holds its 63 - lane-th
+  __device__ __forceinline__ void merge(uint64_t reversed, int top) {
+    key = reversed > key ? reversed : key;  // the best 64 of both, as a bitonic sequence
+    exchanges_from<32>(key);
+    settle(top);
+  }
+  // a candidate per lane (0: none), wavefront-uniform.  A few are inserted one
+  // by one (a ballot and a one-lane shift each, about a sixth of a sort and merge)
+  __device__ __forceinline__ void take(uint64_t candidate, int top) {
+    uint64_t left = __builtin_amdgcn_ballot_w64(candidate > worst);
+    if (__builtin_popcountll(left) > 6) {
+      sort_keys(candidate);
+      const uint64_t reversed = uint64_t(from_lane_xor<63>(uint32_t(candidate >> 32))) << 32 |
+                                from_lane_xor<63>(uint32_t(candidate));
+      merge(reversed, top);
+      return;
+    }
     const int lane = threadIdx.x % 64;
     while (left) {
-      const int src = __builtin_ctzll(left);
+      const uint64_t c = key_in_lane(candidate, __builtin_ctzll(left));
       left &= left - 1;
-      const float cx = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), src));
-      const uint32_t ci = __builtin_amdgcn_readlane(at, src);
-      if (!wants(cx, ci)) continue;  // (uniform)
-      const bool before = lane < top && (v > cx || (v == cx && i < ci));
-      const int pos = __builtin_popcountll(__builtin_amdgcn_ballot_w64(before));
-      const float pv = __shfl_up(v, 1);
-      const uint32_t pi = __shfl_up(i, 1);
-      if (lane == pos) {
-        v = cx;
-        i = ci;
-      } else if (lane > pos) {
-        v = pv;
-        i = pi;
-      }
-      worst_v = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), top - 1));
-      worst_i = __builtin_amdgcn_readlane(i, top - 1);
+      if (c <= worst) continue;  // (uniform)
+      const int pos = __builtin_popcountll(__builtin_amdgcn_ballot_w64(key > c));
+      // lane - 1's key (wave_shr:1)
+      const uint32_t hi = uint32_t(__builtin_amdgcn_update_dpp(0, int(key >> 32), 0x138, 0xF, 0xF, false));
+      const uint32_t lo = uint32_t(__builtin_amdgcn_update_dpp(0, int(key), 0x138, 0xF, 0xF, false));
+      key = lane > pos ? uint64_t(hi) << 32 | lo : lane == pos ? c : key;
+      settle(top);
     }
   }
 };
@@ -147,10 +213,25 @@ __device__ __forceinline__ bool run_of(const int64_t* offsets, int64_t p, int64_
   return false;
 }
 
+// A chosen move's logit, in lane g: read before the run so that its two
+// dependent loads do not follow the pass.
+struct Chosen {
+  int64_t move;
+  float x;
+};
+template <typename T>
+__device__ __forceinline__ Chosen chosen(const T* logits, int64_t stride, int64_t a, int64_t b, int64_t p,
+                                         const int64_t* moves, int64_t n_moves, int64_t g) {
+  Chosen c{-1, 0.f};
+  if (g < n_moves) c.move = moves[p * n_moves + g];
+  if (c.move >= 0 && c.move < b - a) c.x = widen(logits[(a + c.move) * stride]);
+  return c;
+}
+
 // What a position answers, from its joined state and list (in wavefront 0's lanes).
 template <typename T>
 __device__ __forceinline__ void write_run(const T* logits, int64_t stride, int64_t a, int64_t b, int64_t p, State s,
-                                          const Best& best, const int64_t* moves, int64_t n_moves, int top,
+                                          const Best& best, Chosen c, const int64_t* moves, int64_t n_moves, int top,
                                           const Out& out, int32_t* flag) {
   const int lane = threadIdx.x;
   const bool none = s.m == -INFINITY && s.l == 0.f, bad = s.l != s.l;
@@ -163,74 +244,100 @@ __device__ __forceinline__ void write_run(const T* logits, int64_t stride, int64
     out.norm[2 * p + 1] = log_l;
   }
   for (int64_t g = lane; g < n_moves; g += 64) {
-    const int64_t mv = moves[p * n_moves + g];
+    if (g >= 64) c = chosen(logits, stride, a, b, p, moves, n_moves, g);
     float lp = 0.f;
-    if (mv >= 0 && mv < b - a) lp = none ? -INFINITY : (widen(logits[(a + mv) * stride]) - m) - log_l;
-    else if (mv != -1) raise_flag(flag, MANTIS_FLAG_INDEX);
+    if (c.move >= 0 && c.move < b - a) lp = none ? -INFINITY : (c.x - m) - log_l;
+    else if (c.move != -1) raise_flag(flag, MANTIS_FLAG_INDEX);
     out.log_probs[p * n_moves + g] = lp;
   }
   if (lane < top) {
-    const bool there = best.v > -INFINITY && !bad;
-    out.top_moves[p * top + lane] = there ? int64_t(best.i) : -1;
-    out.top_log_probs[p * top + lane] = bad ? NAN : there ? (best.v - m) - log_l : -INFINITY;
+    const bool there = best.key && !bad;
+    out.top_moves[p * top + lane] = there ? int64_t(index_of(best.key)) : -1;
+    out.top_log_probs[p * top + lane] = bad ? NAN : there ? (value_of(best.key) - m) - log_l : -INFINITY;
   }
 }
 
 // The workgroup's join: every wavefront's state and list; the result in wavefront 0.
 __device__ __forceinline__ void block_join(State& s, Best& best, int top) {
   __shared__ State states[kWaves];
-  __shared__ float lv[kWaves][kMaxTop];
-  __shared__ uint32_t li[kWaves][kMaxTop];
+  __shared__ uint64_t keys[kWaves][64];
   const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
   s = wave_join(s);
   if (lane == 0) states[wave] = s;
-  if (wave > 0 && lane < top) {
-    lv[wave][lane] = best.v;
-    li[wave][lane] = best.i;
-  }
+  if (wave > 0) keys[wave][63 - lane] = best.key;
   __syncthreads();
   if (wave > 0) return;
 #pragma unroll
   for (int w = 1; w < kWaves; ++w) {
     join(s, states[w]);
-    if (top > 0) {
-      const float x = lane < top ? lv[w][lane] : -INFINITY;
-      const uint32_t at = lane < top ? li[w][lane] : 0u;
-      best.insert(x, at, best.wants(x, at), top);
+    if (top > 0) best.merge(keys[w][lane], top);
+  }
+}
+
+// kN entries of each lane, x[e] at index at + step * e (past the end: -inf)
+template <int kN>
+__device__ __forceinline__ void absorb(const float (&x)[kN], uint32_t at, uint32_t step, int top, State& s, Best& best) {
+  float m = x[0];
+#pragma unroll
+  for (int e = 1; e < kN; ++e) m = fmaxf(m, x[e]);
+  lift(s, m);
+#pragma unroll
+  for (int e = 0; e < kN; ++e) add(s, x[e]);
+  // (an equal value further on never wins: runs are met in ascending blocks)
+  if (top > 0 && __builtin_amdgcn_ballot_w64(m > best.worst_v || (m == best.worst_v && best.worst && at < index_of(best.worst)))) {
+#pragma unroll
+    for (int e = 0; e < kN; ++e) {
+      const uint64_t c = key_of(x[e], at + step * e);
+      if (__builtin_amdgcn_ballot_w64(c > best.worst)) best.take(c, top);
     }
   }
 }
 
-constexpr int kBatch = 4;  // entries of a lane in flight
-
-// The workgroup's entries [a + from, a + to) of a run into each lane's state and each wavefront's list.
+// The workgroup's entries [from, to) of the run at `a` into each lane's state and
+// each wavefront's list: 16-byte loads where the entries are dense, those before
+// and after the aligned blocks and strided ones one by one; four loads of a lane in flight.
 template <typename T>
 __device__ __forceinline__ void stream(const T* logits, int64_t stride, int64_t a, int64_t from, int64_t to, int top,
                                        State& s, Best& best) {
-  for (int64_t base = from; base < to; base += kThreads * kBatch) {
-    float x[kBatch];
+  constexpr int kV = 16 / sizeof(T), kLoads = 4;
+  const T* run = logits + a * stride;
+  if (stride == 1 && to - from >= kThreads * kV / 2) {
+    const int head = int((kV - reinterpret_cast<uintptr_t>(run + from) / sizeof(T) % kV) % kV);
+    const int64_t blocks = (to - from - head) / kV, body = from + head, tail = body + blocks * kV;
+    for (int64_t base = 0; base < blocks; base += kThreads * kLoads) {
+      uint4 raw[kLoads];
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-      const int64_t i = base + u * kThreads + threadIdx.x;
-      x[u] = i < to ? widen(logits[(a + i) * stride]) : -INFINITY;
-    }
-    float m = x[0];
+      for (int u = 0; u < kLoads; ++u) {
+        const int64_t b = base + u * kThreads + threadIdx.x;
+        raw[u] = *reinterpret_cast<const uint4*>(run + body + (b < blocks ? b : 0) * kV);
+      }
 #pragma unroll
-    for (int u = 1; u < kBatch; ++u) m = fmaxf(m, x[u]);
-    lift(s, m);
-    bool any = false;
+      for (int u = 0; u < kLoads; ++u) {
+        const int64_t b = base + u * kThreads + threadIdx.x;
+        T v[kV];
+        __builtin_memcpy(v, &raw[u], 16);
+        float x[kV];
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-      add(s, x[u]);
-      any = any || best.wants(x[u], uint32_t(base + u * kThreads + threadIdx.x));
-    }
-    if (top > 0 && __builtin_amdgcn_ballot_w64(any)) {
-#pragma unroll
-      for (int u = 0; u < kBatch; ++u) {
-        const uint32_t at = uint32_t(base + u * kThreads + threadIdx.x);
-        best.insert(x[u], at, best.wants(x[u], at), top);
+        for (int e = 0; e < kV; ++e) x[e] = b < blocks ? widen(v[e]) : -INFINITY;
+        absorb<kV>(x, uint32_t(body + b * kV), 1, top, s, best);
       }
     }
+    if (threadIdx.x < 64) {  // up to kV - 1 entries on each side
+      const int lane = threadIdx.x;
+      const int64_t i = lane < head ? from + lane : tail + lane - head;
+      const float x[1] = {i < to && lane < 2 * kV ? widen(run[i]) : -INFINITY};
+      absorb<1>(x, uint32_t(i), 0, top, s, best);
+    }
+    return;
+  }
+  for (int64_t base = from; base < to; base += kThreads * kLoads) {
+    float x[kLoads];
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) {
+      const int64_t i = base + u * kThreads + threadIdx.x;
+      x[u] = i < to ? widen(run[i * stride]) : -INFINITY;
+    }
+    absorb<kLoads>(x, uint32_t(base + threadIdx.x), kThreads, top, s, best);
   }
 }
 
@@ -241,19 +348,19 @@ policy_run_kernel(const T* __restrict__ logits, int64_t stride, const int64_t* _
   const int64_t p = blockIdx.x;
   int64_t a, b;
   run_of(offsets, p, n, a, b, flag);
+  const Chosen c = chosen(logits, stride, a, b, p, moves, n_moves, threadIdx.x < 64 ? threadIdx.x : n_moves);
   State s = empty_state();
   Best best;
   best.clear();
   stream(logits, stride, a, 0, b - a, top, s, best);
   block_join(s, best, top);
-  if (threadIdx.x < 64) write_run(logits, stride, a, b, p, s, best, moves, n_moves, top, out, flag);
+  if (threadIdx.x < 64) write_run(logits, stride, a, b, p, s, best, c, moves, n_moves, top, out, flag);
 }
 
-// Workspace of a sliced call: state, then values, then indices of each (position, slice).
+// Workspace of a sliced call: the list, then the state of each (position, slice).
 struct Parts {
-  float* state;  // (P, S, 3)
-  float* v;      // (P, S, top)
-  uint32_t* i;   // (P, S, top)
+  uint64_t* key;  // (P, S, top), each slice's descending
+  float* state;   // (P, S, 3)
 };
 
 template <typename T>
@@ -276,10 +383,7 @@ policy_slice_kernel(const T* __restrict__ logits, int64_t stride, const int64_t*
     parts.state[3 * at + 1] = s.l;
     parts.state[3 * at + 2] = s.t;
   }
-  if (int(threadIdx.x) < top) {
-    parts.v[at * top + threadIdx.x] = best.v;
-    parts.i[at * top + threadIdx.x] = best.i;
-  }
+  if (int(threadIdx.x) < top) parts.key[at * top + threadIdx.x] = best.key;
 }
 
 template <typename T>
@@ -290,6 +394,7 @@ policy_join_kernel(const T* __restrict__ logits, int64_t stride, const int64_t* 
   const int64_t p = blockIdx.x;
   int64_t a, b;
   run_of(offsets, p, n, a, b, flag);
+  const Chosen c = chosen(logits, stride, a, b, p, moves, n_moves, threadIdx.x < 64 ? threadIdx.x : n_moves);
   State s = empty_state();
   Best best;
   best.clear();
@@ -300,13 +405,10 @@ policy_join_kernel(const T* __restrict__ logits, int64_t stride, const int64_t* 
   const int64_t entries = int64_t(slices) * top;
   for (int64_t e = 0; e < entries; e += kThreads) {
     const int64_t j = p * entries + e + threadIdx.x;
-    const bool in = e + int(threadIdx.x) < entries;
-    const float x = in ? parts.v[j] : -INFINITY;
-    const uint32_t at = in ? parts.i[j] : 0u;
-    best.insert(x, at, best.wants(x, at), top);
+    best.take(e + int(threadIdx.x) < entries ? parts.key[j] : 0u, top);
   }
   block_join(s, best, top);
-  if (threadIdx.x < 64) write_run(logits, stride, a, b, p, s, best, moves, n_moves, top, out, flag);
+  if (threadIdx.x < 64) write_run(logits, stride, a, b, p, s, best, c, moves, n_moves, top, out, flag);
 }
 
 // The gradient of a slice of a run: every entry's share of the sums, then the
@@ -349,12 +451,33 @@ policy_backward_kernel(const T* __restrict__ logits, int64_t stride, const int64
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) total += sums[w];
   const float common = (g_lse ? g_lse[p] : 0.f) - total, ge = g_ent ? g_ent[p] : 0.f;
-  auto base = [&](int64_t i) {
-    const float lp = (widen(logits[(a + i) * stride]) - m) - log_l;
+  auto base_of = [&](float x) {
+    const float lp = (x - m) - log_l;
     const float pr = exp_neg(lp);
     return pr * (common - ge * (fmaxf(lp, -200.f) + h));  // (pr is 0 long before; keeps 0 * inf out)
   };
-  for (int64_t i = from + threadIdx.x; i < to; i += kThreads) narrow(dx[a + i], none ? 0.f : base(i));
+  auto base = [&](int64_t i) { return base_of(widen(logits[(a + i) * stride])); };
+  constexpr int kV = 16 / sizeof(T);
+  int64_t body = from, tail = from;  // the entries in blocks of 16 bytes, where both sides share their alignment
+  if (stride == 1 && (reinterpret_cast<uintptr_t>(logits) - reinterpret_cast<uintptr_t>(dx)) % 16 == 0) {
+    const int64_t head = int64_t((kV - reinterpret_cast<uintptr_t>(dx + a + from) / sizeof(T) % kV) % kV);
+    if (head < to - from) {
+      body = from + head;
+      tail = body + (to - body) / kV * kV;
+    }
+  }
+  for (int64_t i = body + kV * threadIdx.x; i < tail; i += kV * kThreads) {
+    const uint4 raw = *reinterpret_cast<const uint4*>(logits + a + i);
+    T v[kV];
+    __builtin_memcpy(v, &raw, 16);
+#pragma unroll
+    for (int e = 0; e < kV; ++e) narrow(v[e], none ? 0.f : base_of(widen(v[e])));
+    uint4 res;
+    __builtin_memcpy(&res, v, 16);
+    *reinterpret_cast<uint4*>(dx + a + i) = res;
+  }
+  for (int64_t i = from + threadIdx.x; i < body; i += kThreads) narrow(dx[a + i], none ? 0.f : base(i));
+  for (int64_t i = tail + threadIdx.x; i < to; i += kThreads) narrow(dx[a + i], none ? 0.f : base(i));
   // what no run holds has no gradient
   const int64_t stop = p == 0 ? (offsets[0] < 0 ? 0 : offsets[0] > n ? n : offsets[0]) : 0;
   for (int64_t i = sl * kThreads + threadIdx.x; i < stop; i += int64_t(slices) * kThreads) narrow(dx[i], 0.f);
@@ -395,9 +518,8 @@ int32_t forward(const void* logits, int64_t stride, const int64_t* offsets, int6
     return launched();
   }
   Parts parts;
-  parts.state = static_cast<float*>(workspace);
-  parts.v = parts.state + 3 * n_pos * slices;
-  parts.i = reinterpret_cast<uint32_t*>(parts.v + n_pos * slices * top);
+  parts.key = static_cast<uint64_t*>(workspace);
+  parts.state = reinterpret_cast<float*>(parts.key + n_pos * slices * top);
   policy_slice_kernel<T><<<unsigned(n_pos * slices), kThreads, 0, st>>>(x, stride, offsets, n, top, slices, parts, flag);
   policy_join_kernel<T><<<unsigned(n_pos), kThreads, 0, st>>>(x, stride, offsets, n, moves, n_moves, top, slices, parts,
                                                              out, flag);
@@ -433,7 +555,7 @@ extern "C" int32_t mantis_policy_log_probs(const void* logits, int32_t dtype, in
   if (!entropy || !lse || !norm || (n_moves > 0 && !log_probs) || (top > 0 && (!top_log_probs || !top_moves)))
     return MANTIS_E_ARG;
   const int64_t need = mantis_policy_log_probs_workspace(n_pos, n, top);
-  if (need > 0 && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 4)) return MANTIS_E_ARG;
+  if (need > 0 && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 8)) return MANTIS_E_ARG;
   const Out out{log_probs, entropy, lse, top_log_probs, top_moves, norm};
   auto go = dtype == MANTIS_F32 ? forward<float> : dtype == MANTIS_F16 ? forward<_Float16> : forward<Bf16>;
   return go(logits, stride, offsets, n_pos, n, moves, n_moves, top, out, workspace, err_flag, as_stream(stream));
