@@ -274,22 +274,28 @@ __device__ __forceinline__ void block_join(State& s, Best& best, int top) {
   }
 }
 
-// kN entries of each lane, x[e] at index at + step * e (past the end: -inf)
-template <int kN>
-__device__ __forceinline__ void absorb(const float (&x)[kN], uint32_t at, uint32_t step, int top, State& s, Best& best) {
+// kN entries of each lane, x[e] at index at + step(e) >= at (past the end: -inf)
+template <int kN, typename Step>
+__device__ __forceinline__ void absorb(const float (&x)[kN], uint32_t at, Step step, int top, State& s, Best& best) {
   float m = x[0];
 #pragma unroll
   for (int e = 1; e < kN; ++e) m = fmaxf(m, x[e]);
   lift(s, m);
 #pragma unroll
   for (int e = 0; e < kN; ++e) add(s, x[e]);
-  // (an equal value further on never wins: runs are met in ascending blocks)
   if (top > 0 && __builtin_amdgcn_ballot_w64(m > best.worst_v || (m == best.worst_v && best.worst && at < index_of(best.worst)))) {
-#pragma unroll
-    for (int e = 0; e < kN; ++e) {
-      const uint64_t c = key_of(x[e], at + step * e);
-      if (__builtin_amdgcn_ballot_w64(c > best.worst)) best.take(c, top);
+    // What can still be among the best: entries up to the last one's value, or, before there is
+    // one, up to the top-th of the lanes' maxima (top lanes hold at least one that great)
+    float cut = best.worst_v;
+    if (kN > 1 && !best.worst) {
+      uint64_t maxima = key_of(m, 0);
+      sort_keys(maxima);
+      cut = value_of(key_in_lane(maxima, top - 1));
     }
+#pragma unroll
+    for (int e = 0; e < kN; ++e)
+      if (__builtin_amdgcn_ballot_w64(x[e] >= cut && x[e] > -INFINITY))
+        best.take(x[e] >= cut ? key_of(x[e], at + step(e)) : 0u, top);
   }
 }
 
@@ -311,22 +317,23 @@ __device__ __forceinline__ void stream(const T* logits, int64_t stride, int64_t 
         const int64_t b = base + u * kThreads + threadIdx.x;
         raw[u] = *reinterpret_cast<const uint4*>(run + body + (b < blocks ? b : 0) * kV);
       }
+      float x[kLoads * kV];
 #pragma unroll
       for (int u = 0; u < kLoads; ++u) {
-        const int64_t b = base + u * kThreads + threadIdx.x;
         T v[kV];
         __builtin_memcpy(v, &raw[u], 16);
-        float x[kV];
 #pragma unroll
-        for (int e = 0; e < kV; ++e) x[e] = b < blocks ? widen(v[e]) : -INFINITY;
-        absorb<kV>(x, uint32_t(body + b * kV), 1, top, s, best);
+        for (int e = 0; e < kV; ++e)
+          x[u * kV + e] = base + u * kThreads + threadIdx.x < blocks ? widen(v[e]) : -INFINITY;
       }
+      absorb(x, uint32_t(body + (base + threadIdx.x) * kV), [](int i) { return uint32_t(i / kV * kThreads * kV + i % kV); },
+             top, s, best);
     }
     if (threadIdx.x < 64) {  // up to kV - 1 entries on each side
       const int lane = threadIdx.x;
       const int64_t i = lane < head ? from + lane : tail + lane - head;
       const float x[1] = {i < to && lane < 2 * kV ? widen(run[i]) : -INFINITY};
-      absorb<1>(x, uint32_t(i), 0, top, s, best);
+      absorb(x, uint32_t(i), [](int) { return 0u; }, top, s, best);
     }
     return;
   }
@@ -337,7 +344,7 @@ __device__ __forceinline__ void stream(const T* logits, int64_t stride, int64_t 
       const int64_t i = base + u * kThreads + threadIdx.x;
       x[u] = i < to ? widen(run[i * stride]) : -INFINITY;
     }
-    absorb<kLoads>(x, uint32_t(base + threadIdx.x), kThreads, top, s, best);
+    absorb(x, uint32_t(base + threadIdx.x), [](int i) { return uint32_t(i * kThreads); }, top, s, best);
   }
 }
 
