@@ -248,11 +248,9 @@ relative_bwd_q_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int32
   const float2 st = live ? stats[pa * T + i] : make_float2(0.f, INFINITY);
   const Side<true, 8> side(rel, coords_of(rel, pos, T, i, L), i < rel.n_latents);
   const int n_latents = int(rel.n_latents);
-  for (int d = threadIdx.x; d < n_disp + 2; d += 256) {
-    const int b = bucket_of(rel, d);
-    const float x = b < rel.n_buckets ? raw_bias(rel.bias[a * rel.n_buckets + b], root_hd) : 0.f;
+  stage_table(rel, a, root_hd, [&](int d, float x, int b) {
     table[d] = make_uint2(__float_as_uint(x), uint32_t(b) * kColumns * 4);
-  }
+  });
   for (int c = threadIdx.x; c < kBwdWaves * n_rows * kColumns / 4; c += 256)
     reinterpret_cast<float4*>(columns)[c] = make_float4(0.f, 0.f, 0.f, 0.f);
   // this lane's column (the lanes of a dead query spoil only their own, which no sum takes)

@@ -57,23 +57,42 @@ __device__ __forceinline__ float raw_bias(float b, float root_hd) {
   return fabsf(b) <= kLargest ? fminf(fmaxf(x, -kLargest), kLargest) : b;
 }
 
-// Entry displacement d of a head's table: entries nq nr and nq nr + 1 are the latents'.
-__device__ __forceinline__ int bucket_of(const Relative& rel, int i) {
+// The head's table, staged by the workgroup: store(i, bias, bucket) for entry
+// i < nq nr + 2 (entries nq nr and nq nr + 1 are the latents'; a bucket that is
+// none has bias 0 and the number n_buckets).  Four buckets of a thread are
+// requested before their biases, those before the first store: entry by entry
+// the two dependent loads would chain.
+template <typename Store>
+__device__ __forceinline__ void stage_table(const Relative& rel, int64_t head, float root_hd, Store store) {
+  constexpr int kMany = 4;
   const int n = rel.nq * rel.nr;
-  int b = i < n ? rel.buckets[i] : rel.n_buckets - (i == n ? 2 : 1);
-  if (b < 0 || b >= rel.n_buckets) {
-    if (i < n) raise_flag(rel.flag, MANTIS_FLAG_INDEX);
-    b = rel.n_buckets;  // (no bias, no gradient)
+  const float* bias = rel.bias + head * rel.n_buckets;
+  for (int base = 0; base < n + 2; base += 256 * kMany) {
+    int b[kMany];
+    float x[kMany];
+#pragma unroll
+    for (int u = 0; u < kMany; ++u) {
+      const int i = base + 256 * u + int(threadIdx.x);
+      b[u] = rel.buckets[i < n ? i : 0];
+      if (i >= n) b[u] = rel.n_buckets - (i == n ? 2 : 1);
+    }
+#pragma unroll
+    for (int u = 0; u < kMany; ++u) {
+      const bool good = b[u] >= 0 && b[u] < rel.n_buckets;
+      if (!good && base + 256 * u + int(threadIdx.x) < n) raise_flag(rel.flag, MANTIS_FLAG_INDEX);
+      b[u] = good ? b[u] : rel.n_buckets;
+      x[u] = bias[good ? b[u] : 0];
+      x[u] = good ? raw_bias(x[u], root_hd) : 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < kMany; ++u) {
+      const int i = base + 256 * u + int(threadIdx.x);
+      if (i < n + 2) store(i, x[u], b[u]);
+    }
   }
-  return b;
 }
-
-// the head's table, staged by the workgroup: table[i], i < nq nr + 2
 __device__ __forceinline__ void stage_bias(const Relative& rel, int64_t head, float root_hd, float* table) {
-  for (int i = threadIdx.x; i < rel.nq * rel.nr + 2; i += blockDim.x) {
-    const int b = bucket_of(rel, i);
-    table[i] = b < rel.n_buckets ? raw_bias(rel.bias[head * rel.n_buckets + b], root_hd) : 0.f;
-  }
+  stage_table(rel, head, root_hd, [&](int i, float x, int) { table[i] = x; });
 }
 
 // This lane's side of its pairs: the byte offset of the table entry (kEntry
