@@ -161,5 +161,20 @@ __device__ __forceinline__ void store_row(uint16_t* row, int g, const f32x4_t (&
   }
 }
 
+// the A fragment (16 dims x 32 rows) of the transposed rows 32 h .. of a tile
+// at pitch HD + 8, dims 16 dt .., its K slots the rows 4 g + t and 16 + 4 g + t: the transposing
+// read gives lane i of 16 the i-th of the 16 dims of four rows whose 8-byte
+// pieces the 16 lanes name
+typedef short lds_s16x4_t __attribute__((ext_vector_type(4)));
+template <int HD>
+__device__ __forceinline__ uint4 transposed_frag(const uint16_t* s, int h, int dt, int l16, int g) {
+  using Shared = __attribute__((address_space(3))) lds_s16x4_t;
+  const uint16_t* at = s + (32 * h + 4 * g + l16 / 4) * (HD + 8) + 16 * dt + 4 * (l16 % 4);
+  const lds_s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Shared*)at);
+  const lds_s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Shared*)(at + 16 * (HD + 8)));
+  const uint2 a = __builtin_bit_cast(uint2, lo), b = __builtin_bit_cast(uint2, hi);
+  return make_uint4(a.x, a.y, b.x, b.y);
+}
+
 }  // namespace
 }  // namespace mantis

@@ -22,7 +22,7 @@
 // is that key's value, and lse is the log of the unrounded fp32 sum.
 #include <type_traits>
 
-#include "mfma.hpp"
+#include "attention_rows.hpp"
 #include "relative_bias.hpp"
 
 namespace mantis {
@@ -30,7 +30,6 @@ namespace {
 
 constexpr int kWaves = 4;
 constexpr int kKChunk = 64;
-constexpr int kVtPitch = kKChunk + 8;  // 16-bit elements per staged V^T row
 constexpr float kLazyLog2 = 8.f;       // probabilities up to 2^8 before the reference point moves
 
 struct Operand {  // (P, A, T, hd): base and element strides
@@ -44,14 +43,14 @@ relative_attention_kernel(Operand q, Operand k, Operand v, Relative rel, const i
                           int heads, int64_t T, uint16_t* __restrict__ out, int64_t osp, int64_t osa, int64_t ost,
                           float* __restrict__ lse, float2* __restrict__ stats, float c_log2, float root_hd, int64_t n_pa) {
   constexpr int kQTile = kWaves * 16 * kSub;
-  constexpr int kKPitch = HD + 8;              // 16-bit elements per staged K row
+  constexpr int kKPitch = HD + 8;              // 16-bit elements per staged K or V row
   constexpr int kKs = HD < 32 ? 1 : HD / 32;   // K steps of the score product
   constexpr int kDt = HD / 16;                 // 16-dim output tiles
   constexpr int kPieces = kKChunk * HD / 8;    // 16-byte pieces of a chunk's K (or V) rows
   constexpr int kPer = kPieces < 256 ? 1 : kPieces / 256;
   extern __shared__ float table[];  // the head's bias per displacement
   __shared__ __attribute__((aligned(16))) uint16_t sk[2][kKChunk * kKPitch];
-  __shared__ __attribute__((aligned(16))) uint16_t svt[2][HD * kVtPitch];
+  __shared__ __attribute__((aligned(16))) uint16_t sv[2][kKChunk * kKPitch];
   __shared__ __attribute__((aligned(16))) uint32_t sc[2][kKChunk];
   const int64_t n_qt = (T + kQTile - 1) / kQTile;
   const Item item = item_of(n_pa, heads, n_qt);
@@ -125,13 +124,7 @@ relative_attention_kernel(Operand q, Operand k, Operand v, Relative rel, const i
       const int i = int(threadIdx.x) + 256 * r;
       const int st_key = i / (HD / 8), st_d = 8 * (i % (HD / 8));
       *reinterpret_cast<uint4*>(&sk[buf][st_key * kKPitch + st_d]) = kreg[r];
-      const uint32_t w[4] = {vreg[r].x, vreg[r].y, vreg[r].z, vreg[r].w};
-      uint16_t* col = &svt[buf][st_d * kVtPitch + st_key];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        col[(2 * e) * kVtPitch] = uint16_t(w[e] & 0xffffu);
-        col[(2 * e + 1) * kVtPitch] = uint16_t(w[e] >> 16);
-      }
+      *reinterpret_cast<uint4*>(&sv[buf][st_key * kKPitch + st_d]) = vreg[r];
     }
   };
   fetch(0);
@@ -165,27 +158,28 @@ relative_attention_kernel(Operand q, Operand k, Operand v, Relative rel, const i
     constexpr int kNJ = decltype(nj)::value;
     if (more) fetch(kb + kKChunk);
     if constexpr (kNJ > 0) {
+      // keys of the last chunk: tiles of 16 past the last one are left out (uniform)
+      constexpr bool kMasked = decltype(masked)::value;
+      const int n = kMasked ? int(L - kb) : kKChunk;
       f32x4_t s[kNJ][4];
 #pragma unroll
       for (int j = 0; j < kNJ; ++j) {
         int at[4][4];
         pair_offsets(side[j], n_latents, sc[buf], int(kb), g, at);
 #pragma unroll
-        for (int tt = 0; tt < 4; ++tt)
+        for (int tt = 0; tt < 4; ++tt) {
+          s[j][tt] = f32x4_t{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          if (kMasked && 16 * tt >= n) continue;
 #pragma unroll
-          for (int t = 0; t < 4; ++t) s[j][tt][t] = entry(table, at[tt][t]);
-      }
-      if constexpr (decltype(masked)::value) {
-        const int lim = int(L - kb) - 4 * g;
-#pragma unroll
-        for (int tt = 0; tt < 4; ++tt)
-#pragma unroll
-          for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int j = 0; j < kNJ; ++j) s[j][tt][t] = 16 * tt + t < lim ? s[j][tt][t] : -INFINITY;
+          for (int t = 0; t < 4; ++t) {
+            s[j][tt][t] = entry(table, at[tt][t]);
+            if (kMasked) s[j][tt][t] = 16 * tt + t < n - 4 * g ? s[j][tt][t] : -INFINITY;
+          }
+        }
       }
 #pragma unroll
       for (int tt = 0; tt < 4; ++tt) {
+        if (kMasked && 16 * tt >= n) break;
 #pragma unroll
         for (int ks = 0; ks < kKs; ++ks) {
           uint4 ku = *reinterpret_cast<const uint4*>(&sk[buf][(16 * tt + l16) * kKPitch + kdim(ks)]);
@@ -221,6 +215,8 @@ relative_attention_kernel(Operand q, Operand k, Operand v, Relative rel, const i
         uint32_t pw[4][2];
 #pragma unroll
         for (int tt = 0; tt < 4; ++tt) {
+          pw[tt][0] = pw[tt][1] = 0u;
+          if (kMasked && 16 * tt >= n) continue;
           float pr[4];
 #pragma unroll
           for (int t = 0; t < 4; ++t) {
@@ -236,12 +232,10 @@ relative_attention_kernel(Operand q, Operand k, Operand v, Relative rel, const i
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
+        if (kMasked && 32 * h >= n) break;
 #pragma unroll
         for (int dt = 0; dt < kDt; ++dt) {
-          const uint16_t* row = &svt[buf][(16 * dt + l16) * kVtPitch + 32 * h];
-          const uint2 lo = *reinterpret_cast<const uint2*>(row + 4 * g);
-          const uint2 hi = *reinterpret_cast<const uint2*>(row + 16 + 4 * g);
-          const typename FR::vec vf = FR::cast(make_uint4(lo.x, lo.y, hi.x, hi.y));
+          const typename FR::vec vf = FR::cast(transposed_frag<HD>(sv[buf], h, dt, l16, g));
 #pragma unroll
           for (int j = 0; j < kNJ; ++j) o[j][dt] = mfma16x16x32(vf, pf[j][h], o[j][dt]);
         }

@@ -31,7 +31,7 @@
 // at a time; where that table does not fit, the four lane groups in turn to 16
 // columns.  (LDS float atomics instead: 2.5 cycles per lane, half of the whole
 // pass.)  The columns join in a fixed order into the workgroup's partial sums, those
-// of a head in a second launch.  Every sum is fp32 in a fixed order: two calls
+// of a head in the second launch.  Every sum is fp32 in a fixed order: two calls
 // agree bitwise.
 #include <type_traits>
 
@@ -90,21 +90,6 @@ __device__ __forceinline__ void row_frags(i32x4_t rows, int64_t row, int g, uint
     u[ks] = row_load16(rows, int32_t(row), 2 * G::kdim(ks, g));
     if (HD < 32 && g >= 2) u[ks] = make_uint4(0u, 0u, 0u, 0u);
   }
-}
-
-// the A fragment (16 dims x 32 rows) of the transposed rows 32 h .. of a tile,
-// dims 16 dt .., its K slots the rows 4 g + t and 16 + 4 g + t: the transposing
-// read gives lane i of 16 the i-th of the 16 dims of four rows whose 8-byte
-// pieces the 16 lanes name
-typedef short lds_s16x4_t __attribute__((ext_vector_type(4)));
-template <int HD>
-__device__ __forceinline__ uint4 transposed_frag(const uint16_t* s, int h, int dt, int l16, int g) {
-  using Shared = __attribute__((address_space(3))) lds_s16x4_t;
-  const uint16_t* at = s + (32 * h + 4 * g + l16 / 4) * RowTile<HD>::kPitch + 16 * dt + 4 * (l16 % 4);
-  const lds_s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Shared*)at);
-  const lds_s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Shared*)(at + 16 * RowTile<HD>::kPitch));
-  const uint2 a = __builtin_bit_cast(uint2, lo), b = __builtin_bit_cast(uint2, hi);
-  return make_uint4(a.x, a.y, b.x, b.y);
 }
 
 // two fp32 values as their packed 16-bit parts: hi rounded, lo what is left
@@ -398,11 +383,33 @@ relative_bwd_q_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int32
   }
 }
 
+// dbias of one (head, bucket): the head's partial sums of the query pass, each
+// thread a fixed stride of them, joined in a fixed order.  Workgroups of the
+// key pass's launch do it, where a launch of their own would take 4 us.
+__device__ __forceinline__ void sum_bias(const float* __restrict__ partial, int64_t n_parts, int n_buckets,
+                                         uint32_t which, float* __restrict__ dbias) {
+  __shared__ float sums[256];
+  const int64_t a = which / n_buckets, b = which % n_buckets;
+  float sum = 0.f;
+  for (int64_t i = threadIdx.x; i < n_parts; i += 256) sum += partial[(a * n_parts + i) * n_buckets + b];
+  sums[threadIdx.x] = sum;
+  for (int o = 128; o > 0; o >>= 1) {
+    __syncthreads();
+    if (int(threadIdx.x) < o) sums[threadIdx.x] += sums[threadIdx.x + o];
+  }
+  if (threadIdx.x == 0) dbias[which] = sums[0];
+}
+
 template <bool kHalf, int HD>
 __global__ void __launch_bounds__(256)
 relative_bwd_kv_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int32_t* __restrict__ seq_lens, int heads,
                        int64_t T, int64_t n_pa, const float2* __restrict__ stats, float scale, float root_hd,
-                       const float* __restrict__ delta, RowsOut dk, RowsOut dv) {
+                       const float* __restrict__ delta, RowsOut dk, RowsOut dv, const float* __restrict__ partial,
+                       float* __restrict__ dbias, uint32_t n_item_groups) {
+  if (blockIdx.x >= n_item_groups) {  // the workgroups after the items
+    sum_bias(partial, n_pa / heads * ((T + kTile - 1) / kTile), rel.n_buckets, blockIdx.x - n_item_groups, dbias);
+    return;
+  }
   using G = Geom<kHalf, HD>;
   using Tile = RowTile<HD>;
   __shared__ __attribute__((aligned(16))) uint16_t sq[2][kTile * Tile::kPitch], sg[2][kTile * Tile::kPitch];
@@ -511,22 +518,6 @@ relative_bwd_kv_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int3
   }
 }
 
-// dbias[a, b]: the head's partial sums, each thread a fixed stride of them,
-// joined in a fixed order.  One workgroup per (head, bucket).
-__global__ void __launch_bounds__(256)
-relative_bias_sum_kernel(const float* __restrict__ partial, int64_t n_parts, int n_buckets, float* __restrict__ dbias) {
-  __shared__ float sums[256];
-  const int64_t a = blockIdx.x / n_buckets, b = blockIdx.x % n_buckets;
-  float sum = 0.f;
-  for (int64_t i = threadIdx.x; i < n_parts; i += 256) sum += partial[(a * n_parts + i) * n_buckets + b];
-  sums[threadIdx.x] = sum;
-  for (int o = 128; o > 0; o >>= 1) {
-    __syncthreads();
-    if (int(threadIdx.x) < o) sums[threadIdx.x] += sums[threadIdx.x + o];
-  }
-  if (threadIdx.x == 0) dbias[blockIdx.x] = sums[0];
-}
-
 template <bool kHalf, int HD>
 constexpr size_t static_lds() {
   return size_t(4 * kTile * RowTile<HD>::kPitch) * 2 + 2 * kTile * 4;  // (of the query pass)
@@ -552,7 +543,7 @@ int32_t launch(const Rows& q, const Rows& k, const Rows& v, const Rows& go, cons
                float* partial, const RowsOut& dq, const RowsOut& dk, const RowsOut& dv, float* dbias, hipStream_t st) {
   const int64_t n_tiles = (t + kTile - 1) / kTile, n_pa = n_pos * heads;
   const int64_t grid = item_grid(n_pos, heads, n_tiles);
-  if (grid > 2147483647LL) return MANTIS_E_ARG;
+  if (grid + heads * rel.n_buckets > 2147483647LL) return MANTIS_E_ARG;
   const float root = sqrtf(float(HD)), scale = 1.f / root;
   const int n_disp = rel.nq * rel.nr;
   // Columns per wavefront: 64 unless that table keeps workgroups off the CU that the
@@ -576,10 +567,8 @@ int32_t launch(const Rows& q, const Rows& k, const Rows& v, const Rows& go, cons
                                       : MANTIS_QUERY_PASS(8);
 #undef MANTIS_QUERY_PASS
   if (!queued) return MANTIS_E_LAUNCH;
-  relative_bwd_kv_kernel<kHalf, HD><<<unsigned(grid), 256, table_bytes(n_disp, 4), st>>>(
-      q, k, v, go, rel, seq_lens, heads, t, n_pa, stats, scale, root, delta, dk, dv);
-  relative_bias_sum_kernel<<<unsigned(heads * rel.n_buckets), 256, 0, st>>>(partial, n_pos * n_tiles, rel.n_buckets,
-                                                                           dbias);
+  relative_bwd_kv_kernel<kHalf, HD><<<unsigned(grid + heads * rel.n_buckets), 256, table_bytes(n_disp, 4), st>>>(
+      q, k, v, go, rel, seq_lens, heads, t, n_pa, stats, scale, root, delta, dk, dv, partial, dbias, uint32_t(grid));
   return launched();
 }
 
