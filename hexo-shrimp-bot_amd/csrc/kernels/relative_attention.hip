@@ -258,7 +258,7 @@ relative_attention_kernel(Operand q, Operand k, Operand v, Relative rel, const i
   stage(0);
   __syncthreads();
   const int64_t live_q = L - (q0 + wave * 16 * kSub);  // (wavefront-uniform)
-  if (live_q > 16 && kSub > 1) run(std::integral_constant<int, kSub>{});
+  if (kSub > 1 && live_q > 16) run(std::integral_constant<int, kSub>{});
   else if (live_q > 0) run(std::integral_constant<int, 1>{});
   else run(std::integral_constant<int, 0>{});
 #pragma unroll
@@ -334,11 +334,16 @@ extern "C" int32_t mantis_relative_attention(const void* q, const int64_t* qs, c
   uint16_t* o = static_cast<uint16_t*>(out);
   float2* sp = reinterpret_cast<float2*>(stats);
   hipStream_t st = as_stream(stream);
-#define MANTIS_FWD(HD_)                                                                                     \
-  return dtype == MANTIS_F16 ? launch<true, HD_, 2>(Q, K, V, rel, seq_lens, n_pos, heads, t, o, os, lse, sp, st) \
-                             : launch<false, HD_, 2>(Q, K, V, rel, seq_lens, n_pos, heads, t, o, os, lse, sp, st)
-  if (hd == 16) MANTIS_FWD(16);
-  if (hd == 32) MANTIS_FWD(32);
-  MANTIS_FWD(64);
+#define MANTIS_FWD(HD_, SUB)                                                                                      \
+  return dtype == MANTIS_F16 ? launch<true, HD_, SUB>(Q, K, V, rel, seq_lens, n_pos, heads, t, o, os, lse, sp, st) \
+                             : launch<false, HD_, SUB>(Q, K, V, rel, seq_lens, n_pos, heads, t, o, os, lse, sp, st)
+  // Two sub-tiles of 16 queries per wavefront read a key fragment once for both, and 128 queries hold
+  // a usual position whole; one leaves the registers for twice the wavefronts: 192 positions of
+  // 44-124 rows, 32 dims, 14.5 against 16.7 us, longer ones MEASURED4; two lines of
+  // 2,049-4,096 rows, 64 dims, 137 against 131, 16 positions of 511-1,021, 16 dims, 72 against 58.
+  if (hd == 16) MANTIS_FWD(16, 1);
+  if (hd == 32 && t <= 128) MANTIS_FWD(32, 2);
+  if (hd == 32) MANTIS_FWD(32, 1);
+  MANTIS_FWD(64, 1);
 #undef MANTIS_FWD
 }

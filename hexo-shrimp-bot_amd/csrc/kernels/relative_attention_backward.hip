@@ -8,15 +8,18 @@
 //
 // Two passes, each a workgroup per (position, head, 64 rows), 16 rows per
 // wavefront, the other side's rows in 64-row chunks through LDS, two buffers:
-//   query-major  S^T = K Q^T and dP^T = V dO^T, then dQ^T += K^T dS^T and the buckets' sums
+//   query-major  S^T = K Q^T and dP^T = V dO^T, then dQ^T += K^T dS^T
 //   key-major    S = Q K^T and dP = dO V^T, then dV^T += dO^T P, dK^T += Q^T dS
 // Both keep a lane on one row of its own side, so a score fragment is the next
 // product's B operand as it stands, and read the transposed A operand from the
 // same row-major LDS rows (the transposing 64-bit LDS read of gfx950).
-// The query pass goes over the keys twice: delta first, from the fp32 products
-// (the 16-bit output's rounding would stay in every ds of its row, and in the
-// bias gradient's long sums), then ds.  Up to two chunks of keys stay in LDS in
-// between, and their p and dp in registers.
+// delta needs every key of a row before the first ds (and the 16-bit output
+// times its gradient is no substitute: its rounding would stay in every ds of
+// the row and in the bias gradient's long sums).  Up to two chunks of keys (T <=
+// 128) keep p and dp in registers until delta is known.  Longer rows are met
+// once: dq = sum (p dp) k - delta sum p k, with two sums beside delta, and the
+// buckets' sums move to the key pass, which knows delta.  (A second sweep over
+// the keys instead: the query pass 511 us against MEASURED3 at two lines of 2,049-4,096.)
 //
 // Precision: scores and dp are exact products of 16-bit rows summed in fp32.
 // The probabilities and ds enter their products as two 16-bit parts, hi + lo:
@@ -128,6 +131,36 @@ __device__ __forceinline__ void accumulate_parts(const uint16_t* s, int n, int l
   }
 }
 
+// the same for two sums of one operand, whose fragments are read once
+template <bool kHalf, int HD>
+__device__ __forceinline__ void accumulate_two(const uint16_t* s, int n, int l16, int g, const f32x4_t (&x)[4],
+                                               f32x4_t (&acc_x)[Geom<kHalf, HD>::kDt], const f32x4_t (&y)[4],
+                                               f32x4_t (&acc_y)[Geom<kHalf, HD>::kDt]) {
+  using FR = Frag<kHalf>;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    if (32 * h >= n) break;  // uniform
+    uint32_t xh[4], xl[4], yh[4], yl[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      parts<kHalf>(x[2 * h + i / 2][2 * (i % 2)], x[2 * h + i / 2][2 * (i % 2) + 1], xh[i], xl[i]);
+      parts<kHalf>(y[2 * h + i / 2][2 * (i % 2)], y[2 * h + i / 2][2 * (i % 2) + 1], yh[i], yl[i]);
+    }
+#pragma unroll
+    for (int dt = 0; dt < Geom<kHalf, HD>::kDt; ++dt) {
+      const typename FR::vec a = FR::cast(transposed_frag<HD>(s, h, dt, l16, g));
+      acc_x[dt] = mfma16x16x32(a, FR::cast(make_uint4(xh[0], xh[1], xh[2], xh[3])), acc_x[dt]);
+      acc_x[dt] = mfma16x16x32(a, FR::cast(make_uint4(xl[0], xl[1], xl[2], xl[3])), acc_x[dt]);
+      acc_y[dt] = mfma16x16x32(a, FR::cast(make_uint4(yh[0], yh[1], yh[2], yh[3])), acc_y[dt]);
+      acc_y[dt] = mfma16x16x32(a, FR::cast(make_uint4(yl[0], yl[1], yl[2], yl[3])), acc_y[dt]);
+    }
+  }
+}
+
+// the scale of a probability's fp16 parts (it is at most 1)
+template <bool kHalf>
+constexpr float kPScale = kHalf ? 0x1p14f : 1.f;
+
 // The power of two that a column's fp16 parts are scaled by: the largest value
 // met so far lands in [2^13, 2^15].  bf16 parts need none.
 template <bool kHalf>
@@ -177,6 +210,88 @@ __device__ __forceinline__ void add4(char* base, const uint32_t (&at)[4], const 
   *reinterpret_cast<float*>(base + at[3]) = old[3] + x3;
 }
 
+// The workgroup's bucket sums: kColumns columns per wavefront of n_buckets + 1
+// rows (the last for pairs of no bucket), behind the table of (bias, byte
+// offset of the bucket's row) by displacement.
+template <int kColumns>
+struct BucketSums {
+  const char* table;
+  float* columns;
+  char* own;  // this lane's column (a dead row's lanes spoil only their own, which no sum takes)
+  int n_rows;
+  __device__ __forceinline__ BucketSums(const Relative& rel, char* dynamic) {
+    table = dynamic;
+    columns = reinterpret_cast<float*>(dynamic + table_bytes(rel.nq * rel.nr, 8));
+    n_rows = rel.n_buckets + 1;
+    own = reinterpret_cast<char*>(columns + threadIdx.x / 64 * n_rows * kColumns + threadIdx.x % kColumns);
+  }
+  __device__ __forceinline__ void stage(const Relative& rel, int64_t head, float root_hd, char* dynamic) {
+    uint2* entries = reinterpret_cast<uint2*>(dynamic);
+    stage_table(rel, head, root_hd, [&](int d, float x, int b) {
+      entries[d] = make_uint2(__float_as_uint(x), uint32_t(b) * kColumns * 4);
+    });
+    for (int c = threadIdx.x; c < kBwdWaves * n_rows * kColumns / 4; c += 256)
+      reinterpret_cast<float4*>(columns)[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  // four pairs of this lane, by their table offsets
+  __device__ __forceinline__ void add(const int (&at)[4], const f32x4_t& ds, bool live) {
+    uint32_t to[4];
+    float x[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      to[t] = *reinterpret_cast<const uint32_t*>(table + at[t] + 4);
+      x[t] = kColumns < 16 && !live ? 0.f : ds[t];  // (two rows share a column of eight)
+    }
+    if constexpr (kColumns == 64) {
+      add4(own, to, x);
+    } else {
+#pragma unroll
+      for (int turn = 0; turn < 64 / kColumns; ++turn) {
+        if (int(threadIdx.x) % 64 / kColumns == turn) add4(own, to, x);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (the next group reads what this one wrote)
+      }
+    }
+  }
+  // every bucket's sum over the columns of the workgroup's first n_live rows:
+  // eight threads to a bucket, starting apart so that a wavefront's reads meet other banks
+  __device__ __forceinline__ void flush(int n_live, float* sums) const {
+    for (int b0 = 0; b0 < n_rows - 1; b0 += 32) {
+      const int b = b0 + int(threadIdx.x) / 8, eighth = threadIdx.x % 8;
+      float sum = 0.f;
+      if (b < n_rows - 1)
+        for (int w = 0; w < kBwdWaves; ++w)
+#pragma unroll
+          for (int c = 0; c < kColumns / 8; ++c) {
+            const int col = (8 * c + eighth + 8 * (int(threadIdx.x) / 8)) % kColumns;
+            const float x = columns[(w * n_rows + b) * kColumns + col];
+            sum += 16 * w + col % 16 < n_live ? x : 0.f;
+          }
+      sum += __shfl_xor(sum, 1);
+      sum += __shfl_xor(sum, 2);
+      sum += __shfl_xor(sum, 4);
+      if (b < n_rows - 1 && eighth == 0) sums[b] = sum;
+    }
+  }
+};
+
+// a kernel without bucket sums stages the biases alone
+template <>
+struct BucketSums<0> {
+  __device__ __forceinline__ BucketSums(const Relative&, char*) {}
+  __device__ __forceinline__ void stage(const Relative& rel, int64_t head, float root_hd, char* dynamic) {
+    stage_bias(rel, head, root_hd, reinterpret_cast<float*>(dynamic));
+  }
+  __device__ __forceinline__ void add(const int (&)[4], const f32x4_t&, bool) {}
+  __device__ __forceinline__ void flush(int, float*) const {}
+};
+
+// The partial bucket sums of a workgroup: (head, position, tile, bucket).
+__device__ __forceinline__ float* partial_of(float* partial, const Relative& rel, int64_t n_pa, int heads,
+                                             int64_t n_tiles, int64_t pos, int64_t a, int64_t tile) {
+  return partial + ((a * (n_pa / heads) + pos) * n_tiles + tile) * rel.n_buckets;
+}
+
+// kColumns > 0: at most two chunks of keys (T <= 128), with the bucket sums; 0: any number, without.
 template <bool kHalf, int HD, int kColumns>
 __global__ void __launch_bounds__(256)
 relative_bwd_q_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int32_t* __restrict__ seq_lens, int heads,
@@ -190,18 +305,14 @@ relative_bwd_q_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int32
   const int64_t n_tiles = (T + kTile - 1) / kTile;
   const Item item = item_of(n_pa, heads, n_tiles);
   if (item.pa >= n_pa) return;
-  const int n_disp = rel.nq * rel.nr;
-  uint2* table = reinterpret_cast<uint2*>(dynamic);
-  float* columns = reinterpret_cast<float*>(dynamic + table_bytes(n_disp, 8));
   const int64_t pa = item.pa, tile = item.tile, pos = pa / heads, a = pa % heads;
   int64_t L = seq_lens[pos];
   L = L < 0 ? 0 : (L > T ? T : L);
   const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, l16 = lane % 16, g = lane / 16;
   const int64_t first = tile * kTile + 16 * wave, i = first + l16;
   const bool live = i < L;
-  const int n_rows = rel.n_buckets + 1;
-  // partial sums: (head, position, tile, bucket)
-  float* part_sums = partial + ((a * (n_pa / heads) + pos) * n_tiles + tile) * rel.n_buckets;
+  BucketSums<kColumns> sums(rel, dynamic);
+  float* part_sums = kColumns ? partial_of(partial, rel, n_pa, heads, n_tiles, pos, a, tile) : nullptr;
   f32x4_t acc[G::kDt];
 #pragma unroll
   for (int dt = 0; dt < G::kDt; ++dt) acc[dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -210,7 +321,8 @@ relative_bwd_q_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int32
       store_row<kHalf, HD, true>(dq.row(pos, a, i), g, acc, 0.f, false);
       if (g == 0) delta[pa * T + i] = 0.f;
     }
-    for (int b = threadIdx.x; b < rel.n_buckets; b += 256) part_sums[b] = 0.f;
+    if (kColumns)
+      for (int b = threadIdx.x; b < rel.n_buckets; b += 256) part_sums[b] = 0.f;
     return;
   }
   const i32x4_t krs = rows_of(k, pos, a, L), vrs = rows_of(v, pos, a, L);
@@ -231,15 +343,9 @@ relative_bwd_q_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int32
   row_frags<kHalf, HD>(rows_of(q, pos, a, L), i, g, qf);
   row_frags<kHalf, HD>(rows_of(go, pos, a, L), i, g, gf);
   const float2 st = live ? stats[pa * T + i] : make_float2(0.f, INFINITY);
-  const Side<true, 8> side(rel, coords_of(rel, pos, T, i, L), i < rel.n_latents);
+  const Side<true, kColumns ? 8 : 4> side(rel, coords_of(rel, pos, T, i, L), i < rel.n_latents);
   const int n_latents = int(rel.n_latents);
-  stage_table(rel, a, root_hd, [&](int d, float x, int b) {
-    table[d] = make_uint2(__float_as_uint(x), uint32_t(b) * kColumns * 4);
-  });
-  for (int c = threadIdx.x; c < kBwdWaves * n_rows * kColumns / 4; c += 256)
-    reinterpret_cast<float4*>(columns)[c] = make_float4(0.f, 0.f, 0.f, 0.f);
-  // this lane's column (the lanes of a dead query spoil only their own, which no sum takes)
-  char* column = reinterpret_cast<char*>(columns + wave * n_rows * kColumns + lane % kColumns);
+  sums.stage(rel, a, root_hd, dynamic);
   stage(0);
   const int64_t n_chunks = (L + kTile - 1) / kTile;
   if (n_chunks > 1) fetch(kTile);
@@ -249,14 +355,13 @@ relative_bwd_q_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int32
   constexpr std::true_type full{};
   constexpr std::false_type part{};
   // p and dp of this lane's query with chunk c's keys, zeros past the n-th (a full chunk has no branch)
-  auto pairs = [&](auto whole, int buf, int64_t c, int n, f32x4_t (&p)[4], f32x4_t (&dp)[4]) {
+  auto pairs = [&](auto whole, int buf, int64_t c, int n, int (&at)[4][4], f32x4_t (&p)[4], f32x4_t (&dp)[4]) {
     constexpr bool kWhole = decltype(whole)::value;
-    int at[4][4];
     pair_offsets(side, n_latents, sc[buf], int(c * kTile), g, at);
 #pragma unroll
     for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
-      for (int t = 0; t < 4; ++t) p[tt][t] = entry(table, at[tt][t]);
+      for (int t = 0; t < 4; ++t) p[tt][t] = entry(dynamic, at[tt][t]);
     products_onto<kHalf, HD>(sk[buf], kWhole ? kTile : n, l16, g, qf, p);
     products<kHalf, HD>(sv[buf], kWhole ? kTile : n, l16, g, gf, dp);
 #pragma unroll
@@ -279,113 +384,97 @@ relative_bwd_q_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int32
     dl += sum;
   };
   ColumnScale<kHalf> cs;
-  // ds (in p's place) into the buckets' sums and dq
-  auto spread = [&](auto whole, int buf, int64_t c, int n, f32x4_t (&p)[4], const f32x4_t (&dp)[4]) {
-    constexpr bool kWhole = decltype(whole)::value;
-    int at[4][4];
-    pair_offsets(side, n_latents, sc[buf], int(c * kTile), g, at);
-#pragma unroll
-    for (int tt = 0; tt < 4; ++tt) {
-      if (!kWhole && 16 * tt >= n) break;  // uniform
-      uint32_t to[4];
-      float x[4];
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        to[t] = *reinterpret_cast<const uint32_t*>(dynamic + at[tt][t] + 4);
-        x[t] = p[tt][t] * (dp[tt][t] - dl);
-        // (a key past the last one adds nothing, whatever delta is)
-        if (!kWhole) x[t] = 16 * tt + t < n - 4 * g ? x[t] : 0.f;
-        if (kColumns < 16) x[t] = live ? x[t] : 0.f;  // (two queries share a column)
-        p[tt][t] = x[t];
-      }
-      if constexpr (kColumns == 64) {
-        add4(column, to, x);
-      } else {
-#pragma unroll
-        for (int turn = 0; turn < 64 / kColumns; ++turn) {
-          if (lane / kColumns == turn) add4(column, to, x);
-          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (the next group reads what this one wrote)
-        }
-      }
-    }
-    cs.apply(p, acc);
-    accumulate_parts<kHalf, HD>(sk[buf], kWhole ? kTile : n, l16, g, p, acc);
-  };
   f32x4_t p[4], dp[4];
+  int at[4][4];
   const bool working = first < L;  // wavefront-uniform: a live row here
   const int tail = int(L - (n_chunks - 1) * kTile);  // rows of the last chunk
-  if (n_chunks == 1) {
-    if (working) {
-      pairs(part, 0, 0, tail, p, dp);
-      sum_delta(p, dp);
-      dl = sum_xor32(sum_xor16(dl));
-      spread(part, 0, 0, tail, p, dp);
-    }
-  } else if (n_chunks == 2) {
-    f32x4_t p1[4], dp1[4];
-    if (working) {
-      pairs(full, 0, 0, kTile, p, dp);
-      sum_delta(p, dp);
-    }
-    stage(1);
-    __syncthreads();
-    if (working) {
-      pairs(part, 1, 1, tail, p1, dp1);
-      sum_delta(p1, dp1);
-      dl = sum_xor32(sum_xor16(dl));
-      spread(full, 0, 0, kTile, p, dp);
-      spread(part, 1, 1, tail, p1, dp1);
+  if constexpr (kColumns > 0) {
+    // ds (in p's place) into the buckets' sums and dq
+    auto spread = [&](auto whole, int buf, int n, const int (&at)[4][4], f32x4_t (&p)[4], const f32x4_t (&dp)[4]) {
+      constexpr bool kWhole = decltype(whole)::value;
+#pragma unroll
+      for (int tt = 0; tt < 4; ++tt) {
+        if (!kWhole && 16 * tt >= n) break;  // uniform
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          // (a key past the last one adds nothing, whatever delta is)
+          const float x = p[tt][t] * (dp[tt][t] - dl);
+          p[tt][t] = kWhole || 16 * tt + t < n - 4 * g ? x : 0.f;
+        }
+        sums.add(at[tt], p[tt], live);
+      }
+      cs.apply(p, acc);
+      accumulate_parts<kHalf, HD>(sk[buf], kWhole ? kTile : n, l16, g, p, acc);
+    };
+    if (n_chunks == 1) {
+      if (working) {
+        pairs(part, 0, 0, tail, at, p, dp);
+        sum_delta(p, dp);
+        dl = sum_xor32(sum_xor16(dl));
+        spread(part, 0, tail, at, p, dp);
+      }
+    } else {  // two
+      f32x4_t p1[4], dp1[4];
+      if (working) {
+        pairs(full, 0, 0, kTile, at, p, dp);
+        sum_delta(p, dp);
+      }
+      stage(1);
+      __syncthreads();
+      if (working) {
+        int at1[4][4];
+        pairs(part, 1, 1, tail, at1, p1, dp1);
+        sum_delta(p1, dp1);
+        dl = sum_xor32(sum_xor16(dl));
+        spread(full, 0, kTile, at, p, dp);
+        spread(part, 1, tail, at1, p1, dp1);
+      }
     }
   } else {
-    // step s: chunk s % n_chunks in buffer s % 2; the first n_chunks for delta
-    auto step = [&](auto whole, int64_t s, int64_t c, int n) {
-      const int buf = int(s & 1);
+    f32x4_t plain[G::kDt];  // sum p k
+#pragma unroll
+    for (int dt = 0; dt < G::kDt; ++dt) plain[dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    auto step = [&](auto whole, int64_t c, int n) {
+      const int buf = int(c & 1);
       if (working) {
-        pairs(whole, buf, c, n, p, dp);
-        if (s < n_chunks) sum_delta(p, dp);
-        else spread(whole, buf, c, n, p, dp);
-        if (s == n_chunks - 1) dl = sum_xor32(sum_xor16(dl));
+        pairs(whole, buf, c, n, at, p, dp);
+        sum_delta(p, dp);
+#pragma unroll
+        for (int tt = 0; tt < 4; ++tt) {
+          dp[tt] *= p[tt];
+          if (kHalf) p[tt] *= kPScale<kHalf>;
+        }
+        cs.apply(dp, acc);
+        accumulate_two<kHalf, HD>(sk[buf], decltype(whole)::value ? kTile : n, l16, g, dp, acc, p, plain);
       }
-      if (s + 1 < 2 * n_chunks) {
+      if (c + 1 < n_chunks) {
         stage(buf ^ 1);  // (its readers met the barrier of the step before)
-        if (s + 2 < 2 * n_chunks) fetch((s + 2) % n_chunks * kTile);
+        if (c + 2 < n_chunks) fetch((c + 2) * kTile);
       }
       __syncthreads();
     };
-    for (int64_t sweep = 0; sweep < 2 * n_chunks; sweep += n_chunks) {
-      for (int64_t c = 0; c + 1 < n_chunks; ++c) step(full, sweep + c, c, kTile);
-      step(part, sweep + n_chunks - 1, n_chunks - 1, tail);
-    }
+    for (int64_t c = 0; c + 1 < n_chunks; ++c) step(full, c, kTile);
+    step(part, n_chunks - 1, tail);
+    dl = sum_xor32(sum_xor16(dl));
+#pragma unroll
+    for (int dt = 0; dt < G::kDt; ++dt)
+#pragma unroll
+      for (int t = 0; t < 4; ++t) acc[dt][t] = fmaf(-dl / kPScale<kHalf> * cs.s, plain[dt][t], acc[dt][t]);
   }
   if (i < T) {
     store_row<kHalf, HD, true>(dq.row(pos, a, i), g, acc, scale / cs.s, live);
     if (g == 0) delta[pa * T + i] = live ? dl : 0.f;
   }
-  __syncthreads();
-  // eight threads to a bucket's columns, each those of two queries in every
-  // lane group, the eight starting apart so that a wavefront's reads meet other banks
-  const int first_dead = L - tile * kTile < kTile ? int(L - tile * kTile) : kTile;  // queries of this workgroup
-  for (int b0 = 0; b0 < rel.n_buckets; b0 += 32) {
-    const int b = b0 + int(threadIdx.x) / 8, eighth = threadIdx.x % 8;
-    float sum = 0.f;
-    if (b < rel.n_buckets)
-      for (int w = 0; w < kBwdWaves; ++w)
-#pragma unroll
-        for (int c = 0; c < kColumns / 8; ++c) {
-          const int col = (8 * c + eighth + 8 * (int(threadIdx.x) / 8)) % kColumns;
-          const float x = columns[(w * n_rows + b) * kColumns + col];
-          sum += 16 * w + col % 16 < first_dead ? x : 0.f;
-        }
-    sum += __shfl_xor(sum, 1);
-    sum += __shfl_xor(sum, 2);
-    sum += __shfl_xor(sum, 4);
-    if (b < rel.n_buckets && eighth == 0) part_sums[b] = sum;
+  if constexpr (kColumns > 0) {
+    __syncthreads();
+    sums.flush(L - tile * kTile < kTile ? int(L - tile * kTile) : kTile, part_sums);
   }
 }
 
-// dbias of one (head, bucket): the head's partial sums of the query pass, each
-// thread a fixed stride of them, joined in a fixed order.  Workgroups of the
-// key pass's launch do it, where a launch of their own would take 4 us.
+// dbias of one (head, bucket): the head's partial sums, each thread a fixed
+// stride of them, joined in a fixed order.  The query pass's are added up by
+// workgroups of the key pass's launch (a launch of their own takes 4 us), the
+// key pass's by one after it.
 __device__ __forceinline__ void sum_bias(const float* __restrict__ partial, int64_t n_parts, int n_buckets,
                                          uint32_t which, float* __restrict__ dbias) {
   __shared__ float sums[256];
@@ -400,13 +489,19 @@ __device__ __forceinline__ void sum_bias(const float* __restrict__ partial, int6
   if (threadIdx.x == 0) dbias[which] = sums[0];
 }
 
-template <bool kHalf, int HD>
+__global__ void __launch_bounds__(256)
+relative_bias_sum_kernel(const float* __restrict__ partial, int64_t n_parts, int n_buckets, float* __restrict__ dbias) {
+  sum_bias(partial, n_parts, n_buckets, blockIdx.x, dbias);
+}
+
+// kColumns > 0: with the bucket sums; 0: with the workgroups that add up the query pass's.
+template <bool kHalf, int HD, int kColumns>
 __global__ void __launch_bounds__(256)
 relative_bwd_kv_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int32_t* __restrict__ seq_lens, int heads,
                        int64_t T, int64_t n_pa, const float2* __restrict__ stats, float scale, float root_hd,
-                       const float* __restrict__ delta, RowsOut dk, RowsOut dv, const float* __restrict__ partial,
+                       const float* __restrict__ delta, RowsOut dk, RowsOut dv, float* __restrict__ partial,
                        float* __restrict__ dbias, uint32_t n_item_groups) {
-  if (blockIdx.x >= n_item_groups) {  // the workgroups after the items
+  if (!kColumns && blockIdx.x >= n_item_groups) {  // the workgroups after the items
     sum_bias(partial, n_pa / heads * ((T + kTile - 1) / kTile), rel.n_buckets, blockIdx.x - n_item_groups, dbias);
     return;
   }
@@ -426,11 +521,12 @@ relative_bwd_kv_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int3
   const int lane = threadIdx.x % 64, l16 = lane % 16, g = lane / 16;
   const int64_t first = tile * kTile + 16 * (threadIdx.x / 64), j = first + l16;
   const bool live = j < L;
-  constexpr float kPScale = kHalf ? 0x1p14f : 1.f;  // (probabilities are at most 1)
   f32x4_t ak[G::kDt], av[G::kDt];
 #pragma unroll
   for (int dt = 0; dt < G::kDt; ++dt) ak[dt] = av[dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   ColumnScale<kHalf> cs;
+  BucketSums<kColumns> sums(rel, dynamic);
+  float* part_sums = kColumns ? partial_of(partial, rel, n_pa, heads, n_tiles, pos, a, tile) : nullptr;
   if (tile * kTile < L) {  // workgroup-uniform
     const i32x4_t qrs = rows_of(q, pos, a, L), grs = rows_of(go, pos, a, L);
     Tile cq, cg;
@@ -462,9 +558,9 @@ relative_bwd_kv_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int3
     uint4 kf[G::kKs], vf[G::kKs];
     row_frags<kHalf, HD>(rows_of(k, pos, a, L), j, g, kf);
     row_frags<kHalf, HD>(rows_of(v, pos, a, L), j, g, vf);
-    const Side<false, 4> side(rel, coords_of(rel, pos, T, j, L), j < rel.n_latents);
+    const Side<false, kColumns ? 8 : 4> side(rel, coords_of(rel, pos, T, j, L), j < rel.n_latents);
     const int n_latents = int(rel.n_latents);
-    stage_bias(rel, a, root_hd, table);
+    sums.stage(rel, a, root_hd, dynamic);
     const float c_log2 = scale * kLog2e;
     stage(0);
     if (kTile < L) fetch(kTile);
@@ -479,7 +575,7 @@ relative_bwd_kv_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int3
 #pragma unroll
         for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
-          for (int t = 0; t < 4; ++t) p[tt][t] = entry(table, at[tt][t]);
+          for (int t = 0; t < 4; ++t) p[tt][t] = entry(dynamic, at[tt][t]);
         products_onto<kHalf, HD>(sq[buf], kWhole ? kTile : n, l16, g, kf, p);
         products<kHalf, HD>(sg[buf], kWhole ? kTile : n, l16, g, vf, ds);
 #pragma unroll
@@ -494,9 +590,16 @@ relative_bwd_kv_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int3
             ds[tt][t] = in ? p[tt][t] * (ds[tt][t] - d4[t]) : 0.f;
           }
         }
+        if constexpr (kColumns > 0) {
+#pragma unroll
+          for (int tt = 0; tt < 4; ++tt) {
+            if (!kWhole && 16 * tt >= n) break;  // uniform
+            sums.add(at[tt], ds[tt], live);
+          }
+        }
         if constexpr (kHalf) {
 #pragma unroll
-          for (int tt = 0; tt < 4; ++tt) p[tt] *= kPScale;
+          for (int tt = 0; tt < 4; ++tt) p[tt] *= kPScale<kHalf>;
         }
         accumulate_parts<kHalf, HD>(sg[buf], kWhole ? kTile : n, l16, g, p, av);
         cs.apply(ds, ak);
@@ -511,16 +614,19 @@ relative_bwd_kv_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int3
     const int64_t last = (L - 1) / kTile * kTile;
     for (int64_t qb = 0; qb < last; qb += kTile) chunk(std::true_type{}, qb, kTile);
     chunk(std::false_type{}, last, int(L - last));
+    sums.flush(L - tile * kTile < kTile ? int(L - tile * kTile) : kTile, part_sums);
+  } else if (kColumns) {
+    for (int b = threadIdx.x; b < rel.n_buckets; b += 256) part_sums[b] = 0.f;
   }
   if (j < T) {
     store_row<kHalf, HD, true>(dk.row(pos, a, j), g, ak, scale / cs.s, live);
-    store_row<kHalf, HD, true>(dv.row(pos, a, j), g, av, 1.f / kPScale, live);
+    store_row<kHalf, HD, true>(dv.row(pos, a, j), g, av, 1.f / kPScale<kHalf>, live);
   }
 }
 
 template <bool kHalf, int HD>
 constexpr size_t static_lds() {
-  return size_t(4 * kTile * RowTile<HD>::kPitch) * 2 + 2 * kTile * 4;  // (of the query pass)
+  return size_t(4 * kTile * RowTile<HD>::kPitch) * 2 + 2 * kTile * 4 * 4 + 1024;  // (the key pass's, the larger)
 }
 
 // the dynamic LDS that a kernel may ask for, set once per kernel and device
@@ -548,27 +654,37 @@ int32_t launch(const Rows& q, const Rows& k, const Rows& v, const Rows& go, cons
   const int n_disp = rel.nq * rel.nr;
   // Columns per wavefront: 64 unless that table keeps workgroups off the CU that the
   // registers would allow (three, with 64 dims two), then 32 or 16 with the lane
-  // groups in turn.  24 to 28 KB of 64 columns a wavefront against 32 and 16: MEASURED2
+  // groups in turn, or 8 where no more fit.  Query pass of 192 positions of 44-124 rows, 28
+  // buckets, with 64 / 32 / 16 columns: 35 / 30 / 33 us; of two lines of 2,049-4,096, 32
+  // buckets and 64 dims: 508 / 563 / 640; of 16 positions of 511-1,021, 52 buckets: 400 / 262 / 267.
   constexpr size_t fixed = static_lds<kHalf, HD>(), share = kLdsBytes / (HD == 64 ? 2 : 3);
   auto total = [&](int columns) { return fixed + table_bytes(n_disp, 8) + column_bytes(rel.n_buckets, columns); };
   const int columns = total(64) <= share ? 64 : total(32) <= share ? 32 : total(16) <= kLdsBytes ? 16 : 8;
   if (total(columns) > kLdsBytes) return MANTIS_E_ARG;
-  auto query_pass = [&](auto kernel, bool allowed) {
+  const size_t sums_lds = total(columns) - fixed, plain_lds = table_bytes(n_disp, 4);
+  const bool few = t <= 2 * kTile;  // the bucket sums go with the query pass
+  auto passes = [&](auto query, auto key, bool allowed) {
     if (!allowed) return false;
-    kernel<<<unsigned(grid), 256, total(columns) - fixed, st>>>(q, k, v, go, rel, seq_lens, heads, t, n_pa, stats,
-                                                                scale, root, delta, dq, partial);
+    query<<<unsigned(grid), 256, few ? sums_lds : plain_lds, st>>>(q, k, v, go, rel, seq_lens, heads, t, n_pa, stats,
+                                                                   scale, root, delta, dq, partial);
+    key<<<unsigned(few ? grid + heads * rel.n_buckets : grid), 256, few ? plain_lds : sums_lds, st>>>(
+        q, k, v, go, rel, seq_lens, heads, t, n_pa, stats, scale, root, delta, dk, dv, partial, dbias, uint32_t(grid));
     return true;
   };
-#define MANTIS_QUERY_PASS(C) \
-  query_pass(relative_bwd_q_kernel<kHalf, HD, C>, allow_lds<relative_bwd_q_kernel<kHalf, HD, C>>(kLdsBytes - fixed))
-  const bool queued = columns == 64   ? MANTIS_QUERY_PASS(64)
-                      : columns == 32 ? MANTIS_QUERY_PASS(32)
-                      : columns == 16 ? MANTIS_QUERY_PASS(16)
-                                      : MANTIS_QUERY_PASS(8);
-#undef MANTIS_QUERY_PASS
+#define MANTIS_PASSES(C)                                                                                    \
+  (few ? passes(relative_bwd_q_kernel<kHalf, HD, C>, relative_bwd_kv_kernel<kHalf, HD, 0>,                  \
+                allow_lds<relative_bwd_q_kernel<kHalf, HD, C>>(kLdsBytes - fixed))                          \
+       : passes(relative_bwd_q_kernel<kHalf, HD, 0>, relative_bwd_kv_kernel<kHalf, HD, C>,                  \
+                allow_lds<relative_bwd_kv_kernel<kHalf, HD, C>>(kLdsBytes - fixed)))
+  const bool queued = columns == 64   ? MANTIS_PASSES(64)
+                      : columns == 32 ? MANTIS_PASSES(32)
+                      : columns == 16 ? MANTIS_PASSES(16)
+                                      : MANTIS_PASSES(8);
+#undef MANTIS_PASSES
   if (!queued) return MANTIS_E_LAUNCH;
-  relative_bwd_kv_kernel<kHalf, HD><<<unsigned(grid + heads * rel.n_buckets), 256, table_bytes(n_disp, 4), st>>>(
-      q, k, v, go, rel, seq_lens, heads, t, n_pa, stats, scale, root, delta, dk, dv, partial, dbias, uint32_t(grid));
+  if (!few)
+    relative_bias_sum_kernel<<<unsigned(heads * rel.n_buckets), 256, 0, st>>>(partial, n_pos * n_tiles, rel.n_buckets,
+                                                                             dbias);
   return launched();
 }
 
