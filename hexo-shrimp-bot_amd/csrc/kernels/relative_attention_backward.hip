@@ -19,14 +19,15 @@
 // 128) keep p and dp in registers until delta is known.  Longer rows are met
 // once: dq = sum (p dp) k - delta sum p k, with two sums beside delta, and the
 // buckets' sums move to the key pass, which knows delta.  (A second sweep over
-// the keys instead: the query pass 511 us against MEASURED3 at two lines of 2,049-4,096.)
+// the keys instead: the two passes 511 + 285 us against 258 + 352 at two lines of 2,049-4,096 rows.)
 //
 // Precision: scores and dp are exact products of 16-bit rows summed in fp32.
 // The probabilities and ds enter their products as two 16-bit parts, hi + lo:
 // bf16 beside bf16 rows (16 significant bits), beside fp16 rows fp16 parts of the
 // value times a power of two that follows the largest of its column (22
 // bits of that one).  What is cut is 2^-17 of a term, under the 2^-9 or 2^-12
-// that the outputs round.  (fp32 MFMAs with widened rows: MEASURED.)
+// that the outputs round.  (fp32 MFMAs with widened
+// rows: the passes 1,741 + 957 us where these parts took 619 + 337.)
 //
 // The bias gradient: every lane adds its ds to its own column of the
 // workgroup's LDS table (a row of 64 lanes per bucket and wavefront: no two
@@ -652,14 +653,15 @@ int32_t launch(const Rows& q, const Rows& k, const Rows& v, const Rows& go, cons
   if (grid + heads * rel.n_buckets > 2147483647LL) return MANTIS_E_ARG;
   const float root = sqrtf(float(HD)), scale = 1.f / root;
   const int n_disp = rel.nq * rel.nr;
-  // Columns per wavefront: 64 unless that table keeps workgroups off the CU that the
-  // registers would allow (three, with 64 dims two), then 32 or 16 with the lane
-  // groups in turn, or 8 where no more fit.  Query pass of 192 positions of 44-124 rows, 28
-  // buckets, with 64 / 32 / 16 columns: 35 / 30 / 33 us; of two lines of 2,049-4,096, 32
-  // buckets and 64 dims: 508 / 563 / 640; of 16 positions of 511-1,021, 52 buckets: 400 / 262 / 267.
-  constexpr size_t fixed = static_lds<kHalf, HD>(), share = kLdsBytes / (HD == 64 ? 2 : 3);
+  // Columns per wavefront: 64 where that table leaves room for three workgroups on a CU
+  // (with 64 dims, whose registers allow two, for two), else 32 with the lane groups in two
+  // turns where two fit, else 16 or 8 in four or eight.  With 64 / 32 / 16 columns: the query
+  // pass of 192 positions of 44-124 rows, 32 dims, 28 buckets, 31 / 25 / 28 us; the key pass of
+  // 64 positions of 150-300 rows 50 / 43 / 59, of 16 positions of 511-1,021 rows, 16
+  // dims, 52 buckets, 258 / 171 / 185, of two lines of 2,049-4,096, 64 dims, 32 buckets, 352 / 396 / 475.
+  constexpr size_t fixed = static_lds<kHalf, HD>(), wide = kLdsBytes / (HD == 64 ? 2 : 3);
   auto total = [&](int columns) { return fixed + table_bytes(n_disp, 8) + column_bytes(rel.n_buckets, columns); };
-  const int columns = total(64) <= share ? 64 : total(32) <= share ? 32 : total(16) <= kLdsBytes ? 16 : 8;
+  const int columns = total(64) <= wide ? 64 : total(32) <= kLdsBytes / 2 ? 32 : total(16) <= kLdsBytes ? 16 : 8;
   if (total(columns) > kLdsBytes) return MANTIS_E_ARG;
   const size_t sums_lds = total(columns) - fixed, plain_lds = table_bytes(n_disp, 4);
   const bool few = t <= 2 * kTile;  // the bucket sums go with the query pass
