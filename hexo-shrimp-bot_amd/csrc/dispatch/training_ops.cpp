@@ -110,7 +110,7 @@ bool wants_grad(std::initializer_list<const Tensor*> tensors) {
 
 struct HeadRows {  // a (P, A, T, D) operand and its element strides as the kernels take them
   Tensor t;
-  int64_t strides[4];
+  int64_t strides[4] = {};
 };
 
 // whether t's rows are dense, 16-byte aligned and within their descriptors (a
@@ -126,22 +126,27 @@ bool row_strides(const Tensor& t, int64_t (&s)[4]) {
 }
 
 HeadRows head_rows(const Tensor& t) {
-  HeadRows r{t, {}};
+  HeadRows r{t};
   if (row_strides(t, r.strides)) return r;
   r.t = t.clone(at::MemoryFormat::Contiguous);
   TORCH_CHECK_VALUE(row_strides(r.t, r.strides), "a position's rows are past the kernel's 2 GiB");
   return r;
 }
 
-// an empty operand in t's layout, or contiguous where that layout's rows are not the kernels'
+// an empty operand in t's layout, or contiguous where t has gaps or that layout's rows are not the kernels'
 HeadRows head_rows_like(const Tensor& t) {
-  HeadRows r{at::empty_like(t), {}};
-  if (!row_strides(r.t, r.strides)) {
-    r.t = at::empty(t.sizes(), t.options());
-    row_strides(r.t, r.strides);
+  HeadRows r;
+  if (t.is_non_overlapping_and_dense()) {
+    r.t = at::empty_strided(t.sizes(), t.strides(), t.options());
+    if (row_strides(r.t, r.strides)) return r;
   }
+  r.t = at::empty(t.sizes(), t.options());
+  row_strides(r.t, r.strides);
   return r;
 }
+
+// (a conversion that is none costs a dispatch)
+Tensor as(const Tensor& t, at::ScalarType dtype) { return t.scalar_type() == dtype ? t : t.to(dtype); }
 
 void check_relative(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& bias, const Tensor& coords,
                     const Tensor& buckets, const Tensor& seq_lens, int64_t n_latents) {
@@ -196,7 +201,7 @@ Three relative(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tenso
   Tensor lse = at::empty({p, heads, t}, f32), stats = at::empty({p, heads, t, 2}, f32);
   if (out.t.numel() == 0) return {out.t, lse, stats};
   const HeadRows q = head_rows(q_), k = head_rows(k_), v = head_rows(v_);
-  const Tensor bias = bias_.to(at::kFloat).contiguous(), coords = coord_pairs(coords_),
+  const Tensor bias = as(bias_, at::kFloat).contiguous(), coords = coord_pairs(coords_),
                buckets = buckets_.contiguous(), seq_lens = seq_lens_.contiguous();
   check_status(mantis_relative_attention(
                    q.t.data_ptr(), q.strides, k.t.data_ptr(), k.strides, v.t.data_ptr(), v.strides,
@@ -234,8 +239,8 @@ Four relative_backward(const Tensor& q_, const Tensor& k_, const Tensor& v_, con
   const HeadRows dq = head_rows_like(q_), dk = head_rows_like(k_), dv = head_rows_like(v_);
   if (dq.t.numel() == 0) return {dq.t, dk.t, dv.t, at::zeros(bias_.sizes(), bias_.options())};
   const HeadRows q = head_rows(q_), k = head_rows(k_), v = head_rows(v_),
-                 go = head_rows(grad_out_.to(q_.scalar_type()));
-  const Tensor bias = bias_.to(at::kFloat).contiguous(), coords = coord_pairs(coords_),
+                 go = head_rows(as(grad_out_, q_.scalar_type()));
+  const Tensor bias = as(bias_, at::kFloat).contiguous(), coords = coord_pairs(coords_),
                buckets = buckets_.contiguous(), seq_lens = seq_lens_.contiguous(), stats = stats_.contiguous();
   Tensor dbias = at::empty({heads, n_buckets}, q_.options().dtype(at::kFloat));
   const int64_t bytes = mantis_relative_attention_backward_workspace(p, int32_t(heads), t, n_buckets);
@@ -248,7 +253,7 @@ Four relative_backward(const Tensor& q_, const Tensor& k_, const Tensor& v_, con
                    dq.t.data_ptr(), dq.strides, dk.t.data_ptr(), dk.strides, dv.t.data_ptr(), dv.strides,
                    dbias.data_ptr<float>(), error_flag(dev), stream_of(dev)),
                "relative_attention_backward");
-  return {dq.t, dk.t, dv.t, dbias.to(bias_.scalar_type())};
+  return {dq.t, dk.t, dv.t, as(dbias, bias_.scalar_type())};
 }
 
 // ------------------------------------------------------------- policy
@@ -323,7 +328,7 @@ Runs check_policy_backward(const Tensor& logits, const Tensor& offsets, const Te
   auto take = [](optional<Tensor>& grad, at::IntArrayRef shape, const char* name) {
     if (!grad || !grad->defined()) return;
     TORCH_CHECK_VALUE(grad->sizes() == shape, "the gradient of ", name, " must have shape ", shape);
-    grad = grad->to(at::kFloat).contiguous();
+    grad = as(*grad, at::kFloat).contiguous();
   };
   take(g.log_probs, {p, moves.size(1)}, "log_probs");
   take(g.entropy, {p}, "entropy");
@@ -431,6 +436,14 @@ MANTIS_OPERATOR(residual_dropout, dropout)
 MANTIS_OPERATOR(residual_dropout_backward, dropout_backward)
 #undef MANTIS_OPERATOR
 
+// In a backward without create_graph the operators' Autograd keys have nothing to do.
+struct BelowAutograd {
+  optional<at::AutoDispatchBelowADInplaceOrView> below;
+  BelowAutograd() {
+    if (!at::GradMode::is_enabled()) below.emplace();
+  }
+};
+
 struct RelativeAttention : torch::autograd::Function<RelativeAttention> {
   static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v,
                                const Tensor& bias, const Tensor& coords, const Tensor& buckets,
@@ -446,6 +459,7 @@ struct RelativeAttention : torch::autograd::Function<RelativeAttention> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     variable_list res(8);
     if (!grads[0].defined()) return res;
+    const BelowAutograd below;
     const auto s = ctx->get_saved_variables();
     std::tie(res[0], res[1], res[2], res[3]) = call_fused_attention_relative_backward().call(
         s[0], s[1], s[2], s[3], s[4], s[5], s[6], ctx->saved_data["n_latents"].toInt(), s[7], grads[0]);
@@ -476,6 +490,7 @@ struct PolicyLogProbs : torch::autograd::Function<PolicyLogProbs> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     variable_list res(4);
     auto given = [](const Tensor& t) { return t.defined() ? optional<Tensor>(t) : std::nullopt; };
+    const BelowAutograd below;
     const auto s = ctx->get_saved_variables();
     res[0] = call_policy_log_probs_backward().call(s[0], s[1], s[2], s[3], s[4], s[5], given(grads[0]),
                                                    given(grads[1]), given(grads[2]), given(grads[3]));
@@ -508,6 +523,7 @@ struct ResidualDropout : torch::autograd::Function<ResidualDropout> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     variable_list res(5);
     if (!grads[0].defined()) return res;
+    const BelowAutograd below;
     if (ctx->needs_input_grad(0))
       res[0] = call_residual_dropout_backward().call(grads[0], ctx->get_saved_variables()[0],
                                                      ctx->saved_data["p"].toDouble(), ctx->saved_data["salt"].toInt(),
