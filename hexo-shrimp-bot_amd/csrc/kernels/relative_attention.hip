@@ -93,7 +93,7 @@ relative_attention_kernel(Operand q, Operand k, Operand v, Relative rel, const i
   int64_t qrow[kSub];
 #pragma unroll
   for (int j = 0; j < kSub; ++j) {
-    qrow[j] = q0 + (wave * kSub + j) * 16 + l16;
+    qrow[j] = q0 + (kWaves * j + wave) * 16 + l16;  // (sub-tiles dealt over the wavefronts)
 #pragma unroll
     for (int ks = 0; ks < kKs; ++ks) {
       uint4 u = row_load16(qrs, int32_t(qrow[j]), 2 * kdim(ks));
@@ -102,32 +102,38 @@ relative_attention_kernel(Operand q, Operand k, Operand v, Relative rel, const i
     }
   }
 
-  // staging role of this thread: kPer 16-byte pieces of the chunk's K and V rows, a row's coordinates
+  // staging role of this thread: kPer 16-byte pieces of a chunk's K and V rows, a row's coordinates.
+  // kSub 2 holds a position of at most two chunks: both are requested at once and met without a
+  // barrier in between; else the next chunk's are in registers while one is met.
+  constexpr bool kAll = kSub == 2;
   const bool stager = int(threadIdx.x) < kPieces;
-  uint4 kreg[kPer], vreg[kPer];
-  uint32_t creg = 0u;
-  auto fetch = [&](int64_t kb) {
+  struct Pieces {
+    uint4 k[kPer], v[kPer];
+    uint32_t c;
+  } held[kAll ? 2 : 1];
+  auto fetch = [&](Pieces& h, int64_t kb) {
 #pragma unroll
     for (int r = 0; r < kPer; ++r) {
       const int i = int(threadIdx.x) + 256 * r;
       const int32_t row = stager ? int32_t(kb) + i / (HD / 8) : -1;
-      kreg[r] = row_load16(krs, row, 16 * (i % (HD / 8)));
-      vreg[r] = row_load16(vrs, row, 16 * (i % (HD / 8)));
+      h.k[r] = row_load16(krs, row, 16 * (i % (HD / 8)));
+      h.v[r] = row_load16(vrs, row, 16 * (i % (HD / 8)));
     }
-    if (threadIdx.x < kKChunk) creg = coords_of(rel, p, T, kb + threadIdx.x, L);
+    h.c = threadIdx.x < kKChunk ? coords_of(rel, p, T, kb + threadIdx.x, L) : 0u;
   };
-  auto stage = [&](int buf) {
-    if (threadIdx.x < kKChunk) sc[buf][threadIdx.x] = creg;
+  auto stage = [&](const Pieces& h, int buf) {
+    if (threadIdx.x < kKChunk) sc[buf][threadIdx.x] = h.c;
     if (!stager) return;
 #pragma unroll
     for (int r = 0; r < kPer; ++r) {
       const int i = int(threadIdx.x) + 256 * r;
       const int st_key = i / (HD / 8), st_d = 8 * (i % (HD / 8));
-      *reinterpret_cast<uint4*>(&sk[buf][st_key * kKPitch + st_d]) = kreg[r];
-      *reinterpret_cast<uint4*>(&sv[buf][st_key * kKPitch + st_d]) = vreg[r];
+      *reinterpret_cast<uint4*>(&sk[buf][st_key * kKPitch + st_d]) = h.k[r];
+      *reinterpret_cast<uint4*>(&sv[buf][st_key * kKPitch + st_d]) = h.v[r];
     }
   };
-  fetch(0);
+  fetch(held[0], 0);
+  if (kAll) fetch(held[kAll], kKChunk);
   uint32_t qc[kSub];
 #pragma unroll
   for (int j = 0; j < kSub; ++j) qc[j] = coords_of(rel, p, T, qrow[j], L);
@@ -156,7 +162,7 @@ relative_attention_kernel(Operand q, Operand k, Operand v, Relative rel, const i
   // one chunk for the first kNJ sub-tiles (those with a live query)
   auto chunk = [&](auto nj, auto masked, int buf, int64_t kb, bool more) {
     constexpr int kNJ = decltype(nj)::value;
-    if (more) fetch(kb + kKChunk);
+    if (!kAll && more) fetch(held[0], kb + kKChunk);
     if constexpr (kNJ > 0) {
       // keys of the last chunk: tiles of 16 past the last one are left out (uniform)
       constexpr bool kMasked = decltype(masked)::value;
@@ -243,7 +249,8 @@ relative_attention_kernel(Operand q, Operand k, Operand v, Relative rel, const i
         for (int j = 0; j < kNJ; ++j) lsum[j] = mfma16x16x32(ones, pf[j][h], lsum[j]);
       }
     }
-    if (more) stage(buf ^ 1);
+    if (kAll) return;
+    if (more) stage(held[0], buf ^ 1);
     __syncthreads();
   };
 
@@ -255,12 +262,13 @@ relative_attention_kernel(Operand q, Operand k, Operand v, Relative rel, const i
     for (int64_t ch = 0; ch < last; ++ch) chunk(nj, no, int(ch & 1), ch * kKChunk, true);
     chunk(nj, yes, int(last & 1), last * kKChunk, false);
   };
-  stage(0);
+  stage(held[0], 0);
+  if (kAll) stage(held[kAll], 1);
   __syncthreads();
-  const int64_t live_q = L - (q0 + wave * 16 * kSub);  // (wavefront-uniform)
-  if (kSub > 1 && live_q > 16) run(std::integral_constant<int, kSub>{});
-  else if (live_q > 0) run(std::integral_constant<int, 1>{});
-  else run(std::integral_constant<int, 0>{});
+  const int64_t subs = (L - q0 + 15) / 16;  // with a live query (wavefront-uniform)
+  if (kSub > 1 && subs > kWaves + wave) run(std::integral_constant<int, kSub>{});
+  else if (subs > wave) run(std::integral_constant<int, 1>{});
+  else if (!kAll) run(std::integral_constant<int, 0>{});
 #pragma unroll
   for (int j = 0; j < kSub; ++j) {
     const float lt = lsum[j][0], lr = sum_xor32(sum_xor16(lreal[j]));
