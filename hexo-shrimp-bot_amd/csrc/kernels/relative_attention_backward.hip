@@ -327,19 +327,22 @@ relative_bwd_q_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int32
     return;
   }
   const i32x4_t krs = rows_of(k, pos, a, L), vrs = rows_of(v, pos, a, L);
-  Tile ck, cv;
-  uint32_t cc = 0u;
-  auto fetch = [&](int64_t kb) {
-    ck.fetch(krs, int32_t(kb));
-    cv.fetch(vrs, int32_t(kb));
-    if (threadIdx.x < kTile) cc = coords_of(rel, pos, T, kb + threadIdx.x, L);
+  struct Held {
+    Tile k, v;
+    uint32_t c;
+  } held[kColumns ? 2 : 1];  // (both chunks of a short row are requested at once)
+  auto fetch = [&](Held& h, int64_t kb) {
+    h.k.fetch(krs, int32_t(kb));
+    h.v.fetch(vrs, int32_t(kb));
+    h.c = threadIdx.x < kTile ? coords_of(rel, pos, T, kb + threadIdx.x, L) : 0u;
   };
-  auto stage = [&](int buf) {
-    ck.stage(sk[buf]);
-    cv.stage(sv[buf]);
-    if (threadIdx.x < kTile) sc[buf][threadIdx.x] = cc;
+  auto stage = [&](const Held& h, int buf) {
+    h.k.stage(sk[buf]);
+    h.v.stage(sv[buf]);
+    if (threadIdx.x < kTile) sc[buf][threadIdx.x] = h.c;
   };
-  fetch(0);
+  fetch(held[0], 0);
+  if (kColumns) fetch(held[kColumns != 0], kTile);
   uint4 qf[G::kKs], gf[G::kKs];
   row_frags<kHalf, HD>(rows_of(q, pos, a, L), i, g, qf);
   row_frags<kHalf, HD>(rows_of(go, pos, a, L), i, g, gf);
@@ -347,9 +350,10 @@ relative_bwd_q_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int32
   const Side<true, kColumns ? 8 : 4> side(rel, coords_of(rel, pos, T, i, L), i < rel.n_latents);
   const int n_latents = int(rel.n_latents);
   sums.stage(rel, a, root_hd, dynamic);
-  stage(0);
+  stage(held[0], 0);
   const int64_t n_chunks = (L + kTile - 1) / kTile;
-  if (n_chunks > 1) fetch(kTile);
+  if (kColumns) stage(held[kColumns != 0], 1);
+  else if (n_chunks > 1) fetch(held[0], kTile);
   __syncthreads();
 
   const float c_log2 = scale * kLog2e;
@@ -417,13 +421,9 @@ relative_bwd_q_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int32
     } else {  // two
       f32x4_t p1[4], dp1[4];
       if (working) {
+        int at1[4][4];
         pairs(full, 0, 0, kTile, at, p, dp);
         sum_delta(p, dp);
-      }
-      stage(1);
-      __syncthreads();
-      if (working) {
-        int at1[4][4];
         pairs(part, 1, 1, tail, at1, p1, dp1);
         sum_delta(p1, dp1);
         dl = sum_xor32(sum_xor16(dl));
@@ -449,8 +449,8 @@ relative_bwd_q_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int32
         accumulate_two<kHalf, HD>(sk[buf], decltype(whole)::value ? kTile : n, l16, g, dp, acc, p, plain);
       }
       if (c + 1 < n_chunks) {
-        stage(buf ^ 1);  // (its readers met the barrier of the step before)
-        if (c + 2 < n_chunks) fetch((c + 2) * kTile);
+        stage(held[0], buf ^ 1);  // (its readers met the barrier of the step before)
+        if (c + 2 < n_chunks) fetch(held[0], (c + 2) * kTile);
       }
       __syncthreads();
     };
@@ -530,32 +530,35 @@ relative_bwd_kv_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int3
   float* part_sums = kColumns ? partial_of(partial, rel, n_pa, heads, n_tiles, pos, a, tile) : nullptr;
   if (tile * kTile < L) {  // workgroup-uniform
     const i32x4_t qrs = rows_of(q, pos, a, L), grs = rows_of(go, pos, a, L);
-    Tile cq, cg;
-    float rm = 0.f, rl = INFINITY, rd = 0.f;
-    uint32_t cc = 0u;
-    auto fetch = [&](int64_t qb) {
-      cq.fetch(qrs, int32_t(qb));
-      cg.fetch(grs, int32_t(qb));
+    struct Held {
+      Tile q, g;
+      float m, l, d;
+      uint32_t c;
+    } held[kColumns ? 1 : 2];  // (both chunks of a short row are requested at once)
+    auto fetch = [&](Held& h, int64_t qb) {
+      h.q.fetch(qrs, int32_t(qb));
+      h.g.fetch(grs, int32_t(qb));
       if (threadIdx.x < kTile) {
         const int64_t i = qb + threadIdx.x;
         const bool in = i < L;
         const float2 st = in ? stats[pa * T + i] : make_float2(0.f, INFINITY);
-        rm = st.x, rl = st.y;
-        rd = in ? delta[pa * T + i] : 0.f;
-        cc = coords_of(rel, pos, T, i, L);
+        h.m = st.x, h.l = st.y;
+        h.d = in ? delta[pa * T + i] : 0.f;
+        h.c = coords_of(rel, pos, T, i, L);
       }
     };
-    auto stage = [&](int buf) {
-      cq.stage(sq[buf]);
-      cg.stage(sg[buf]);
+    auto stage = [&](const Held& h, int buf) {
+      h.q.stage(sq[buf]);
+      h.g.stage(sg[buf]);
       if (threadIdx.x < kTile) {
-        sm[buf][threadIdx.x] = rm;
-        sl[buf][threadIdx.x] = rl;
-        sd[buf][threadIdx.x] = rd;
-        sc[buf][threadIdx.x] = cc;
+        sm[buf][threadIdx.x] = h.m;
+        sl[buf][threadIdx.x] = h.l;
+        sd[buf][threadIdx.x] = h.d;
+        sc[buf][threadIdx.x] = h.c;
       }
     };
-    fetch(0);
+    fetch(held[0], 0);
+    if (!kColumns) fetch(held[!kColumns], kTile);
     uint4 kf[G::kKs], vf[G::kKs];
     row_frags<kHalf, HD>(rows_of(k, pos, a, L), j, g, kf);
     row_frags<kHalf, HD>(rows_of(v, pos, a, L), j, g, vf);
@@ -563,8 +566,9 @@ relative_bwd_kv_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int3
     const int n_latents = int(rel.n_latents);
     sums.stage(rel, a, root_hd, dynamic);
     const float c_log2 = scale * kLog2e;
-    stage(0);
-    if (kTile < L) fetch(kTile);
+    stage(held[0], 0);
+    if (!kColumns) stage(held[!kColumns], 1);
+    else if (kTile < L) fetch(held[0], kTile);
     __syncthreads();
     auto chunk = [&](auto whole, int64_t qb, int n) {
       constexpr bool kWhole = decltype(whole)::value;  // (a full chunk has no branch)
@@ -606,9 +610,10 @@ relative_bwd_kv_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int3
         cs.apply(ds, ak);
         accumulate_parts<kHalf, HD>(sq[buf], kWhole ? kTile : n, l16, g, ds, ak);
       }
+      if (!kColumns) return;
       if (qb + kTile < L) {
-        stage(buf ^ 1);  // (its readers met the barrier of the chunk before)
-        if (qb + 2 * kTile < L) fetch(qb + 2 * kTile);
+        stage(held[0], buf ^ 1);  // (its readers met the barrier of the chunk before)
+        if (qb + 2 * kTile < L) fetch(held[0], qb + 2 * kTile);
       }
       __syncthreads();
     };

@@ -10,6 +10,8 @@
 // salt) under the 64-bit key `seed`, with (seed, step) read on the device, so a
 // captured graph draws another mask when the caller advances step.
 // Sums and products are fp32 (one fma), the output rounds once.
+#include <cmath>
+
 #include "common.hpp"
 
 namespace mantis {
@@ -122,7 +124,7 @@ extern "C" int32_t mantis_residual_dropout(const void* x, int32_t x_dtype, const
       reinterpret_cast<uintptr_t>(residual) % width(out_dtype) || reinterpret_cast<uintptr_t>(rng) % 8)
     return MANTIS_E_ARG;
   // p within 2^-33 of 1 drops every element, as p = 1 does
-  const double border = p * 4294967296.0 + 0.5;
+  const double border = std::nearbyint(p * 4294967296.0);
   const bool none = border >= 4294967296.0;
   const uint32_t threshold = none ? 0xFFFFFFFFu : uint32_t(border);
   const float scale = none ? 0.f : float(1.0 / (1.0 - p));
