@@ -5,21 +5,28 @@
 // A live row whose every key has bias -inf gives zeros and lse -inf; rows past L
 // give zeros and lse 0.
 //
-// One workgroup serves an item (position, head, query tile of 4 kSub 16 rows); each
-// of its four wavefronts owns kSub 16-query sub-tiles and the keys stream
+// One workgroup serves an item (position, head, query tile of 4 kSub 16 rows);
+// each of its four wavefronts owns kSub 16-query sub-tiles and the keys stream
 // through LDS in 64-key chunks, double-buffered, the next one's rows in
-// registers meanwhile.  The transposed products S^T = K Q^T and O^T += V^T P^T keep a
-// lane on one query, and a score fragment is the next product's B operand as it
-// stands.  The bias is the score product's C operand (relative_bias.hpp), so
-// adding it costs the lookup alone.
+// registers meanwhile (where such tiles are few, few_groups, an item has 16
+// queries, each wavefront its own chunks, and their sums join at the end).  The
+// transposed products S^T = K Q^T and O^T += V^T P^T keep a lane on one query, and
+// a score fragment is the next product's B operand as it stands.  The bias is the
+// score product's C operand (relative_bias.hpp), so adding it costs the lookup alone.
 //
 // Softmax: p = exp2(c (s - m)), c = log2(e) / sqrt(hd), over the raw scores
 // (bias * sqrt(hd) included), in fp32 and with the difference first, so a row
 // of scores at the type's lowest value is still uniform; m moves only when a
-// score passes it by more than 8 in log2 units.  The probabilities enter the value product rounded to
-// 16 bits (relative 2^-9 or 2^-12 of each, as their output rounds once more);
-// the output is divided by the sum of the rounded ones, so a row of one key
-// is that key's value, and lse is the log of the unrounded fp32 sum.
+// score passes it by more than 8 in log2 units.  The probabilities enter the
+// value product rounded to 16 bits (relative 2^-9 or 2^-12 of each, as their
+// output rounds once more); the output is divided by the sum of the rounded ones,
+// so a row of one key is that key's value, and lse is the log of the unrounded fp32 sum.
+//
+// Bound by the pairs' vector work (table offset, lookup, maximum, exp2, sum, pack:
+// some 20 instructions for each, against 4 hd matrix operations), not by memory.
+// Measured: 512 positions of 44-124 rows, 4 heads, 32 dims, 27 us (q, k, v and out
+// at the rate of a large copy: 10); 192 of them 14.6; 16 of 511-1,021 rows, 8 heads
+// of 16 dims, 60; two lines of 2,049-4,096 rows, 2 heads of 64 dims, 136.
 #include <type_traits>
 
 #include "attention_rows.hpp"
@@ -30,28 +37,30 @@ namespace {
 
 constexpr int kWaves = 4;
 constexpr int kKChunk = 64;
-constexpr float kLazyLog2 = 8.f;       // probabilities up to 2^8 before the reference point moves
+constexpr float kLazyLog2 = 8.f;  // probabilities up to 2^8 before the reference point moves
 
 struct Operand {  // (P, A, T, hd): base and element strides
   const uint16_t* p;
   int64_t sp, sa, st;
 };
 
-template <bool kHalf, int HD, int kSub>
+// kSplit (kSub 1): an item has 16 queries, and its wavefronts every fourth chunk of keys each.
+template <bool kHalf, int HD, int kSub, bool kSplit>
 __global__ void __launch_bounds__(256)
 relative_attention_kernel(Operand q, Operand k, Operand v, Relative rel, const int32_t* __restrict__ seq_lens,
                           int heads, int64_t T, uint16_t* __restrict__ out, int64_t osp, int64_t osa, int64_t ost,
                           float* __restrict__ lse, float2* __restrict__ stats, float c_log2, float root_hd, int64_t n_pa) {
-  constexpr int kQTile = kWaves * 16 * kSub;
+  constexpr int kQTile = (kSplit ? 1 : kWaves) * 16 * kSub;
+  constexpr int kStagers = kSplit ? 64 : 256, kBufs = kSplit ? kWaves : 2;
   constexpr int kKPitch = HD + 8;              // 16-bit elements per staged K or V row
   constexpr int kKs = HD < 32 ? 1 : HD / 32;   // K steps of the score product
   constexpr int kDt = HD / 16;                 // 16-dim output tiles
   constexpr int kPieces = kKChunk * HD / 8;    // 16-byte pieces of a chunk's K (or V) rows
-  constexpr int kPer = kPieces < 256 ? 1 : kPieces / 256;
+  constexpr int kPer = kPieces < kStagers ? 1 : kPieces / kStagers;
   extern __shared__ float table[];  // the head's bias per displacement
-  __shared__ __attribute__((aligned(16))) uint16_t sk[2][kKChunk * kKPitch];
-  __shared__ __attribute__((aligned(16))) uint16_t sv[2][kKChunk * kKPitch];
-  __shared__ __attribute__((aligned(16))) uint32_t sc[2][kKChunk];
+  __shared__ __attribute__((aligned(16))) uint16_t sk[kBufs][kKChunk * kKPitch];
+  __shared__ __attribute__((aligned(16))) uint16_t sv[kBufs][kKChunk * kKPitch];
+  __shared__ __attribute__((aligned(16))) uint32_t sc[kBufs][kKChunk];
   const int64_t n_qt = (T + kQTile - 1) / kQTile;
   const Item item = item_of(n_pa, heads, n_qt);
   if (item.pa >= n_pa) return;
@@ -93,7 +102,7 @@ relative_attention_kernel(Operand q, Operand k, Operand v, Relative rel, const i
   int64_t qrow[kSub];
 #pragma unroll
   for (int j = 0; j < kSub; ++j) {
-    qrow[j] = q0 + (kWaves * j + wave) * 16 + l16;  // (sub-tiles dealt over the wavefronts)
+    qrow[j] = q0 + (kSplit ? 0 : kWaves * j + wave) * 16 + l16;  // (sub-tiles dealt over the wavefronts)
 #pragma unroll
     for (int ks = 0; ks < kKs; ++ks) {
       uint4 u = row_load16(qrs, int32_t(qrow[j]), 2 * kdim(ks));
@@ -106,7 +115,7 @@ relative_attention_kernel(Operand q, Operand k, Operand v, Relative rel, const i
   // kSub 2 holds a position of at most two chunks: both are requested at once and met without a
   // barrier in between; else the next chunk's are in registers while one is met.
   constexpr bool kAll = kSub == 2;
-  const bool stager = int(threadIdx.x) < kPieces;
+  const int stager = int(threadIdx.x) % kStagers;
   struct Pieces {
     uint4 k[kPer], v[kPer];
     uint32_t c;
@@ -114,25 +123,25 @@ relative_attention_kernel(Operand q, Operand k, Operand v, Relative rel, const i
   auto fetch = [&](Pieces& h, int64_t kb) {
 #pragma unroll
     for (int r = 0; r < kPer; ++r) {
-      const int i = int(threadIdx.x) + 256 * r;
-      const int32_t row = stager ? int32_t(kb) + i / (HD / 8) : -1;
+      const int i = stager + kStagers * r;
+      const int32_t row = i < kPieces ? int32_t(kb) + i / (HD / 8) : -1;
       h.k[r] = row_load16(krs, row, 16 * (i % (HD / 8)));
       h.v[r] = row_load16(vrs, row, 16 * (i % (HD / 8)));
     }
-    h.c = threadIdx.x < kKChunk ? coords_of(rel, p, T, kb + threadIdx.x, L) : 0u;
+    h.c = stager < kKChunk ? coords_of(rel, p, T, kb + stager, L) : 0u;
   };
   auto stage = [&](const Pieces& h, int buf) {
-    if (threadIdx.x < kKChunk) sc[buf][threadIdx.x] = h.c;
-    if (!stager) return;
+    if (stager < kKChunk) sc[buf][stager] = h.c;
 #pragma unroll
     for (int r = 0; r < kPer; ++r) {
-      const int i = int(threadIdx.x) + 256 * r;
+      const int i = stager + kStagers * r;
+      if (i >= kPieces) break;
       const int st_key = i / (HD / 8), st_d = 8 * (i % (HD / 8));
       *reinterpret_cast<uint4*>(&sk[buf][st_key * kKPitch + st_d]) = h.k[r];
       *reinterpret_cast<uint4*>(&sv[buf][st_key * kKPitch + st_d]) = h.v[r];
     }
   };
-  fetch(held[0], 0);
+  fetch(held[0], kSplit ? wave * kKChunk : 0);
   if (kAll) fetch(held[kAll], kKChunk);
   uint32_t qc[kSub];
 #pragma unroll
@@ -162,7 +171,13 @@ relative_attention_kernel(Operand q, Operand k, Operand v, Relative rel, const i
   // one chunk for the first kNJ sub-tiles (those with a live query)
   auto chunk = [&](auto nj, auto masked, int buf, int64_t kb, bool more) {
     constexpr int kNJ = decltype(nj)::value;
-    if (!kAll && more) fetch(held[0], kb + kKChunk);
+    if (kSplit) {
+      stage(held[0], buf);
+      if (kb + kWaves * kKChunk < L) fetch(held[0], kb + kWaves * kKChunk);
+      wave_sync();
+    } else if (!kAll && more) {
+      fetch(held[0], kb + kKChunk);
+    }
     if constexpr (kNJ > 0) {
       // keys of the last chunk: tiles of 16 past the last one are left out (uniform)
       constexpr bool kMasked = decltype(masked)::value;
@@ -249,7 +264,8 @@ relative_attention_kernel(Operand q, Operand k, Operand v, Relative rel, const i
         for (int j = 0; j < kNJ; ++j) lsum[j] = mfma16x16x32(ones, pf[j][h], lsum[j]);
       }
     }
-    if (kAll) return;
+    if (kSplit) wave_sync();
+    if (kAll || kSplit) return;
     if (more) stage(held[0], buf ^ 1);
     __syncthreads();
   };
@@ -259,16 +275,59 @@ relative_attention_kernel(Operand q, Operand k, Operand v, Relative rel, const i
     constexpr std::true_type yes{};
     constexpr std::false_type no{};
     const int64_t last = n_chunks - 1;  // only the last chunk can hold padding keys
-    for (int64_t ch = 0; ch < last; ++ch) chunk(nj, no, int(ch & 1), ch * kKChunk, true);
-    chunk(nj, yes, int(last & 1), last * kKChunk, false);
+    if constexpr (kSplit) {
+      int64_t ch = wave;
+      for (; ch < last; ch += kWaves) chunk(nj, no, wave, ch * kKChunk, true);
+      if (ch == last) chunk(nj, yes, wave, last * kKChunk, false);
+    } else {
+      for (int64_t ch = 0; ch < last; ++ch) chunk(nj, no, int(ch & 1), ch * kKChunk, true);
+      chunk(nj, yes, int(last & 1), last * kKChunk, false);
+    }
   };
-  stage(held[0], 0);
+  if (!kSplit) stage(held[0], 0);
   if (kAll) stage(held[kAll], 1);
   __syncthreads();
   const int64_t subs = (L - q0 + 15) / 16;  // with a live query (wavefront-uniform)
-  if (kSub > 1 && subs > kWaves + wave) run(std::integral_constant<int, kSub>{});
+  if (kSplit) run(std::integral_constant<int, 1>{});
+  else if (kSub > 1 && subs > kWaves + wave) run(std::integral_constant<int, kSub>{});
   else if (subs > wave) run(std::integral_constant<int, 1>{});
   else if (!kAll) run(std::integral_constant<int, 0>{});
+  if constexpr (kSplit) {
+    // the wavefronts' sums, in their order, brought to the largest of their reference points
+    constexpr int kN = 4 * kDt + 3;
+    static_assert((kWaves - 1) * kN * 64 * 4 <= sizeof(sk), "the tiles' LDS holds them");
+    float* room = reinterpret_cast<float*>(sk);
+    __syncthreads();
+    if (wave > 0) {
+      float* mine = room + (wave - 1) * kN * 64 + lane;
+      mine[0] = m[0];
+      mine[64] = lreal[0];
+      mine[128] = lsum[0][0];
+#pragma unroll
+      for (int i = 0; i < 4 * kDt; ++i) mine[(3 + i) * 64] = o[0][i / 4][i % 4];
+    }
+    __syncthreads();
+    if (wave > 0) return;
+    float top = m[0];
+#pragma unroll
+    for (int w = 0; w < kWaves - 1; ++w) top = fmaxf(top, room[w * kN * 64 + lane]);
+    auto factor = [&](float mw) { return mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mw - top) * c_log2); };
+    const float own = factor(m[0]);
+    lreal[0] *= own;
+    lsum[0][0] *= own;
+#pragma unroll
+    for (int i = 0; i < 4 * kDt; ++i) o[0][i / 4][i % 4] *= own;
+#pragma unroll
+    for (int w = 0; w < kWaves - 1; ++w) {
+      const float* theirs = room + w * kN * 64 + lane;
+      const float f = factor(theirs[0]);
+      lreal[0] = fmaf(theirs[64], f, lreal[0]);
+      lsum[0][0] = fmaf(theirs[128], f, lsum[0][0]);
+#pragma unroll
+      for (int i = 0; i < 4 * kDt; ++i) o[0][i / 4][i % 4] = fmaf(theirs[(3 + i) * 64], f, o[0][i / 4][i % 4]);
+    }
+    m[0] = top;
+  }
 #pragma unroll
   for (int j = 0; j < kSub; ++j) {
     const float lt = lsum[j][0], lr = sum_xor32(sum_xor16(lreal[j]));
@@ -294,15 +353,15 @@ relative_attention_kernel(Operand q, Operand k, Operand v, Relative rel, const i
   }
 }
 
-template <bool kHalf, int HD, int kSub>
+template <bool kHalf, int HD, int kSub, bool kSplit>
 int32_t launch(const Operand& q, const Operand& k, const Operand& v, const Relative& rel, const int32_t* seq_lens,
                int64_t n_pos, int heads, int64_t t, uint16_t* out, const int64_t* os, float* lse, float2* stats, hipStream_t st) {
-  constexpr int kQTile = kWaves * 16 * kSub;
+  constexpr int kQTile = (kSplit ? 1 : kWaves) * 16 * kSub;
   const int64_t grid = item_grid(n_pos, heads, (t + kQTile - 1) / kQTile);
   if (grid > 2147483647LL) return MANTIS_E_ARG;
   const size_t lds = size_t(rel.nq * rel.nr + 2) * sizeof(float);
   const float root = sqrtf(float(HD));
-  relative_attention_kernel<kHalf, HD, kSub><<<unsigned(grid), 256, lds, st>>>(
+  relative_attention_kernel<kHalf, HD, kSub, kSplit><<<unsigned(grid), 256, lds, st>>>(
       q, k, v, rel, seq_lens, heads, t, out, os[0], os[1], os[2], lse, stats, 1.4426950408889634f / root, root, n_pos * heads);
   return launched();
 }
@@ -342,16 +401,21 @@ extern "C" int32_t mantis_relative_attention(const void* q, const int64_t* qs, c
   uint16_t* o = static_cast<uint16_t*>(out);
   float2* sp = reinterpret_cast<float2*>(stats);
   hipStream_t st = as_stream(stream);
-#define MANTIS_FWD(HD_, SUB)                                                                                      \
-  return dtype == MANTIS_F16 ? launch<true, HD_, SUB>(Q, K, V, rel, seq_lens, n_pos, heads, t, o, os, lse, sp, st) \
-                             : launch<false, HD_, SUB>(Q, K, V, rel, seq_lens, n_pos, heads, t, o, os, lse, sp, st)
+#define MANTIS_FWD(HD_, ...)                                                                                       \
+  return dtype == MANTIS_F16                                                                                      \
+             ? launch<true, HD_, __VA_ARGS__>(Q, K, V, rel, seq_lens, n_pos, heads, t, o, os, lse, sp, st)        \
+             : launch<false, HD_, __VA_ARGS__>(Q, K, V, rel, seq_lens, n_pos, heads, t, o, os, lse, sp, st)
   // Two sub-tiles of 16 queries per wavefront read a key fragment once for both, and 128 queries hold
   // a usual position whole; one leaves the registers for twice the wavefronts: 192 positions of
   // 44-124 rows, 32 dims, 14.5 against 16.7 us, 64 of 150-300 rows 21.6 against 19.7; two lines of
   // 2,049-4,096 rows, 64 dims, 137 against 131, 16 positions of 511-1,021, 16 dims, 72 against 58.
-  if (hd == 16) MANTIS_FWD(16, 1);
-  if (hd == 32 && t <= 128) MANTIS_FWD(32, 2);
-  if (hd == 32) MANTIS_FWD(32, 1);
-  MANTIS_FWD(64, 1);
+  const bool split = few_groups(n_pos, heads, t, hd);
+  if (hd == 16 && split) MANTIS_FWD(16, 1, true);
+  if (hd == 16) MANTIS_FWD(16, 1, false);
+  if (hd == 32 && split) MANTIS_FWD(32, 1, true);
+  if (hd == 32 && t <= 128) MANTIS_FWD(32, 2, false);
+  if (hd == 32) MANTIS_FWD(32, 1, false);
+  if (split) MANTIS_FWD(64, 1, true);
+  MANTIS_FWD(64, 1, false);
 #undef MANTIS_FWD
 }

@@ -7,7 +7,9 @@
 //   dv_j = sum_i p_ij go_i,  dbias[a, b] = sum of ds_ij over the pairs of bucket b.
 //
 // Two passes, each a workgroup per (position, head, 64 rows), 16 rows per
-// wavefront, the other side's rows in 64-row chunks through LDS, two buffers:
+// wavefront, the other side's rows in 64-row chunks through LDS, two buffers
+// (where those are few workgroups, 16 rows each and the chunks dealt over the
+// wavefronts, whose sums join at the end in their order):
 //   query-major  S^T = K Q^T and dP^T = V dO^T, then dQ^T += K^T dS^T
 //   key-major    S = Q K^T and dP = dO V^T, then dV^T += dO^T P, dK^T += Q^T dS
 // Both keep a lane on one row of its own side, so a score fragment is the next
@@ -57,25 +59,25 @@ __host__ __device__ constexpr size_t column_bytes(int n_buckets, int columns) {
   return size_t(kBwdWaves) * (n_buckets + 1) * columns * 4;  // (a row for the pairs of no bucket)
 }
 
-// 64 rows of one operand: kPer 16-byte pieces per thread, in registers and then
-// in LDS at kPitch; rows at or past the descriptor's count are zeros.
-template <int HD>
+// 64 rows of one operand, staged by kThreads threads: kPer 16-byte pieces of each, in registers and
+// then in LDS at kPitch; rows at or past the descriptor's count are zeros.
+template <int HD, int kThreads>
 struct RowTile {
   static constexpr int kPitch = HD + 8;           // 16-bit elements
   static constexpr int kPieces = kTile * HD / 8;  // 16-byte pieces
-  static constexpr int kPer = kPieces < 256 ? 1 : kPieces / 256;
+  static constexpr int kPer = kPieces < kThreads ? 1 : kPieces / kThreads;
   uint4 reg[kPer];
   __device__ __forceinline__ void fetch(i32x4_t rows, int32_t first) {
 #pragma unroll
     for (int r = 0; r < kPer; ++r) {
-      const int i = int(threadIdx.x) + 256 * r;
+      const int i = int(threadIdx.x) % kThreads + kThreads * r;
       reg[r] = row_load16(rows, i < kPieces ? first + i / (HD / 8) : -1, 16 * (i % (HD / 8)));
     }
   }
   __device__ __forceinline__ void stage(uint16_t* s) const {
 #pragma unroll
     for (int r = 0; r < kPer; ++r) {
-      const int i = int(threadIdx.x) + 256 * r;
+      const int i = int(threadIdx.x) % kThreads + kThreads * r;
       if (i < kPieces) *reinterpret_cast<uint4*>(s + (i / (HD / 8)) * kPitch + 8 * (i % (HD / 8))) = reg[r];
     }
   }
@@ -253,9 +255,10 @@ struct BucketSums {
       }
     }
   }
-  // every bucket's sum over the columns of the workgroup's first n_live rows:
+  // every bucket's sum over the columns of the workgroup's first n_live rows
+  // (`step` rows on from a wavefront to the next; 0: the same 16 in each):
   // eight threads to a bucket, starting apart so that a wavefront's reads meet other banks
-  __device__ __forceinline__ void flush(int n_live, float* sums) const {
+  __device__ __forceinline__ void flush(int n_live, int step, float* sums) const {
     for (int b0 = 0; b0 < n_rows - 1; b0 += 32) {
       const int b = b0 + int(threadIdx.x) / 8, eighth = threadIdx.x % 8;
       float sum = 0.f;
@@ -265,7 +268,7 @@ struct BucketSums {
           for (int c = 0; c < kColumns / 8; ++c) {
             const int col = (8 * c + eighth + 8 * (int(threadIdx.x) / 8)) % kColumns;
             const float x = columns[(w * n_rows + b) * kColumns + col];
-            sum += 16 * w + col % 16 < n_live ? x : 0.f;
+            sum += step * w + col % 16 < n_live ? x : 0.f;
           }
       sum += __shfl_xor(sum, 1);
       sum += __shfl_xor(sum, 2);
@@ -283,7 +286,7 @@ struct BucketSums<0> {
     stage_bias(rel, head, root_hd, reinterpret_cast<float*>(dynamic));
   }
   __device__ __forceinline__ void add(const int (&)[4], const f32x4_t&, bool) {}
-  __device__ __forceinline__ void flush(int, float*) const {}
+  __device__ __forceinline__ void flush(int, int, float*) const {}
 };
 
 // The partial bucket sums of a workgroup: (head, position, tile, bucket).
@@ -292,33 +295,55 @@ __device__ __forceinline__ float* partial_of(float* partial, const Relative& rel
   return partial + ((a * (n_pa / heads) + pos) * n_tiles + tile) * rel.n_buckets;
 }
 
+// What the four wavefronts of a split workgroup hold of one row's sums, added
+// up in wavefront 0 in their order; `room` is LDS that no one reads any more.
+template <int kN>
+__device__ __forceinline__ void join_waves(float (&x)[kN], float* room) {
+  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+  __syncthreads();
+  if (wave > 0) {
+#pragma unroll
+    for (int k = 0; k < kN; ++k) room[((wave - 1) * kN + k) * 64 + lane] = x[k];
+  }
+  __syncthreads();
+  if (wave > 0) return;
+#pragma unroll
+  for (int k = 0; k < kN; ++k)
+#pragma unroll
+    for (int w = 0; w < kBwdWaves - 1; ++w) x[k] += room[(w * kN + k) * 64 + lane];
+}
+
 // kColumns > 0: at most two chunks of keys (T <= 128), with the bucket sums; 0: any number, without.
-template <bool kHalf, int HD, int kColumns>
+// kSplit (few_groups): a workgroup has 16 rows, and its wavefronts every fourth chunk of keys each.
+template <bool kHalf, int HD, int kColumns, bool kSplit>
 __global__ void __launch_bounds__(256)
 relative_bwd_q_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int32_t* __restrict__ seq_lens, int heads,
                       int64_t T, int64_t n_pa, const float2* __restrict__ stats, float scale, float root_hd,
                       float* __restrict__ delta, RowsOut dq, float* __restrict__ partial) {
   using G = Geom<kHalf, HD>;
-  using Tile = RowTile<HD>;
-  __shared__ __attribute__((aligned(16))) uint16_t sk[2][kTile * Tile::kPitch], sv[2][kTile * Tile::kPitch];
-  __shared__ __attribute__((aligned(16))) uint32_t sc[2][kTile];
+  static_assert(!kSplit || kColumns == 0, "split rows are long ones");
+  using Tile = RowTile<HD, kSplit ? 64 : 256>;
+  constexpr int kRows = kSplit ? 16 : kTile, kBufs = kSplit ? kBwdWaves : 2;
+  __shared__ __attribute__((aligned(16))) uint16_t sk[kBufs][kTile * Tile::kPitch], sv[kBufs][kTile * Tile::kPitch];
+  __shared__ __attribute__((aligned(16))) uint32_t sc[kBufs][kTile];
   extern __shared__ __attribute__((aligned(16))) char dynamic[];
-  const int64_t n_tiles = (T + kTile - 1) / kTile;
+  const int64_t n_tiles = (T + kRows - 1) / kRows;
   const Item item = item_of(n_pa, heads, n_tiles);
   if (item.pa >= n_pa) return;
   const int64_t pa = item.pa, tile = item.tile, pos = pa / heads, a = pa % heads;
   int64_t L = seq_lens[pos];
   L = L < 0 ? 0 : (L > T ? T : L);
   const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, l16 = lane % 16, g = lane / 16;
-  const int64_t first = tile * kTile + 16 * wave, i = first + l16;
+  const int64_t first = tile * kRows + (kSplit ? 0 : 16 * wave), i = first + l16;
+  const bool writer = !kSplit || wave == 0;
   const bool live = i < L;
   BucketSums<kColumns> sums(rel, dynamic);
   float* part_sums = kColumns ? partial_of(partial, rel, n_pa, heads, n_tiles, pos, a, tile) : nullptr;
   f32x4_t acc[G::kDt];
 #pragma unroll
   for (int dt = 0; dt < G::kDt; ++dt) acc[dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  if (tile * kTile >= L) {  // no live row
-    if (i < T) {
+  if (tile * kRows >= L) {  // no live row
+    if (i < T && writer) {
       store_row<kHalf, HD, true>(dq.row(pos, a, i), g, acc, 0.f, false);
       if (g == 0) delta[pa * T + i] = 0.f;
     }
@@ -334,14 +359,14 @@ relative_bwd_q_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int32
   auto fetch = [&](Held& h, int64_t kb) {
     h.k.fetch(krs, int32_t(kb));
     h.v.fetch(vrs, int32_t(kb));
-    h.c = threadIdx.x < kTile ? coords_of(rel, pos, T, kb + threadIdx.x, L) : 0u;
+    h.c = kSplit || threadIdx.x < kTile ? coords_of(rel, pos, T, kb + lane, L) : 0u;
   };
   auto stage = [&](const Held& h, int buf) {
     h.k.stage(sk[buf]);
     h.v.stage(sv[buf]);
-    if (threadIdx.x < kTile) sc[buf][threadIdx.x] = h.c;
+    if (kSplit || threadIdx.x < kTile) sc[buf][lane] = h.c;
   };
-  fetch(held[0], 0);
+  fetch(held[0], kSplit ? wave * kTile : 0);
   if (kColumns) fetch(held[kColumns != 0], kTile);
   uint4 qf[G::kKs], gf[G::kKs];
   row_frags<kHalf, HD>(rows_of(q, pos, a, L), i, g, qf);
@@ -350,10 +375,10 @@ relative_bwd_q_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int32
   const Side<true, kColumns ? 8 : 4> side(rel, coords_of(rel, pos, T, i, L), i < rel.n_latents);
   const int n_latents = int(rel.n_latents);
   sums.stage(rel, a, root_hd, dynamic);
-  stage(held[0], 0);
   const int64_t n_chunks = (L + kTile - 1) / kTile;
+  if (!kSplit) stage(held[0], 0);
   if (kColumns) stage(held[kColumns != 0], 1);
-  else if (n_chunks > 1) fetch(held[0], kTile);
+  else if (!kSplit && n_chunks > 1) fetch(held[0], kTile);
   __syncthreads();
 
   const float c_log2 = scale * kLog2e;
@@ -436,7 +461,12 @@ relative_bwd_q_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int32
 #pragma unroll
     for (int dt = 0; dt < G::kDt; ++dt) plain[dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     auto step = [&](auto whole, int64_t c, int n) {
-      const int buf = int(c & 1);
+      const int buf = kSplit ? wave : int(c & 1);
+      if (kSplit) {
+        stage(held[0], buf);
+        if (c + kBwdWaves < n_chunks) fetch(held[0], (c + kBwdWaves) * kTile);
+        wave_sync();
+      }
       if (working) {
         pairs(whole, buf, c, n, at, p, dp);
         sum_delta(p, dp);
@@ -448,15 +478,39 @@ relative_bwd_q_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int32
         cs.apply(dp, acc);
         accumulate_two<kHalf, HD>(sk[buf], decltype(whole)::value ? kTile : n, l16, g, dp, acc, p, plain);
       }
+      if (kSplit) {
+        wave_sync();
+        return;
+      }
       if (c + 1 < n_chunks) {
         stage(held[0], buf ^ 1);  // (its readers met the barrier of the step before)
         if (c + 2 < n_chunks) fetch(held[0], (c + 2) * kTile);
       }
       __syncthreads();
     };
-    for (int64_t c = 0; c + 1 < n_chunks; ++c) step(full, c, kTile);
-    step(part, n_chunks - 1, tail);
+    int64_t c = kSplit ? wave : 0;
+    for (; c + 1 < n_chunks; c += kSplit ? kBwdWaves : 1) step(full, c, kTile);
+    if (c + 1 == n_chunks) step(part, c, tail);
     dl = sum_xor32(sum_xor16(dl));
+    if constexpr (kSplit) {
+      float x[8 * G::kDt + 1];
+#pragma unroll
+      for (int k = 0; k < 4 * G::kDt; ++k) {
+        x[k] = acc[k / 4][k % 4] / cs.s;
+        x[4 * G::kDt + k] = plain[k / 4][k % 4];
+      }
+      x[8 * G::kDt] = dl;
+      static_assert((kBwdWaves - 1) * sizeof(x) * 64 <= sizeof(sk), "the tiles' LDS holds them");
+      join_waves(x, reinterpret_cast<float*>(sk));
+      if (wave > 0) return;
+      cs.s = 1.f;
+      dl = x[8 * G::kDt];
+#pragma unroll
+      for (int k = 0; k < 4 * G::kDt; ++k) {
+        acc[k / 4][k % 4] = x[k];
+        plain[k / 4][k % 4] = x[4 * G::kDt + k];
+      }
+    }
 #pragma unroll
     for (int dt = 0; dt < G::kDt; ++dt)
 #pragma unroll
@@ -468,7 +522,7 @@ relative_bwd_q_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int32
   }
   if constexpr (kColumns > 0) {
     __syncthreads();
-    sums.flush(L - tile * kTile < kTile ? int(L - tile * kTile) : kTile, part_sums);
+    sums.flush(L - tile * kTile < kTile ? int(L - tile * kTile) : kTile, 16, part_sums);
   }
 }
 
@@ -496,7 +550,8 @@ relative_bias_sum_kernel(const float* __restrict__ partial, int64_t n_parts, int
 }
 
 // kColumns > 0: with the bucket sums; 0: with the workgroups that add up the query pass's.
-template <bool kHalf, int HD, int kColumns>
+// kSplit (few_groups): a workgroup has 16 rows, and its wavefronts every fourth chunk of queries each.
+template <bool kHalf, int HD, int kColumns, bool kSplit>
 __global__ void __launch_bounds__(256)
 relative_bwd_kv_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int32_t* __restrict__ seq_lens, int heads,
                        int64_t T, int64_t n_pa, const float2* __restrict__ stats, float scale, float root_hd,
@@ -507,20 +562,21 @@ relative_bwd_kv_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int3
     return;
   }
   using G = Geom<kHalf, HD>;
-  using Tile = RowTile<HD>;
-  __shared__ __attribute__((aligned(16))) uint16_t sq[2][kTile * Tile::kPitch], sg[2][kTile * Tile::kPitch];
-  __shared__ __attribute__((aligned(16))) float sm[2][kTile], sl[2][kTile], sd[2][kTile];
-  __shared__ __attribute__((aligned(16))) uint32_t sc[2][kTile];
+  static_assert(!kSplit || kColumns > 0, "split rows are long ones");
+  using Tile = RowTile<HD, kSplit ? 64 : 256>;
+  constexpr int kRows = kSplit ? 16 : kTile, kBufs = kSplit ? kBwdWaves : 2;
+  __shared__ __attribute__((aligned(16))) uint16_t sq[kBufs][kTile * Tile::kPitch], sg[kBufs][kTile * Tile::kPitch];
+  __shared__ __attribute__((aligned(16))) float sm[kBufs][kTile], sl[kBufs][kTile], sd[kBufs][kTile];
+  __shared__ __attribute__((aligned(16))) uint32_t sc[kBufs][kTile];
   extern __shared__ __attribute__((aligned(16))) char dynamic[];
-  const int64_t n_tiles = (T + kTile - 1) / kTile;
+  const int64_t n_tiles = (T + kRows - 1) / kRows;
   const Item item = item_of(n_pa, heads, n_tiles);
   if (item.pa >= n_pa) return;
-  float* table = reinterpret_cast<float*>(dynamic);
   const int64_t pa = item.pa, tile = item.tile, pos = pa / heads, a = pa % heads;
   int64_t L = seq_lens[pos];
   L = L < 0 ? 0 : (L > T ? T : L);
-  const int lane = threadIdx.x % 64, l16 = lane % 16, g = lane / 16;
-  const int64_t first = tile * kTile + 16 * (threadIdx.x / 64), j = first + l16;
+  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, l16 = lane % 16, g = lane / 16;
+  const int64_t first = tile * kRows + (kSplit ? 0 : 16 * wave), j = first + l16;
   const bool live = j < L;
   f32x4_t ak[G::kDt], av[G::kDt];
 #pragma unroll
@@ -528,7 +584,7 @@ relative_bwd_kv_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int3
   ColumnScale<kHalf> cs;
   BucketSums<kColumns> sums(rel, dynamic);
   float* part_sums = kColumns ? partial_of(partial, rel, n_pa, heads, n_tiles, pos, a, tile) : nullptr;
-  if (tile * kTile < L) {  // workgroup-uniform
+  if (tile * kRows < L) {  // workgroup-uniform
     const i32x4_t qrs = rows_of(q, pos, a, L), grs = rows_of(go, pos, a, L);
     struct Held {
       Tile q, g;
@@ -538,8 +594,8 @@ relative_bwd_kv_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int3
     auto fetch = [&](Held& h, int64_t qb) {
       h.q.fetch(qrs, int32_t(qb));
       h.g.fetch(grs, int32_t(qb));
-      if (threadIdx.x < kTile) {
-        const int64_t i = qb + threadIdx.x;
+      if (kSplit || threadIdx.x < kTile) {
+        const int64_t i = qb + lane;
         const bool in = i < L;
         const float2 st = in ? stats[pa * T + i] : make_float2(0.f, INFINITY);
         h.m = st.x, h.l = st.y;
@@ -550,14 +606,14 @@ relative_bwd_kv_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int3
     auto stage = [&](const Held& h, int buf) {
       h.q.stage(sq[buf]);
       h.g.stage(sg[buf]);
-      if (threadIdx.x < kTile) {
-        sm[buf][threadIdx.x] = h.m;
-        sl[buf][threadIdx.x] = h.l;
-        sd[buf][threadIdx.x] = h.d;
-        sc[buf][threadIdx.x] = h.c;
+      if (kSplit || threadIdx.x < kTile) {
+        sm[buf][lane] = h.m;
+        sl[buf][lane] = h.l;
+        sd[buf][lane] = h.d;
+        sc[buf][lane] = h.c;
       }
     };
-    fetch(held[0], 0);
+    fetch(held[0], kSplit ? wave * kTile : 0);
     if (!kColumns) fetch(held[!kColumns], kTile);
     uint4 kf[G::kKs], vf[G::kKs];
     row_frags<kHalf, HD>(rows_of(k, pos, a, L), j, g, kf);
@@ -566,13 +622,18 @@ relative_bwd_kv_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int3
     const int n_latents = int(rel.n_latents);
     sums.stage(rel, a, root_hd, dynamic);
     const float c_log2 = scale * kLog2e;
-    stage(held[0], 0);
+    if (!kSplit) stage(held[0], 0);
     if (!kColumns) stage(held[!kColumns], 1);
-    else if (kTile < L) fetch(held[0], kTile);
+    else if (!kSplit && kTile < L) fetch(held[0], kTile);
     __syncthreads();
     auto chunk = [&](auto whole, int64_t qb, int n) {
       constexpr bool kWhole = decltype(whole)::value;  // (a full chunk has no branch)
-      const int buf = int(qb / kTile & 1);
+      const int buf = kSplit ? wave : int(qb / kTile & 1);
+      if (kSplit) {
+        stage(held[0], buf);
+        if (qb + kBwdWaves * kTile < L) fetch(held[0], qb + kBwdWaves * kTile);
+        wave_sync();
+      }
       if (first < L) {  // wavefront-uniform
         f32x4_t p[4], ds[4];
         int at[4][4];
@@ -610,7 +671,8 @@ relative_bwd_kv_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int3
         cs.apply(ds, ak);
         accumulate_parts<kHalf, HD>(sq[buf], kWhole ? kTile : n, l16, g, ds, ak);
       }
-      if (!kColumns) return;
+      if (kSplit) wave_sync();
+      if (!kColumns || kSplit) return;
       if (qb + kTile < L) {
         stage(held[0], buf ^ 1);  // (its readers met the barrier of the chunk before)
         if (qb + 2 * kTile < L) fetch(held[0], qb + 2 * kTile);
@@ -618,21 +680,40 @@ relative_bwd_kv_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int3
       __syncthreads();
     };
     const int64_t last = (L - 1) / kTile * kTile;
-    for (int64_t qb = 0; qb < last; qb += kTile) chunk(std::true_type{}, qb, kTile);
-    chunk(std::false_type{}, last, int(L - last));
-    sums.flush(L - tile * kTile < kTile ? int(L - tile * kTile) : kTile, part_sums);
+    int64_t qb = kSplit ? wave * kTile : 0;
+    for (; qb < last; qb += kSplit ? kBwdWaves * kTile : kTile) chunk(std::true_type{}, qb, kTile);
+    if (qb == last) chunk(std::false_type{}, last, int(L - last));
+    if constexpr (kSplit) {
+      float x[8 * G::kDt];
+#pragma unroll
+      for (int k = 0; k < 4 * G::kDt; ++k) {
+        x[k] = ak[k / 4][k % 4] / cs.s;
+        x[4 * G::kDt + k] = av[k / 4][k % 4];
+      }
+      static_assert((kBwdWaves - 1) * sizeof(x) * 64 <= sizeof(sq), "the tiles' LDS holds them");
+      join_waves(x, reinterpret_cast<float*>(sq));
+      cs.s = 1.f;
+#pragma unroll
+      for (int k = 0; k < 4 * G::kDt; ++k) {
+        ak[k / 4][k % 4] = x[k];
+        av[k / 4][k % 4] = x[4 * G::kDt + k];
+      }
+    }
+    sums.flush(L - tile * kRows < kRows ? int(L - tile * kRows) : kRows, kSplit ? 0 : 16, part_sums);
   } else if (kColumns) {
     for (int b = threadIdx.x; b < rel.n_buckets; b += 256) part_sums[b] = 0.f;
   }
-  if (j < T) {
+  if (j < T && (!kSplit || wave == 0)) {
     store_row<kHalf, HD, true>(dk.row(pos, a, j), g, ak, scale / cs.s, live);
     store_row<kHalf, HD, true>(dv.row(pos, a, j), g, av, 1.f / kPScale<kHalf>, live);
   }
 }
 
-template <bool kHalf, int HD>
-constexpr size_t static_lds() {
-  return size_t(4 * kTile * RowTile<HD>::kPitch) * 2 + 2 * kTile * 4 * 4 + 1024;  // (the key pass's, the larger)
+// static LDS of the passes (the key pass's, the larger)
+template <int HD>
+constexpr size_t static_lds(bool split) {
+  const int bufs = split ? kBwdWaves : 2;
+  return size_t(2 * bufs * kTile * (HD + 8)) * 2 + bufs * kTile * 4 * 4 + 1024;
 }
 
 // the dynamic LDS that a kernel may ask for, set once per kernel and device
@@ -653,19 +734,23 @@ template <bool kHalf, int HD>
 int32_t launch(const Rows& q, const Rows& k, const Rows& v, const Rows& go, const Relative& rel,
                const int32_t* seq_lens, int64_t n_pos, int heads, int64_t t, const float2* stats, float* delta,
                float* partial, const RowsOut& dq, const RowsOut& dk, const RowsOut& dv, float* dbias, hipStream_t st) {
-  const int64_t n_tiles = (t + kTile - 1) / kTile, n_pa = n_pos * heads;
+  const int n_disp = rel.nq * rel.nr;
+  bool split = few_groups(n_pos, heads, t, HD);
+  auto total = [&](int columns) {
+    return static_lds<HD>(split) + table_bytes(n_disp, 8) + column_bytes(rel.n_buckets, columns);
+  };
+  if (split && total(16) > kLdsBytes) split = false;
+  const int64_t rows = split ? 16 : kTile, n_tiles = (t + rows - 1) / rows, n_pa = n_pos * heads;
   const int64_t grid = item_grid(n_pos, heads, n_tiles);
   if (grid + heads * rel.n_buckets > 2147483647LL) return MANTIS_E_ARG;
   const float root = sqrtf(float(HD)), scale = 1.f / root;
-  const int n_disp = rel.nq * rel.nr;
   // Columns per wavefront: 64 where that table leaves room for three workgroups on a CU
-  // (with 64 dims, whose registers allow two, for two), else 32 with the lane groups in two
+  // (with 64 dims, whose registers allow two, for two; with 64 split, for one), else 32 with the lane groups in two
   // turns where two fit, else 16 or 8 in four or eight.  With 64 / 32 / 16 columns: the query
   // pass of 192 positions of 44-124 rows, 32 dims, 28 buckets, 31 / 25 / 28 us; the key pass of
   // 64 positions of 150-300 rows 50 / 43 / 59, of 16 positions of 511-1,021 rows, 16
   // dims, 52 buckets, 258 / 171 / 185, of two lines of 2,049-4,096, 64 dims, 32 buckets, 352 / 396 / 475.
-  constexpr size_t fixed = static_lds<kHalf, HD>(), wide = kLdsBytes / (HD == 64 ? 2 : 3);
-  auto total = [&](int columns) { return fixed + table_bytes(n_disp, 8) + column_bytes(rel.n_buckets, columns); };
+  const size_t fixed = static_lds<HD>(split), wide = kLdsBytes / (HD < 64 ? 3 : split ? 1 : 2);
   const int columns = total(64) <= wide ? 64 : total(32) <= kLdsBytes / 2 ? 32 : total(16) <= kLdsBytes ? 16 : 8;
   if (total(columns) > kLdsBytes) return MANTIS_E_ARG;
   const size_t sums_lds = total(columns) - fixed, plain_lds = table_bytes(n_disp, 4);
@@ -678,11 +763,15 @@ int32_t launch(const Rows& q, const Rows& k, const Rows& v, const Rows& go, cons
         q, k, v, go, rel, seq_lens, heads, t, n_pa, stats, scale, root, delta, dk, dv, partial, dbias, uint32_t(grid));
     return true;
   };
-#define MANTIS_PASSES(C)                                                                                    \
-  (few ? passes(relative_bwd_q_kernel<kHalf, HD, C>, relative_bwd_kv_kernel<kHalf, HD, 0>,                  \
-                allow_lds<relative_bwd_q_kernel<kHalf, HD, C>>(kLdsBytes - fixed))                          \
-       : passes(relative_bwd_q_kernel<kHalf, HD, 0>, relative_bwd_kv_kernel<kHalf, HD, C>,                  \
-                allow_lds<relative_bwd_kv_kernel<kHalf, HD, C>>(kLdsBytes - fixed)))
+  const size_t most = kLdsBytes - fixed;
+#define MANTIS_PASSES(C)                                                                                         \
+  (few     ? passes(relative_bwd_q_kernel<kHalf, HD, C, false>, relative_bwd_kv_kernel<kHalf, HD, 0, false>,     \
+                    allow_lds<relative_bwd_q_kernel<kHalf, HD, C, false>>(most))                                 \
+   : split ? passes(relative_bwd_q_kernel<kHalf, HD, 0, true>, relative_bwd_kv_kernel<kHalf, HD, C, true>,       \
+                    allow_lds<relative_bwd_q_kernel<kHalf, HD, 0, true>>(most) &&                                \
+                        allow_lds<relative_bwd_kv_kernel<kHalf, HD, C, true>>(most))                             \
+           : passes(relative_bwd_q_kernel<kHalf, HD, 0, false>, relative_bwd_kv_kernel<kHalf, HD, C, false>,     \
+                    allow_lds<relative_bwd_kv_kernel<kHalf, HD, C, false>>(most)))
   const bool queued = columns == 64   ? MANTIS_PASSES(64)
                       : columns == 32 ? MANTIS_PASSES(32)
                       : columns == 16 ? MANTIS_PASSES(16)
@@ -704,7 +793,8 @@ extern "C" int64_t mantis_relative_attention_backward_workspace(int64_t n_pos, i
                                                                 int64_t n_buckets) {
   if (n_pos <= 0 || heads <= 0 || t <= 0 || n_buckets <= 0) return 0;
   // delta, then the partial bias sums
-  return 4 * (n_pos * heads * t + n_pos * heads * ((t + kTile - 1) / kTile) * n_buckets);
+  const int64_t rows = few_groups(n_pos, heads, t, 16) ? 16 : kTile;  // (enough for every width)
+  return 4 * (n_pos * heads * t + n_pos * heads * ((t + rows - 1) / rows) * n_buckets);
 }
 
 extern "C" int32_t mantis_relative_attention_backward(

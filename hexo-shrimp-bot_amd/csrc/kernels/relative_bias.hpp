@@ -175,6 +175,21 @@ inline int64_t item_grid(int64_t n_pos, int heads, int64_t n_tiles) {
   return (units + kXcds - 1) / kXcds * kXcds * per;
 }
 
+// Long rows (T > 128) whose 64-row tiles leave half the CUs or more without a
+// workgroup: tiles of 16 rows, the other side's chunks dealt over a workgroup's
+// wavefronts.  Each stages its own, so the LDS grows with the head's width and at
+// 64 dims the few workgroups that fit a CU gain from this only when tiles are fewer
+// still.  The three passes of one position, 16 rows to a workgroup against 64: 2,000
+// rows of 4 heads, 32 dims (128 tiles of 64) 138 against 169 us, 16 dims 122 / 161;
+// 1,024 rows, 32 dims 54 / 93; 4,096 rows, 32 dims (256 tiles) 459 / 431, 16 dims 412 / 402;
+// 64 dims, 2 heads, 1,024 rows (32 tiles) 73 / 103, 2,048 rows (64 tiles) 226 / 200.
+inline bool few_groups(int64_t n_pos, int64_t heads, int64_t t, int64_t hd) {
+  return t > 128 && n_pos * heads * ((t + 63) / 64) <= (hd < 64 ? 128 : 32);
+}
+
+// orders a wavefront's own LDS accesses around a tile that no other one uses
+__device__ __forceinline__ void wave_sync() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
+
 inline bool good_relative(const Relative& rel, int64_t t) {
   if (!rel.coords || !rel.buckets || !rel.bias || reinterpret_cast<uintptr_t>(rel.coords) % 8) return false;
   if (rel.nq < 1 || rel.nr < 1 || rel.nq % 2 == 0 || rel.nr % 2 == 0) return false;

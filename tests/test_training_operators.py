@@ -468,6 +468,10 @@ BF, HF = torch.bfloat16, torch.float16
     ([80, 33], 2, 32, HF, {"n_buckets": 2, "n_latents": 40, "table": (1, 3)}),
     ([700, 511, 1021], 2, 32, BF, {"n_buckets": 97}),
     ([40, 20, 9] * 30, 4, 32, BF, {}),
+    ([129, 0, 150] * 15, 4, 32, HF, {}),  # 540 tiles of 64 rows: long rows that fill the chip
+    ([260, 40, 193] * 12, 3, 16, BF, {"extra": 9, "n_buckets": 384, "table": (63, 65), "spread": 20.0}),
+    ([129, 17, 192, 64] * 22, 2, 64, BF, {}),
+    ([129, 1, 0, 4, 16, 17, 145], 2, 64, HF, {"n_buckets": 384, "table": (1, 4095), "spread": 900.0}),
 ])
 def test_relative_attention(device, lens, heads, d, dtype, kw):
     case = relative_case(lens, heads, d, dtype, len(lens) + d, device=device, **kw)
