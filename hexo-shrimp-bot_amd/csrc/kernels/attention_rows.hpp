@@ -1,6 +1,6 @@
-// Row chunks and products shared by the backward passes of the ragged
-// attentions: a workgroup of four wavefronts, 16 rows of its own side each,
-// meets the other side's rows in 64-row chunks through LDS.
+// Row chunks and products shared by the ragged attentions' passes: a workgroup
+// of four wavefronts, 16 rows of its own side each, meets the other side's rows
+// in 64-row chunks through LDS.
 #pragma once
 
 #include "common.hpp"

