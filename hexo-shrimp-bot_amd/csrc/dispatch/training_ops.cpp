@@ -78,6 +78,8 @@ int32_t* error_flag(at::Device dev) {
   TORCH_CHECK(asked && status == hipStreamCaptureStatusNone,
               "the device's error flag does not exist yet: run the operator once before capturing it");
   set_error_words(at::zeros({2}, at::TensorOptions(at::kInt).device(dev)));
+  // (another stream's kernels may write them next)
+  TORCH_CHECK(hipStreamSynchronize(static_cast<hipStream_t>(stream_of(dev))) == hipSuccess, "the error flag's fill failed");
   std::lock_guard<std::mutex> hold(words_lock);
   return words_of[i]->data_ptr<int32_t>();
 }

@@ -113,15 +113,32 @@ struct Side {
     row_bytes = uint32_t(kEntry * rel.nr);
     latent_other = kEntry * (rel.nq * rel.nr + (kQuery || latent ? 0 : 1));
   }
-  __device__ __forceinline__ int at(uint32_t other) const {
-    const s16x2_t o = __builtin_bit_cast(s16x2_t, other);
-    s16x2_t d = kQuery ? __builtin_elementwise_sub_sat(o, own) : __builtin_elementwise_sub_sat(own, o);
-    d = __builtin_elementwise_max(__builtin_elementwise_min(d, hi), lo);
-    const uint32_t u = __builtin_bit_cast(uint32_t, d);
-    int r;
-    asm("v_mad_i32_i16 %0, %1, %2, 0 op_sel:[1,0,0,0]" : "=v"(r) : "v"(u), "n"(kEntry));  // (the high half)
-    asm("v_mad_i32_i16 %0, %1, %2, %3" : "=v"(r) : "v"(u), "s"(row_bytes), "v"(r));
-    return r;
+  // Four pairs side by side: saturating difference, clamps, column * entry bytes + row * row_bytes.
+  // (Such instructions wait a cycle for the one before; left to itself the compiler puts a
+  // pair's five in a row where registers are few, with an empty cycle after each: the passes of
+  // two lines of 2,049-4,096 rows, 64 dims, 254 + 339 against 245 + 333 us.)
+  __device__ __forceinline__ void at(uint4 other, int (&at)[4]) const {
+    const uint32_t l = __builtin_bit_cast(uint32_t, lo), h = __builtin_bit_cast(uint32_t, hi);
+    uint32_t o[4] = {other.x, other.y, other.z, other.w};
+#define MANTIS_FOUR(op, a, b, c, d) op a "\n" op b "\n" op c "\n" op d "\n"
+#define MANTIS_REST                                                                                              \
+  MANTIS_FOUR("v_pk_min_i16 ", "%4, %4, %10", "%5, %5, %10", "%6, %6, %10", "%7, %7, %10")                       \
+  MANTIS_FOUR("v_pk_max_i16 ", "%4, %4, %9", "%5, %5, %9", "%6, %6, %9", "%7, %7, %9")                           \
+  MANTIS_FOUR("v_mad_i32_i16 ", "%0, %4, %12, 0 op_sel:[1,0,0,0]", "%1, %5, %12, 0 op_sel:[1,0,0,0]",            \
+              "%2, %6, %12, 0 op_sel:[1,0,0,0]", "%3, %7, %12, 0 op_sel:[1,0,0,0]")                              \
+  MANTIS_FOUR("v_mad_i32_i16 ", "%0, %4, %11, %0", "%1, %5, %11, %1", "%2, %6, %11, %2", "%3, %7, %11, %3")
+#define MANTIS_OPERANDS                                                                                          \
+  : "=&v"(at[0]), "=&v"(at[1]), "=&v"(at[2]), "=&v"(at[3]), "+v"(o[0]), "+v"(o[1]), "+v"(o[2]), "+v"(o[3])      \
+  : "v"(own), "v"(l), "v"(h), "s"(row_bytes), "n"(kEntry)
+    if constexpr (kQuery)
+      asm(MANTIS_FOUR("v_pk_sub_i16 ", "%4, %4, %8 clamp", "%5, %5, %8 clamp", "%6, %6, %8 clamp", "%7, %7, %8 clamp")
+              MANTIS_REST MANTIS_OPERANDS);
+    else
+      asm(MANTIS_FOUR("v_pk_sub_i16 ", "%4, %8, %4 clamp", "%5, %8, %5 clamp", "%6, %8, %6 clamp", "%7, %8, %7 clamp")
+              MANTIS_REST MANTIS_OPERANDS);
+#undef MANTIS_FOUR
+#undef MANTIS_REST
+#undef MANTIS_OPERANDS
   }
 };
 
@@ -131,12 +148,7 @@ template <bool kQuery, int kEntry>
 __device__ __forceinline__ void pair_offsets(const Side<kQuery, kEntry>& side, int n_latents, const uint32_t* sc,
                                              int first, int g, int (&at)[4][4]) {
 #pragma unroll
-  for (int tt = 0; tt < 4; ++tt) {
-    const uint4 c = *reinterpret_cast<const uint4*>(&sc[16 * tt + 4 * g]);
-    const uint32_t cs[4] = {c.x, c.y, c.z, c.w};
-#pragma unroll
-    for (int t = 0; t < 4; ++t) at[tt][t] = side.at(cs[t]);
-  }
+  for (int tt = 0; tt < 4; ++tt) side.at(*reinterpret_cast<const uint4*>(&sc[16 * tt + 4 * g]), at[tt]);
   if (first < n_latents) {  // uniform
     asm volatile("");       // (a branch: most chunks hold no latent row)
     const int lat = n_latents - first - 4 * g;
