@@ -65,6 +65,8 @@ relative_attention_kernel(Operand q, Operand k, Operand v, Relative rel, const i
   const Item item = item_of(n_pa, heads, n_qt);
   if (item.pa >= n_pa) return;
   const int64_t pa = item.pa, qt = item.tile, p = pa / heads, a = pa % heads;
+  TableStage bias_table;
+  bias_table.request(rel);
   int64_t L = seq_lens[p];
   L = L < 0 ? 0 : (L > T ? T : L);
   const int64_t q0 = qt * kQTile;
@@ -143,10 +145,11 @@ relative_attention_kernel(Operand q, Operand k, Operand v, Relative rel, const i
   };
   fetch(held[0], kSplit ? wave * kKChunk : 0);
   if (kAll) fetch(held[kAll], kKChunk);
+  bias_table.biases(rel, a);
   uint32_t qc[kSub];
 #pragma unroll
   for (int j = 0; j < kSub; ++j) qc[j] = coords_of(rel, p, T, qrow[j], L);
-  stage_bias(rel, a, root_hd, table);
+  bias_table.finish(rel, a, root_hd, [&](int i, float x, int) { table[i] = x; });
   const Side<true, 4> side[2] = {{rel, qc[0], qrow[0] < rel.n_latents},
                                 {rel, qc[kSub - 1], qrow[kSub - 1] < rel.n_latents}};
   const int n_latents = int(rel.n_latents);

@@ -234,9 +234,10 @@ struct BucketSums {
     n_rows = rel.n_buckets + 1;
     own = reinterpret_cast<char*>(columns + threadIdx.x / 64 * n_rows * kColumns + threadIdx.x % kColumns);
   }
-  __device__ __forceinline__ void stage(const Relative& rel, int64_t head, float root_hd, char* dynamic) {
+  __device__ __forceinline__ void stage(TableStage& biases, const Relative& rel, int64_t head, float root_hd,
+                                        char* dynamic) {
     uint2* entries = reinterpret_cast<uint2*>(dynamic);
-    stage_table(rel, head, root_hd, [&](int d, float x, int b) {
+    biases.finish(rel, head, root_hd, [&](int d, float x, int b) {
       entries[d] = make_uint2(__float_as_uint(x), uint32_t(b) * kColumns * 4);
     });
     for (int c = threadIdx.x; c < kBwdWaves * n_rows * kColumns / 4; c += 256)
@@ -292,8 +293,9 @@ struct BucketSums<0> {
   const char* table;
   __device__ __forceinline__ BucketSums(const Relative&, char* dynamic) : table(dynamic) {}
   __device__ __forceinline__ float entry(int at) const { return mantis::entry(table, at); }
-  __device__ __forceinline__ void stage(const Relative& rel, int64_t head, float root_hd, char* dynamic) {
-    stage_bias(rel, head, root_hd, reinterpret_cast<float*>(dynamic));
+  __device__ __forceinline__ void stage(TableStage& biases, const Relative& rel, int64_t head, float root_hd,
+                                        char* dynamic) {
+    biases.finish(rel, head, root_hd, [&](int d, float x, int) { reinterpret_cast<float*>(dynamic)[d] = x; });
   }
   __device__ __forceinline__ void add(const int (&)[4], const f32x4_t&, bool) {}
   __device__ __forceinline__ void flush(int, int, float*) const {}
@@ -341,6 +343,8 @@ relative_bwd_q_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int32
   const Item item = item_of(n_pa, heads, n_tiles);
   if (item.pa >= n_pa) return;
   const int64_t pa = item.pa, tile = item.tile, pos = pa / heads, a = pa % heads;
+  TableStage biases;
+  biases.request(rel);
   int64_t L = seq_lens[pos];
   L = L < 0 ? 0 : (L > T ? T : L);
   const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, l16 = lane % 16, g = lane / 16;
@@ -378,13 +382,14 @@ relative_bwd_q_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int32
   };
   fetch(held[0], kSplit ? wave * kTile : 0);
   if (kColumns) fetch(held[kColumns != 0], kTile);
+  biases.biases(rel, a);
   uint4 qf[G::kKs], gf[G::kKs];
   row_frags<kHalf, HD>(rows_of(q, pos, a, L), i, g, qf);
   row_frags<kHalf, HD>(rows_of(go, pos, a, L), i, g, gf);
   const float2 st = live ? stats[pa * T + i] : make_float2(0.f, INFINITY);
   const Side<true, kColumns ? 8 : 4> side(rel, coords_of(rel, pos, T, i, L), i < rel.n_latents);
   const int n_latents = int(rel.n_latents);
-  sums.stage(rel, a, root_hd, dynamic);
+  sums.stage(biases, rel, a, root_hd, dynamic);
   const int64_t n_chunks = (L + kTile - 1) / kTile;
   if (!kSplit) stage(held[0], 0);
   if (kColumns) stage(held[kColumns != 0], 1);
@@ -583,6 +588,8 @@ relative_bwd_kv_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int3
   const Item item = item_of(n_pa, heads, n_tiles);
   if (item.pa >= n_pa) return;
   const int64_t pa = item.pa, tile = item.tile, pos = pa / heads, a = pa % heads;
+  TableStage biases;
+  biases.request(rel);
   int64_t L = seq_lens[pos];
   L = L < 0 ? 0 : (L > T ? T : L);
   const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, l16 = lane % 16, g = lane / 16;
@@ -625,12 +632,13 @@ relative_bwd_kv_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int3
     };
     fetch(held[0], kSplit ? wave * kTile : 0);
     if (!kColumns) fetch(held[!kColumns], kTile);
+    biases.biases(rel, a);
     uint4 kf[G::kKs], vf[G::kKs];
     row_frags<kHalf, HD>(rows_of(k, pos, a, L), j, g, kf);
     row_frags<kHalf, HD>(rows_of(v, pos, a, L), j, g, vf);
     const Side<false, kColumns ? 8 : 4> side(rel, coords_of(rel, pos, T, j, L), j < rel.n_latents);
     const int n_latents = int(rel.n_latents);
-    sums.stage(rel, a, root_hd, dynamic);
+    sums.stage(biases, rel, a, root_hd, dynamic);
     const float c_log2 = scale * kLog2e;
     if (!kSplit) stage(held[0], 0);
     if (!kColumns) stage(held[!kColumns], 1);

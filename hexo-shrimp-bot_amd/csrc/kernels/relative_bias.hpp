@@ -59,41 +59,54 @@ __device__ __forceinline__ float raw_bias(float b, float root_hd) {
 
 // The head's table, staged by the workgroup: store(i, bias, bucket) for entry
 // i < nq nr + 2 (entries nq nr and nq nr + 1 are the latents'; a bucket that is
-// none has bias 0 and the number n_buckets).  Four buckets of a thread are
-// requested before their biases, those before the first store: entry by entry
-// the two dependent loads would chain.
-template <typename Store>
-__device__ __forceinline__ void stage_table(const Relative& rel, int64_t head, float root_hd, Store store) {
-  constexpr int kMany = 4;
-  const int n = rel.nq * rel.nr;
-  const float* bias = rel.bias + head * rel.n_buckets;
-  for (int base = 0; base < n + 2; base += 256 * kMany) {
-    int b[kMany];
-    float x[kMany];
+// none has bias 0 and the number n_buckets).  A bias is a load that depends on
+// another one: the first kMany buckets of a thread are requested as a kernel
+// begins, their biases once its rows are on their way.
+struct TableStage {
+  static constexpr int kMany = 4;
+  int b[kMany];
+  float x[kMany];
+  __device__ __forceinline__ void request(const Relative& rel, int base = 0) {
+    const int n = rel.nq * rel.nr;
 #pragma unroll
     for (int u = 0; u < kMany; ++u) {
       const int i = base + 256 * u + int(threadIdx.x);
       b[u] = rel.buckets[i < n ? i : 0];
-      if (i >= n) b[u] = rel.n_buckets - (i == n ? 2 : 1);
     }
-#pragma unroll
-    for (int u = 0; u < kMany; ++u) {
-      const bool good = b[u] >= 0 && b[u] < rel.n_buckets;
-      if (!good && base + 256 * u + int(threadIdx.x) < n) raise_flag(rel.flag, MANTIS_FLAG_INDEX);
-      b[u] = good ? b[u] : rel.n_buckets;
-      x[u] = bias[good ? b[u] : 0];
-      x[u] = good ? raw_bias(x[u], root_hd) : 0.f;
-    }
+  }
+  __device__ __forceinline__ void biases(const Relative& rel, int64_t head, int base = 0) {
+    const int n = rel.nq * rel.nr;
+    const float* bias = rel.bias + head * rel.n_buckets;
 #pragma unroll
     for (int u = 0; u < kMany; ++u) {
       const int i = base + 256 * u + int(threadIdx.x);
-      if (i < n + 2) store(i, x[u], b[u]);
+      if (i >= n) b[u] = rel.n_buckets - (i == n ? 2 : 1);
+      const bool good = b[u] >= 0 && b[u] < rel.n_buckets;
+      if (!good && i < n) raise_flag(rel.flag, MANTIS_FLAG_INDEX);
+      b[u] = good ? b[u] : rel.n_buckets;
+      x[u] = bias[good ? b[u] : 0];
     }
   }
-}
-__device__ __forceinline__ void stage_bias(const Relative& rel, int64_t head, float root_hd, float* table) {
-  stage_table(rel, head, root_hd, [&](int i, float x, int) { table[i] = x; });
-}
+  template <typename Store>
+  __device__ __forceinline__ void store(const Relative& rel, float root_hd, Store put, int base = 0) const {
+    const int n = rel.nq * rel.nr;
+#pragma unroll
+    for (int u = 0; u < kMany; ++u) {
+      const int i = base + 256 * u + int(threadIdx.x);
+      if (i < n + 2) put(i, b[u] < rel.n_buckets ? raw_bias(x[u], root_hd) : 0.f, b[u]);
+    }
+  }
+  // after request and biases: the whole table
+  template <typename Store>
+  __device__ __forceinline__ void finish(const Relative& rel, int64_t head, float root_hd, Store put) {
+    store(rel, root_hd, put);
+    for (int base = 256 * kMany; base < rel.nq * rel.nr + 2; base += 256 * kMany) {
+      request(rel, base);
+      biases(rel, head, base);
+      store(rel, root_hd, put, base);
+    }
+  }
+};
 
 // This lane's side of its pairs: the byte offset of the table entry (kEntry
 // bytes each) of a pair with the other side's packed coordinates (kQuery: this
