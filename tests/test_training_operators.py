@@ -886,3 +886,73 @@ def test_a_captured_step_replays_with_another_mask(device):
         elif replay == 2:
             assert not torch.equal(first[0], held[0])  # another step, another mask
     ops.raise_on_device_error(device)
+
+
+@gpu
+def test_calls_on_two_streams_and_graphs_side_by_side(device):
+    # long rows of one position (tiles of 16 rows), a sliced run: the calls with workspaces
+    cases = [relative_case([300, 257], 2, 32, BF, s, device=device) for s in (1, 2)]
+    logits = [torch.randn(2 * 30000, generator=_gen(s)).to(device) for s in (3, 4)]
+    offsets = torch.tensor([0, 30000, 60000], device=device)
+    moves = torch.tensor([[7, 29999], [0, -1]], device=device)
+
+    def step(i):
+        leaf = logits[i].detach().requires_grad_(True)
+        log_probs, entropy, lse, top, _moves, _norm = OPS.policy_log_probs(leaf, offsets, moves, 5)
+        (grad,) = torch.autograd.grad(log_probs.sum() + entropy.sum() + top.sum(), leaf)
+        return [*_run_relative(cases[i]).values(), log_probs.detach(), lse.detach(), grad]
+
+    want = [step(0), step(1)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(3):
+        got = []
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got.append(step(i))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for g, w in zip(got, want) for a, b in zip(g, w))
+    graphs, held = [], []
+    for i in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[i]):
+            held.append(step(i))
+    for _ in range(3):
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for h, w in zip(held, want) for a, b in zip(h, w))
+    ops.raise_on_device_error(device)
+
+
+@gpu
+def test_relative_attention_positions_further_apart_than_32_bits(device):
+    q, k, v, bias, coords, buckets, lens, n_latents, grad = relative_case([20, 17], 2, 16, BF, 12, device=device)
+    apart = 2**31 + 8  # elements: more than 2^32 bytes
+    far = torch.empty(apart + q[0].numel(), dtype=BF, device=device).as_strided(q.shape, (apart, *q.stride()[1:]))
+    far.copy_(q)
+    got = _run_relative((q, k, v, bias, coords, buckets, lens, n_latents, grad))
+    for at in range(3):
+        ops3 = [q, k, v]
+        ops3[at] = far.copy_(ops3[at])
+        out, lse, stats = OPS.fused_attention_relative(*ops3, bias, coords, buckets, lens, n_latents)
+        dq, dk, dv, dbias = OPS.fused_attention_relative_backward(*ops3, bias, coords, buckets, lens, n_latents, stats,
+                                                                  grad)
+        for name, x in zip(("out", "lse", "dq", "dk", "dv", "dbias"), (out, lse, dq, dk, dv, dbias)):
+            assert torch.equal(x, got[name]), (at, name)
+
+
+@gpu
+def test_backwards_are_not_differentiable(device):
+    q, k, v, bias, coords, buckets, lens, n_latents, grad = relative_case([9], 1, 16, BF, 13, device=device)
+    leaf = q.clone().requires_grad_(True)
+    out, _, _ = OPS.fused_attention_relative(leaf, k, v, bias, coords, buckets, lens, n_latents)
+    x = torch.randn(6, device=device, requires_grad=True)
+    log_probs = OPS.policy_log_probs(x, torch.tensor([0, 6], device=device), torch.tensor([[2]], device=device), 0)[0]
+    y = OPS.residual_dropout(x, None, torch.tensor([1, 2], device=device), 0.5, 0)
+    for result, wrt in ((out, leaf), (log_probs, x), (y, x)):
+        weight = torch.ones_like(result, requires_grad=True)
+        (first,) = torch.autograd.grad(result, wrt, weight, create_graph=True)
+        with pytest.raises(RuntimeError, match="not implemented"):
+            first.sum().backward()
