@@ -482,6 +482,26 @@ def test_relative_attention(device, lens, heads, d, dtype, kw):
 
 
 @gpu
+@pytest.mark.parametrize("d", [16, 32, 64])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_relative_attention_reference_point_is_a_score(device, dtype, d):
+    # the sum of exp2(c (s - m)) holds the term of m itself, an exact 1, where m is one of the row's
+    # scores: its log2 is never below 0; the biases here lie far from the scores
+    lens = [*range(1, 68), 80, 81, 112, 113, 128]
+    for p, extra in ((1, 0), (len(lens), 0), (len(lens), 13)):
+        q, k, v, bias, coords, buckets, sl, n_latents, _grad = relative_case(lens[:p] if p > 1 else [1], 4, d, dtype, 31,
+                                                                            device=device, extra=extra)
+        case = (2.0 * q, 2.0 * k, v, 4.0 * bias, coords, buckets, sl, n_latents)
+        runs = [OPS.fused_attention_relative(*case) for _ in range(4)]
+        live = torch.arange(q.shape[2], device=device)[None, None] < sl[:, None, None]
+        for out, lse, stats in runs:
+            assert bool((stats[..., 1] >= 0)[live.expand(stats.shape[:3])].all())
+            assert all(torch.equal(a, b) for a, b in zip((out, lse, stats), runs[0]))
+        one = runs[0][2][sl == 1][:, :, 0]
+        assert bool((one[..., 1] == 0).all())
+
+
+@gpu
 def test_relative_attention_far_coordinates_and_extents(device):
     # clamped displacements past the table, the coordinates' corners (a difference past int16 saturates)
     case = list(relative_case([50, 50], 2, 32, BF, 3, n_latents=0, table=(9, 5), device=device))
