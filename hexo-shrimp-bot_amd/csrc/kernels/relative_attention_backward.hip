@@ -204,19 +204,24 @@ struct ColumnScale {
   }
 };
 
-// four adds of a lane to its own LDS words, all read before the first is
-// written: words named twice take the sum so far
-__device__ __forceinline__ void add4(char* base, const int (&at)[4], const float (&x)[4]) {
+// Four adds of a lane to its own LDS words, all read before the first is
+// written: words named twice take the sum so far (merge4, before the reads'
+// answer where it can be: one set of comparisons serves every turn).
+__device__ __forceinline__ void merge4(const int (&at)[4], float (&x)[4]) {
+  const float x1 = x[1] + (at[1] == at[0] ? x[0] : 0.f);
+  const float x2 = x[2] + (at[2] == at[1] ? x1 : at[2] == at[0] ? x[0] : 0.f);
+  x[3] += at[3] == at[2] ? x2 : at[3] == at[1] ? x1 : at[3] == at[0] ? x[0] : 0.f;
+  x[1] = x1;
+  x[2] = x2;
+}
+template <bool kMerged>
+__device__ __forceinline__ void add4(char* base, const int (&at)[4], float (&x)[4]) {
   float old[4];
 #pragma unroll
   for (int t = 0; t < 4; ++t) old[t] = *reinterpret_cast<const float*>(base + at[t]);
-  const float x1 = x[1] + (at[1] == at[0] ? x[0] : 0.f);
-  const float x2 = x[2] + (at[2] == at[1] ? x1 : at[2] == at[0] ? x[0] : 0.f);
-  const float x3 = x[3] + (at[3] == at[2] ? x2 : at[3] == at[1] ? x1 : at[3] == at[0] ? x[0] : 0.f);
-  *reinterpret_cast<float*>(base + at[0]) = old[0] + x[0];
-  *reinterpret_cast<float*>(base + at[1]) = old[1] + x1;
-  *reinterpret_cast<float*>(base + at[2]) = old[2] + x2;
-  *reinterpret_cast<float*>(base + at[3]) = old[3] + x3;
+  if (!kMerged) merge4(at, x);
+#pragma unroll
+  for (int t = 0; t < 4; ++t) *reinterpret_cast<float*>(base + at[t]) = old[t] + x[t];
 }
 
 // The workgroup's bucket sums: kColumns columns per wavefront of n_buckets + 1
@@ -255,11 +260,12 @@ struct BucketSums {
 #pragma unroll
     for (int t = 0; t < 4; ++t) x[t] = kColumns < 16 && !live ? 0.f : ds[t];  // (two rows share a column of eight)
     if constexpr (kColumns == 64) {
-      add4(own, to, x);
+      add4<false>(own, to, x);
     } else {
+      merge4(to, x);
 #pragma unroll
       for (int turn = 0; turn < 64 / kColumns; ++turn) {
-        if (int(threadIdx.x) % 64 / kColumns == turn) add4(own, to, x);
+        if (int(threadIdx.x) % 64 / kColumns == turn) add4<true>(own, to, x);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (the next group reads what this one wrote)
       }
     }
