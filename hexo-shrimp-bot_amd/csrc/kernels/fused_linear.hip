@@ -434,6 +434,9 @@ __global__ void __launch_bounds__((threads_for<N1, kX2, kStage2>())) fused_linea
         else r = *reinterpret_cast<const float4*>(a.add2 + (grp >= 0 ? grp : 0) * N1 + f);
         if (grp >= 0) add.x += r.x, add.y += r.y, add.z += r.z, add.w += r.w;
       }
+      // (the branches above, taken, can leave five of the eight wait states between the last
+      // product and its first reader, and the compiler's count misses that way)
+      asm volatile("s_nop 2" : "+v"(acc));
       acc[0] += add.x, acc[1] += add.y, acc[2] += add.z, acc[3] += add.w;
       if constexpr (kRelu)
 #pragma unroll
