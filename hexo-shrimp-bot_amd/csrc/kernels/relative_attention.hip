@@ -26,7 +26,7 @@
 // some 20 instructions for each, against 4 hd matrix operations), not by memory.
 // Measured: 512 positions of 44-124 rows, 4 heads, 32 dims, 27 us (q, k, v and out
 // at the rate of a large copy: 10); 192 of them 14.6; 16 of 511-1,021 rows, 8 heads
-// of 16 dims, 58; two lines of 2,049-4,096 rows, 8 heads of 64 dims, 134.
+// of 16 dims, 58; two lines of 2,049-4,096 rows, 8 heads of 64 dims, 131.
 #include <type_traits>
 
 #include "attention_rows.hpp"

@@ -42,9 +42,9 @@
 // Bound by the pairs' vector and LDS work, not by memory or the matrix units: a
 // pair takes two products to recompute p and dp, exp2, the split into parts and,
 // in the pass with the bucket sums, two LDS accesses more.  Measured, query pass
-// + key pass: 192 positions of 44-124 rows, 4 heads, 32 dims, 24.7 + 20.2 us; 16 of
-// 511-1,021 rows, 8 heads of 16 dims, 91 + 159; two lines of 2,049-4,096 rows, 8
-// heads of 64 dims, 245 + 333 (their products alone at the rate of a large matrix product: 118).
+// + key pass: 192 positions of 44-124 rows, 4 heads, 32 dims, 24 + 20 us; 16 of
+// 511-1,021 rows, 8 heads of 16 dims, 91 + 157; two lines of 2,049-4,096 rows, 8
+// heads of 64 dims, 244 + 329 (their products alone at the rate of a large matrix product: 118).
 #include <type_traits>
 
 #include "attention_rows.hpp"
