@@ -19,7 +19,9 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
+#include <array>
 #include <mutex>
+#include <utility>
 
 #include "../../../include/mantis_hip.h"
 
@@ -135,14 +137,37 @@ HeadRows head_rows(const Tensor& t) {
   return r;
 }
 
-// an empty operand in t's layout, or contiguous where t has gaps or that layout's rows are not the kernels'
-HeadRows head_rows_like(const Tensor& t) {
-  HeadRows r;
-  if (t.is_non_overlapping_and_dense()) {
-    r.t = at::empty_strided(t.sizes(), t.strides(), t.options());
-    if (row_strides(r.t, r.strides)) return r;
+// An empty result beside the operand t (P, A, T, D), kernels and fakes alike: whole rows in the
+// order that t's own lie in memory (heads inside rows for a projection's view, packed or not),
+// without its gaps; contiguous where t has no such order (a repeated dimension, D not innermost)
+// or the kernels do not take its rows.
+Tensor empty_rows_like(const Tensor& t) {
+  const auto n = t.sym_sizes(), s = t.sym_strides();
+  std::array<c10::SymInt, 4> strides{n[1] * n[2] * n[3], n[2] * n[3], n[3], 1};
+  // outermost first; a dimension of one entry has no place of its own and stands before the others
+  std::array<int, 3> order{0, 1, 2};
+  const auto before = [&](int a, int b) {
+    if (n[a] == 1 || n[b] == 1) return n[a] == 1 && n[b] != 1;
+    return s[a] > s[b];
+  };
+  for (int i = 1; i < 3; ++i)
+    for (int j = i; j > 0 && before(order[j], order[j - 1]); --j) std::swap(order[j], order[j - 1]);
+  bool ordered = s[3] == 1;
+  for (int i = 0; i < 3 && ordered; ++i) ordered = n[i] == 1 || s[i] != 0;
+  if (ordered) {
+    std::array<c10::SymInt, 4> own = strides;
+    c10::SymInt step = n[3];
+    for (int i = 2; i >= 0; --i) {
+      own[order[i]] = step;
+      step = step * n[order[i]];
+    }
+    if (n[2] == 1 || (own[2] < 8192 && n[2] * own[2] * 2 <= 0x7FFFFFFF)) strides = own;
   }
-  r.t = at::empty(t.sizes(), t.options());
+  return at::empty_strided_symint(n, strides, t.options());
+}
+
+HeadRows head_rows_like(const Tensor& t) {
+  HeadRows r{empty_rows_like(t)};
   row_strides(r.t, r.strides);
   return r;
 }
@@ -188,7 +213,7 @@ Three relative_meta(const Tensor& q, const Tensor& k, const Tensor& v, const Ten
                     const Tensor& buckets, const Tensor& seq_lens, int64_t n_latents) {
   check_relative(q, k, v, bias, coords, buckets, seq_lens, n_latents);
   const auto f32 = q.options().dtype(at::kFloat);
-  return {at::empty_like(q), at::empty({q.size(0), q.size(1), q.size(2)}, f32),
+  return {empty_rows_like(q), at::empty({q.size(0), q.size(1), q.size(2)}, f32),
           at::empty({q.size(0), q.size(1), q.size(2), 2}, f32)};
 }
 
@@ -227,7 +252,7 @@ Four relative_backward_meta(const Tensor& q, const Tensor& k, const Tensor& v, c
                             const Tensor& stats, const Tensor& grad_out) {
   check_relative(q, k, v, bias, coords, buckets, seq_lens, n_latents);
   check_relative_backward(q, stats, grad_out);
-  return {at::empty_like(q), at::empty_like(k), at::empty_like(v), at::empty(bias.sizes(), bias.options())};
+  return {empty_rows_like(q), empty_rows_like(k), empty_rows_like(v), at::empty(bias.sizes(), bias.options())};
 }
 
 Four relative_backward(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& bias_,

@@ -1808,8 +1808,9 @@ def relative_attention(q: Tensor, k: Tensor, v: Tensor, bias: Tensor, coords: Te
     (P, A, T, hd) fp16 or bf16, bias (A, buckets), coords (P, T, 2) int32 as
     ``Batch.coords`` holds them, buckets the displacement's bucket
     (``tables.relative_buckets``), the first n_latents rows without
-    coordinates.  out has q's layout; lse (P, A, T) and stats (P, A, T, 2)
-    fp32, stats for the backward.  Differentiable in q, k, v and bias."""
+    coordinates.  out is dense, its rows in q's order in memory (contiguous
+    where q has none); lse (P, A, T) and stats (P, A, T, 2) fp32, stats for the
+    backward.  Differentiable in q, k, v and bias."""
     p, heads, t, hd = q.shape if q.ndim == 4 else (0, 0, 0, 0)
     nbytes = p * t * heads * (4 * hd * q.element_size() + 12)
     return _launch("relative_attention", nbytes, 0.0, lambda: torch.ops.mantisnet.fused_attention_relative(
@@ -1820,7 +1821,7 @@ def relative_attention_backward(q: Tensor, k: Tensor, v: Tensor, bias: Tensor, c
                                 seq_lens: Tensor, n_latents: int, stats: Tensor,
                                 grad_out: Tensor) -> tuple[Tensor, Tensor, Tensor, Tensor]:
     """(dq, dk, dv, dbias) of relative_attention, given its stats: dq, dk and dv
-    in q's dtype and their operand's layout, dbias in bias's dtype."""
+    in q's dtype and their operand's order in memory, dense; dbias in bias's dtype."""
     p, heads, t, hd = q.shape if q.ndim == 4 else (0, 0, 0, 0)
     nbytes = p * t * heads * (7 * hd * q.element_size() + 8)
     return _launch("relative_attention_backward", nbytes, 0.0,

@@ -1,0 +1,130 @@
+"""Edges of the training operators: layouts and traces of their results, infinite
+and cancelling gradients, broken index tables, the library's absence.
+
+The formulas in float64 and the tolerances are those of
+``test_training_operators.py`` unless a test states its own.
+"""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from tests import test_training_operators as base
+
+OPS, INF, BF, HF = base.OPS, base.INF, base.BF, base.HF
+gpu = base.gpu
+
+
+# ----------------------------------------------------------------- layouts of results
+
+
+def _layouts(p, a, t, d, new):
+    """Operands (P, A, T, D) as programs hold them, and the order (outermost first) of their results' memory."""
+    rows, heads = (0, 2, 1, 3), (0, 1, 2, 3)
+    return {
+        "contiguous": (new(p, a, t, d), heads),
+        "projection": (new(p, t, a, d).transpose(1, 2), rows),
+        "packed": (new(p, t, 3, a, d)[:, :, 1].transpose(1, 2), rows),
+        "packed first": (new(3, p, t, a, d)[2].transpose(1, 2), rows),
+        "sliced": (new(p, a, t, 2 * d)[..., :d], heads),
+        "every other row": (new(p, 2 * t, a, d)[:, ::2].transpose(1, 2), rows),
+        "heads outermost": (new(a, t + 3, p, d)[:, 3:].permute(2, 0, 1, 3), (1, 2, 0, 3)),
+        "shared head": (new(p, 1, t, d).expand(p, a, t, d), heads),
+        "shared position": (new(1, t, a, d).transpose(1, 2).expand(p, a, t, d), heads if p > 1 else rows),
+        "not innermost": (new(p, a, d, t).transpose(2, 3), heads),
+        "far rows": (new(p, t, 8200).as_strided((p, a, t, d), (t * 8200, d, 8200, 1)), rows),
+    }
+
+
+def _dense(shape, order):
+    strides, step = [0] * 4, 1
+    for i in reversed(order):
+        strides[i] = step
+        step *= shape[i]
+    return tuple(strides)
+
+
+def _relative_on(q, new, i32):
+    p, a, t, _ = q.shape
+    return (q, q, q, new(a, 12), i32(p, t, 2), i32(5, 7), i32(p), min(4, t))
+
+
+def test_fake_results_lie_in_their_operands_order():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        half = lambda *s: torch.empty(s, dtype=BF, device="cuda")  # noqa: E731
+        new = lambda *s: torch.empty(s, device="cuda")  # noqa: E731
+        i32 = lambda *s: torch.empty(s, dtype=torch.int32, device="cuda")  # noqa: E731
+        for shape in ((2, 4, 64, 32), (3, 2, 1, 16), (1, 4, 9, 64), (5, 1, 7, 16)):
+            for name, (q, order) in _layouts(*shape, half).items():
+                out, lse, stats = OPS.fused_attention_relative(*_relative_on(q, new, i32))
+                want = _dense(shape, order)
+                for x in (out, *OPS.fused_attention_relative_backward(*_relative_on(q, new, i32), stats, q)[:3]):
+                    assert x.shape == shape
+                    assert all(n == 1 or s == w for n, s, w in zip(shape, x.stride(), want)), (name, shape, x.stride())
+                assert lse.is_contiguous() and stats.is_contiguous()
+        # 256 heads of 64 in a row: past the kernels' pitch
+        wide, _ = _layouts(2, 256, 5, 64, half)["projection"]
+        assert OPS.fused_attention_relative(*_relative_on(wide, new, i32))[0].is_contiguous()
+
+
+def _fakes_of(mode, xs):
+    return [mode.from_tensor(x) if isinstance(x, torch.Tensor) else x for x in xs]
+
+
+@gpu
+def test_results_lie_where_their_fakes_say(device):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    def agree(op, *args):
+        res = op(*args)
+        mode = FakeTensorMode()
+        with mode:
+            fake = op(*_fakes_of(mode, args))
+        for r, f in zip(res if isinstance(res, tuple) else [res], fake if isinstance(fake, tuple) else [fake]):
+            assert (r.shape, r.stride(), r.dtype, r.device) == (f.shape, f.stride(), f.dtype, f.device), op
+        return res
+
+    for shape in ((2, 4, 64, 32), (3, 2, 1, 16), (1, 2, 200, 64)):
+        p, a, t, _ = shape
+        _q, _k, _v, bias, coords, buckets, _l, _n, _g = base.relative_case([t] * p, a, shape[3], BF, 3, device=device)
+        lens = torch.randint(0, t + 1, (p,), dtype=torch.int32, device=device)
+        half = lambda *s: torch.randn(s, device=device).to(BF)  # noqa: E731
+        for q, _order in _layouts(*shape, half).values():
+            args = (q, q, q, bias, coords, buckets, lens, min(4, t))
+            out, _lse, stats = agree(OPS.fused_attention_relative, *args)
+            grads = agree(OPS.fused_attention_relative_backward, *args, stats, out)
+            plain = tuple(x.contiguous() if isinstance(x, torch.Tensor) else x for x in args)
+            assert torch.equal(out, OPS.fused_attention_relative(*plain)[0])
+            for x, y in zip(grads, OPS.fused_attention_relative_backward(*plain, stats, out.contiguous())):
+                assert torch.equal(x, y)
+    x, off, mv, top, grads = base.policy_case([50, 333], BF, 12, device, top=6)
+    for logits in (x, torch.stack([x, x], 1)[:, 1], x[:1].expand(x.numel())):
+        res = agree(OPS.policy_log_probs, logits, off, mv, top)
+        agree(OPS.policy_log_probs_backward, logits, off, mv, res[4], res[1], res[5], *grads)
+    rng = torch.tensor([3, 4], device=device)
+    for y in (torch.randn(6, 10, device=device), torch.randn(10, 6, device=device).t()):
+        out = agree(OPS.residual_dropout, y, y.half(), rng, 0.1, 2)
+        agree(OPS.residual_dropout_backward, out, rng, 0.1, 2, BF)
+
+
+@gpu
+def test_a_traced_step_over_packed_rows(device):
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    params, x, extra = base._block_case(device)
+    leaves = [w.clone().requires_grad_(True) for w in params.values()]
+
+    def step(*leaves):
+        loss = base._block(dict(zip(params, leaves)), x, extra)
+        return loss, *torch.autograd.grad(loss, leaves)
+
+    want = step(*leaves)
+    traced = make_fx(step, tracing_mode="fake", _allow_non_fake_inputs=True)(*leaves)
+    got = traced(*[w.detach() for w in leaves])
+    for name, g, w in zip(("loss", *params), got, want):
+        assert torch.equal(g.detach(), w.detach()), name
