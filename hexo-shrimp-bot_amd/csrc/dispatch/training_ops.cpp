@@ -175,28 +175,29 @@ HeadRows head_rows_like(const Tensor& t) {
 // (a conversion that is none costs a dispatch)
 Tensor as(const Tensor& t, at::ScalarType dtype) { return t.scalar_type() == dtype ? t : t.to(dtype); }
 
+// (sizes as symbols here and in the fakes, which see them where a trace leaves them open)
 void check_relative(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& bias, const Tensor& coords,
                     const Tensor& buckets, const Tensor& seq_lens, int64_t n_latents) {
-  TORCH_CHECK_VALUE(q.dim() == 4 && k.sizes() == q.sizes() && v.sizes() == q.sizes(),
+  TORCH_CHECK_VALUE(q.dim() == 4 && k.sym_sizes() == q.sym_sizes() && v.sym_sizes() == q.sym_sizes(),
                     "q, k and v must have the same (P, A, T, D) shape");
-  const int64_t p = q.size(0), heads = q.size(1), t = q.size(2), hd = q.size(3);
+  const auto p = q.sym_size(0), heads = q.sym_size(1), t = q.sym_size(2), hd = q.sym_size(3);
   TORCH_CHECK_VALUE((q.scalar_type() == at::kHalf || q.scalar_type() == at::kBFloat16) &&
                         k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(),
                     "relative attention runs 16-bit MFMA: q, k and v must share float16 or bfloat16");
   TORCH_CHECK_VALUE(hd == 16 || hd == 32 || hd == 64, "relative attention supports head_dim 16, 32 and 64");
-  TORCH_CHECK_VALUE(seq_lens.dim() == 1 && seq_lens.size(0) == p && seq_lens.scalar_type() == at::kInt,
+  TORCH_CHECK_VALUE(seq_lens.dim() == 1 && seq_lens.sym_size(0) == p && seq_lens.scalar_type() == at::kInt,
                     "seq_lens must be int32 with shape (P,)");
-  TORCH_CHECK_VALUE(bias.dim() == 2 && bias.size(0) == heads && bias.is_floating_point(),
+  TORCH_CHECK_VALUE(bias.dim() == 2 && bias.sym_size(0) == heads && bias.is_floating_point(),
                     "bias must be floating point with shape (heads, buckets)");
-  TORCH_CHECK_VALUE(bias.size(1) >= 1 && bias.size(1) <= 384, "bias must hold 1 to 384 buckets");
-  TORCH_CHECK_VALUE(coords.dim() == 3 && coords.size(0) == p && coords.size(1) == t && coords.size(2) == 2 &&
+  TORCH_CHECK_VALUE(bias.sym_size(1) >= 1 && bias.sym_size(1) <= 384, "bias must hold 1 to 384 buckets");
+  TORCH_CHECK_VALUE(coords.dim() == 3 && coords.sym_size(0) == p && coords.sym_size(1) == t && coords.sym_size(2) == 2 &&
                         coords.scalar_type() == at::kInt,
                     "coords must be int32 with shape (P, T, 2)");
-  TORCH_CHECK_VALUE(buckets.dim() == 2 && buckets.scalar_type() == at::kInt && buckets.size(0) % 2 == 1 &&
-                        buckets.size(1) % 2 == 1,
+  TORCH_CHECK_VALUE(buckets.dim() == 2 && buckets.scalar_type() == at::kInt && buckets.sym_size(0) % 2 == 1 &&
+                        buckets.sym_size(1) % 2 == 1,
                     "buckets must be int32 with an odd number of rows and of columns");
-  TORCH_CHECK_VALUE(buckets.numel() <= 4096, "buckets must hold at most 4096 displacements");
-  TORCH_CHECK_VALUE(n_latents >= 0 && n_latents <= t && (n_latents == 0 || bias.size(1) >= 2),
+  TORCH_CHECK_VALUE(buckets.sym_numel() <= 4096, "buckets must hold at most 4096 displacements");
+  TORCH_CHECK_VALUE(n_latents >= 0 && n_latents <= t && (n_latents == 0 || bias.sym_size(1) >= 2),
                     "n_latents must lie in [0, T], with two buckets of their own");
 }
 
@@ -213,8 +214,8 @@ Three relative_meta(const Tensor& q, const Tensor& k, const Tensor& v, const Ten
                     const Tensor& buckets, const Tensor& seq_lens, int64_t n_latents) {
   check_relative(q, k, v, bias, coords, buckets, seq_lens, n_latents);
   const auto f32 = q.options().dtype(at::kFloat);
-  return {empty_rows_like(q), at::empty({q.size(0), q.size(1), q.size(2)}, f32),
-          at::empty({q.size(0), q.size(1), q.size(2), 2}, f32)};
+  const auto n = q.sym_sizes();
+  return {empty_rows_like(q), at::empty_symint({n[0], n[1], n[2]}, f32), at::empty_symint({n[0], n[1], n[2], 2}, f32)};
 }
 
 Three relative(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& bias_, const Tensor& coords_,
@@ -241,9 +242,9 @@ Three relative(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tenso
 }
 
 void check_relative_backward(const Tensor& q, const Tensor& stats, const Tensor& grad_out) {
-  TORCH_CHECK_VALUE(grad_out.sizes() == q.sizes(), "grad_out must have q's shape");
-  TORCH_CHECK_VALUE(stats.dim() == 4 && stats.size(0) == q.size(0) && stats.size(1) == q.size(1) &&
-                        stats.size(2) == q.size(2) && stats.size(3) == 2 && stats.scalar_type() == at::kFloat,
+  TORCH_CHECK_VALUE(grad_out.sym_sizes() == q.sym_sizes(), "grad_out must have q's shape");
+  TORCH_CHECK_VALUE(stats.dim() == 4 && stats.sym_size(0) == q.sym_size(0) && stats.sym_size(1) == q.sym_size(1) &&
+                        stats.sym_size(2) == q.sym_size(2) && stats.sym_size(3) == 2 && stats.scalar_type() == at::kFloat,
                     "stats must be the forward's (P, A, T, 2) fp32 statistics");
 }
 
@@ -252,7 +253,7 @@ Four relative_backward_meta(const Tensor& q, const Tensor& k, const Tensor& v, c
                             const Tensor& stats, const Tensor& grad_out) {
   check_relative(q, k, v, bias, coords, buckets, seq_lens, n_latents);
   check_relative_backward(q, stats, grad_out);
-  return {empty_rows_like(q), empty_rows_like(k), empty_rows_like(v), at::empty(bias.sizes(), bias.options())};
+  return {empty_rows_like(q), empty_rows_like(k), empty_rows_like(v), at::empty_symint(bias.sym_sizes(), bias.options())};
 }
 
 Four relative_backward(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& bias_,
@@ -285,33 +286,36 @@ Four relative_backward(const Tensor& q_, const Tensor& k_, const Tensor& v_, con
 
 // ------------------------------------------------------------- policy
 
+void check_policy(const Tensor& logits, const Tensor& offsets, const Tensor& moves, int64_t top) {
+  TORCH_CHECK_VALUE(logits.dim() == 1, "logits must be flat (N,)");
+  dtype_of(logits.scalar_type());
+  TORCH_CHECK_VALUE(offsets.dim() == 1 && offsets.sym_size(0) >= 1, "offsets must hold P + 1 entries");
+  TORCH_CHECK_VALUE(offsets.scalar_type() == at::kLong, "offsets must have dtype int64");
+  TORCH_CHECK_VALUE(moves.dim() == 2 && moves.sym_size(0) == offsets.sym_size(0) - 1, "moves must have shape (P, moves)");
+  TORCH_CHECK_VALUE(moves.scalar_type() == at::kLong, "moves must have dtype int64");
+  TORCH_CHECK_VALUE(moves.sym_size(1) <= 1024, "at most 1024 moves of a position");
+  TORCH_CHECK_VALUE(top >= 0 && top <= 64, "top must lie in [0, 64], got ", top);
+}
+
 struct Runs {  // the logits' stride and the index tables as the kernels take them
   Tensor logits;
   int64_t stride;
   Tensor offsets, moves;
+  Runs(const Tensor& logits_, const Tensor& offsets_, const Tensor& moves_)
+      : logits(logits_), stride(logits_.numel() > 1 ? logits_.stride(0) : 1), offsets(offsets_.contiguous()),
+        moves(moves_.contiguous()) {
+    if (stride < 1) logits = logits_.contiguous(), stride = 1;
+  }
 };
-
-Runs check_policy(const Tensor& logits, const Tensor& offsets, const Tensor& moves, int64_t top) {
-  TORCH_CHECK_VALUE(logits.dim() == 1, "logits must be flat (N,)");
-  dtype_of(logits.scalar_type());
-  TORCH_CHECK_VALUE(offsets.dim() == 1 && offsets.numel() >= 1, "offsets must hold P + 1 entries");
-  TORCH_CHECK_VALUE(offsets.scalar_type() == at::kLong, "offsets must have dtype int64");
-  TORCH_CHECK_VALUE(moves.dim() == 2 && moves.size(0) == offsets.numel() - 1, "moves must have shape (P, moves)");
-  TORCH_CHECK_VALUE(moves.scalar_type() == at::kLong, "moves must have dtype int64");
-  TORCH_CHECK_VALUE(moves.size(1) <= 1024, "at most 1024 moves of a position");
-  TORCH_CHECK_VALUE(top >= 0 && top <= 64, "top must lie in [0, 64], got ", top);
-  Runs r{logits, logits.numel() > 1 ? logits.stride(0) : 1, offsets.contiguous(), moves.contiguous()};
-  if (r.stride < 1) r.logits = logits.contiguous(), r.stride = 1;
-  return r;
-}
 
 using Six = std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor>;
 
 Six policy_outputs(const Tensor& logits, const Tensor& moves, int64_t top) {
-  const int64_t p = moves.size(0);
+  const auto p = moves.sym_size(0);
+  const c10::SymInt k = top;
   const auto f32 = logits.options().dtype(at::kFloat);
-  return {at::empty({p, moves.size(1)}, f32), at::empty({p}, f32), at::empty({p}, f32), at::empty({p, top}, f32),
-          at::empty({p, top}, moves.options()), at::empty({p, 2}, f32)};
+  return {at::empty_symint({p, moves.sym_size(1)}, f32), at::empty_symint({p}, f32), at::empty_symint({p}, f32),
+          at::empty_symint({p, k}, f32), at::empty_symint({p, k}, moves.options()), at::empty_symint({p, 2}, f32)};
 }
 
 Six policy_meta(const Tensor& logits, const Tensor& offsets, const Tensor& moves, int64_t top) {
@@ -322,7 +326,8 @@ Six policy_meta(const Tensor& logits, const Tensor& offsets, const Tensor& moves
 Six policy(const Tensor& logits, const Tensor& offsets, const Tensor& moves, int64_t top) {
   const at::Device dev = on_gpu({&logits, &offsets, &moves});
   const c10::DeviceGuard guard(dev);
-  const Runs r = check_policy(logits, offsets, moves, top);
+  check_policy(logits, offsets, moves, top);
+  const Runs r(logits, offsets, moves);
   Six res = policy_outputs(logits, moves, top);
   const int64_t p = moves.size(0), n = logits.numel();
   if (p == 0) return res;
@@ -343,34 +348,32 @@ struct PolicyGrads {
   optional<Tensor> log_probs, entropy, lse, top;
 };
 
-Runs check_policy_backward(const Tensor& logits, const Tensor& offsets, const Tensor& moves, const Tensor& top_moves,
-                           const Tensor& entropy, const Tensor& norm, PolicyGrads& g) {
+void check_policy_backward(const Tensor& logits, const Tensor& offsets, const Tensor& moves, const Tensor& top_moves,
+                           const Tensor& entropy, const Tensor& norm, const PolicyGrads& g) {
   TORCH_CHECK_VALUE(top_moves.dim() == 2 && top_moves.scalar_type() == at::kLong, "top_moves must be the forward's");
-  const int64_t p = top_moves.size(0);
-  const Runs r = check_policy(logits, offsets, moves, top_moves.size(1));
-  TORCH_CHECK_VALUE(moves.size(0) == p && entropy.dim() == 1 && entropy.size(0) == p && norm.dim() == 2 &&
-                        norm.size(0) == p && norm.size(1) == 2 && entropy.scalar_type() == at::kFloat &&
+  const auto p = top_moves.sym_size(0), k = top_moves.sym_size(1);
+  TORCH_CHECK_VALUE(k <= 64, "top_moves must be the forward's");
+  check_policy(logits, offsets, moves, 0);
+  TORCH_CHECK_VALUE(moves.sym_size(0) == p && entropy.dim() == 1 && entropy.sym_size(0) == p && norm.dim() == 2 &&
+                        norm.sym_size(0) == p && norm.sym_size(1) == 2 && entropy.scalar_type() == at::kFloat &&
                         norm.scalar_type() == at::kFloat,
                     "top_moves, entropy and norm must be the forward's");
-  auto take = [](optional<Tensor>& grad, at::IntArrayRef shape, const char* name) {
-    if (!grad || !grad->defined()) return;
-    TORCH_CHECK_VALUE(grad->sizes() == shape, "the gradient of ", name, " must have shape ", shape);
-    grad = as(*grad, at::kFloat).contiguous();
+  const auto check = [](const optional<Tensor>& grad, c10::SymIntArrayRef shape, const char* name) {
+    TORCH_CHECK_VALUE(!grad || !grad->defined() || grad->sym_sizes() == shape, "the gradient of ", name,
+                      " must have shape ", shape);
   };
-  take(g.log_probs, {p, moves.size(1)}, "log_probs");
-  take(g.entropy, {p}, "entropy");
-  take(g.lse, {p}, "lse");
-  take(g.top, {p, top_moves.size(1)}, "top_log_probs");
-  return r;
+  check(g.log_probs, {p, moves.sym_size(1)}, "log_probs");
+  check(g.entropy, {p}, "entropy");
+  check(g.lse, {p}, "lse");
+  check(g.top, {p, k}, "top_log_probs");
 }
 
 Tensor policy_backward_meta(const Tensor& logits, const Tensor& offsets, const Tensor& moves, const Tensor& top_moves,
                             const Tensor& entropy, const Tensor& norm, const optional<Tensor>& g_log,
                             const optional<Tensor>& g_ent, const optional<Tensor>& g_lse,
                             const optional<Tensor>& g_top) {
-  PolicyGrads g{g_log, g_ent, g_lse, g_top};
-  check_policy_backward(logits, offsets, moves, top_moves, entropy, norm, g);
-  return at::empty(logits.sizes(), logits.options());
+  check_policy_backward(logits, offsets, moves, top_moves, entropy, norm, {g_log, g_ent, g_lse, g_top});
+  return at::empty_symint(logits.sym_sizes(), logits.options());
 }
 
 Tensor policy_backward(const Tensor& logits, const Tensor& offsets, const Tensor& moves, const Tensor& top_moves_,
@@ -381,7 +384,10 @@ Tensor policy_backward(const Tensor& logits, const Tensor& offsets, const Tensor
   const at::Device dev = on_gpu({&logits, &offsets, &moves, &top_moves_, &entropy_, &norm_, given(g_log), given(g_ent),
                                  given(g_lse), given(g_top)});
   const c10::DeviceGuard guard(dev);
-  const Runs r = check_policy_backward(logits, offsets, moves, top_moves_, entropy_, norm_, g);
+  check_policy_backward(logits, offsets, moves, top_moves_, entropy_, norm_, g);
+  for (optional<Tensor>* grad : {&g.log_probs, &g.entropy, &g.lse, &g.top})
+    if (*grad && (*grad)->defined()) *grad = as(**grad, at::kFloat).contiguous();
+  const Runs r(logits, offsets, moves);
   const int64_t p = moves.size(0), n = logits.numel();
   if (p == 0) return at::zeros({n}, logits.options());
   Tensor out = at::empty({n}, logits.options());
@@ -402,9 +408,9 @@ void check_dropout(const Tensor& x, const optional<Tensor>& residual, const Tens
   dtype_of(x.scalar_type());
   if (residual) {
     dtype_of(residual->scalar_type());
-    TORCH_CHECK_VALUE(residual->sizes() == x.sizes(), "x and residual must have one shape");
+    TORCH_CHECK_VALUE(residual->sym_sizes() == x.sym_sizes(), "x and residual must have one shape");
   }
-  TORCH_CHECK_VALUE(rng.dim() == 1 && rng.size(0) == 2 && rng.scalar_type() == at::kLong,
+  TORCH_CHECK_VALUE(rng.dim() == 1 && rng.sym_size(0) == 2 && rng.scalar_type() == at::kLong,
                     "rng must hold two int64, (seed, step)");
   TORCH_CHECK_VALUE(p >= 0.0 && p <= 1.0, "the dropout probability must lie in [0, 1], got ", p);
   TORCH_CHECK_VALUE(salt >= 0 && salt <= 0xFFFFFFFFLL, "salt must lie in [0, 2^32), got ", salt);
@@ -412,7 +418,7 @@ void check_dropout(const Tensor& x, const optional<Tensor>& residual, const Tens
 
 Tensor dropout_meta(const Tensor& x, const optional<Tensor>& residual, const Tensor& rng, double p, int64_t salt) {
   check_dropout(x, residual, rng, p, salt);
-  return at::empty(x.sizes(), (residual ? *residual : x).options());
+  return at::empty_symint(x.sym_sizes(), (residual ? *residual : x).options());
 }
 
 Tensor dropout_into(const Tensor& x_, const optional<Tensor>& residual_, const Tensor& rng_, double p, int64_t salt,
@@ -439,7 +445,7 @@ Tensor dropout(const Tensor& x, const optional<Tensor>& residual, const Tensor& 
 Tensor dropout_backward_meta(const Tensor& grad_out, const Tensor& rng, double p, int64_t salt, at::ScalarType dtype) {
   check_dropout(grad_out, std::nullopt, rng, p, salt);
   dtype_of(dtype);
-  return at::empty(grad_out.sizes(), grad_out.options().dtype(dtype));
+  return at::empty_symint(grad_out.sym_sizes(), grad_out.options().dtype(dtype));
 }
 
 Tensor dropout_backward(const Tensor& grad_out, const Tensor& rng, double p, int64_t salt, at::ScalarType dtype) {

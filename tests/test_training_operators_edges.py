@@ -128,3 +128,62 @@ def test_a_traced_step_over_packed_rows(device):
     got = traced(*[w.detach() for w in leaves])
     for name, g, w in zip(("loss", *params), got, want):
         assert torch.equal(g.detach(), w.detach()), name
+
+
+def _block_args(device, positions=6, t=61):
+    params, x, (coords, buckets, lens, rng, _offsets, _moves) = base._block_case("cpu")
+    x = torch.randn(positions, t, 128, generator=base._gen(t))
+    coords = (torch.randn(positions, t, 2, generator=base._gen(t + 1)) * 4).round().to(torch.int32)
+    lens = torch.randint(4, t + 1, (positions,), generator=base._gen(t + 2)).to(torch.int32)
+    moves = torch.randint(0, t, (positions, 2), generator=base._gen(t + 3))
+    extra = (coords, buckets, lens, rng, torch.arange(positions + 1) * t, moves)
+    leaves = [w.to(device).requires_grad_(True) for w in params.values()]
+    return list(params), leaves, x.to(device), [e.to(device) for e in extra]
+
+
+def test_a_step_traces_with_open_sizes():
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    names, leaves, x, extra = _block_args("meta")
+
+    def step(x, extra, *leaves):
+        loss = base._block(dict(zip(names, leaves)), x, extra)
+        return loss, *torch.autograd.grad(loss, leaves)
+
+    graph = make_fx(step, tracing_mode="symbolic")(x, extra, *leaves)
+    shapes = {}
+    for node in graph.graph.nodes:
+        if "mantisnet" in str(node.target):
+            val = node.meta["val"]
+            shapes[node.target._opname] = (val[0] if isinstance(val, (tuple, list)) else val).shape
+    assert set(shapes) == set(base.NAMES)
+    for name, shape in shapes.items():  # the batch and the rows stay open
+        assert not isinstance(shape[0], int), name
+    assert not isinstance(shapes["fused_attention_relative"][2], int)
+
+
+@gpu
+def test_a_compiled_step_takes_other_sizes(device):
+    names, _, _, _ = _block_args("cpu")
+
+    def loss_of(leaves, x, extra):
+        return base._block(dict(zip(names, leaves)), x, extra)
+
+    torch._dynamo.reset()
+    graphs = []
+
+    def backend(gm, example):
+        from torch._dynamo.backends.common import aot_autograd
+
+        graphs.append(gm)
+        return aot_autograd(fw_compiler=lambda g, _: g)(gm, example)
+
+    compiled = torch.compile(loss_of, backend=backend, dynamic=True, fullgraph=True)
+    for positions, t in ((6, 61), (9, 37), (5, 150)):  # (no other size is one of these: equal sizes share a symbol)
+        _, leaves, x, extra = _block_args(device, positions, t)
+        got = torch.autograd.grad(compiled(leaves, x, extra), leaves)
+        want = torch.autograd.grad(loss_of(leaves, x, extra), leaves)
+        for name, g, w in zip(names, got, want):
+            assert torch.equal(g, w), (name, positions, t)
+    assert len(graphs) == 1
+    torch._dynamo.reset()
