@@ -30,6 +30,9 @@
 // bits of that one).  What is cut is 2^-17 of a term, under the 2^-9 or 2^-12
 // that the outputs round.  (fp32 MFMAs with widened rows instead: the passes
 // 1,741 + 957 us where these parts took 619 + 337.)
+// dk and dv keep the sums of both parts apart until the end, where an infinite one is
+// the hi parts' alone (join_parts); any infinity that reaches dq is NaN by the formula.
+// (A position of 1,024 rows, 2 heads of 64 dims: backward 53.3 -> 55.9 us, wider grids the same.)
 //
 // The bias gradient: every lane adds its ds to its own column of the
 // workgroup's LDS table (a row of 64 lanes per bucket and wavefront: no two
@@ -116,11 +119,14 @@ __device__ __forceinline__ void parts(float a, float b, uint32_t& hi, uint32_t& 
   }
 }
 
-// acc (HD dims x this lane's row) += transposed rows . x for the staged rows
-// below n, x the 16 fp32 values of this lane (rows 16 tt + 4 g + t; zeros from n on)
+// hi + lo (HD dims x this lane's row) += transposed rows . x for the staged rows
+// below n, x the 16 fp32 values of this lane (rows 16 tt + 4 g + t; zeros from n on).
+// Each part has its own sum where a row or a value may be infinite (join_parts);
+// one serves as both where every such product is NaN anyhow.
 template <bool kHalf, int HD>
 __device__ __forceinline__ void accumulate_parts(const uint16_t* s, int n, int l16, int g, const f32x4_t (&x)[4],
-                                                 f32x4_t (&acc)[Geom<kHalf, HD>::kDt]) {
+                                                 f32x4_t (&acc_hi)[Geom<kHalf, HD>::kDt],
+                                                 f32x4_t (&acc_lo)[Geom<kHalf, HD>::kDt]) {
   using FR = Frag<kHalf>;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -134,10 +140,21 @@ __device__ __forceinline__ void accumulate_parts(const uint16_t* s, int n, int l
 #pragma unroll
     for (int dt = 0; dt < Geom<kHalf, HD>::kDt; ++dt) {
       const typename FR::vec a = FR::cast(transposed_frag<HD>(s, h, dt, l16, g));
-      acc[dt] = mfma16x16x32(a, bh, acc[dt]);
-      acc[dt] = mfma16x16x32(a, bl, acc[dt]);
+      acc_hi[dt] = mfma16x16x32(a, bh, acc_hi[dt]);
+      acc_lo[dt] = mfma16x16x32(a, bl, acc_lo[dt]);
     }
   }
+}
+
+// The sum of both parts; a sum that is not finite is the hi parts' alone.  An infinite row
+// meets the lo parts too, which are zero or of either sign, and an infinite value
+// has lo = inf - inf: added, they would make a NaN of an infinity.
+template <int kDt>
+__device__ __forceinline__ void join_parts(f32x4_t (&hi)[kDt], const f32x4_t (&lo)[kDt]) {
+#pragma unroll
+  for (int dt = 0; dt < kDt; ++dt)
+#pragma unroll
+    for (int t = 0; t < 4; ++t) hi[dt][t] = __builtin_isfinite(hi[dt][t]) ? hi[dt][t] + lo[dt][t] : hi[dt][t];
 }
 
 // the same for two sums of one operand, whose fragments are read once
@@ -175,9 +192,9 @@ constexpr float kPScale = kHalf ? 0x1p14f : 1.f;
 template <bool kHalf>
 struct ColumnScale {
   float s = kHalf ? 0x1p126f : 1.f;
-  // scales x, and acc when the scale moves; the four lanes of a column agree
-  template <int kDt>
-  __device__ __forceinline__ void apply(f32x4_t (&x)[4], f32x4_t (&acc)[kDt]) {
+  // scales x, and the sums when the scale moves; the four lanes of a column agree
+  template <int kDt, typename... Acc>
+  __device__ __forceinline__ void apply(f32x4_t (&x)[4], f32x4_t (&acc)[kDt], Acc&... more) {
     if constexpr (kHalf) {
       float m = 0.f;
 #pragma unroll
@@ -194,7 +211,10 @@ struct ColumnScale {
 #pragma unroll
         for (int dt = 0; dt < kDt; ++dt)
 #pragma unroll
-          for (int t = 0; t < 4; ++t) acc[dt][t] *= ratio;
+          for (int t = 0; t < 4; ++t) {
+            acc[dt][t] *= ratio;
+            ((more[dt][t] *= ratio), ...);
+          }
       }
 #pragma unroll
       for (int tt = 0; tt < 4; ++tt)
@@ -455,7 +475,7 @@ relative_bwd_q_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int32
         sums.add(at[tt], p[tt], live);
       }
       cs.apply(p, acc);
-      accumulate_parts<kHalf, HD>(sk[buf], kWhole ? kTile : n, l16, g, p, acc);
+      accumulate_parts<kHalf, HD>(sk[buf], kWhole ? kTile : n, l16, g, p, acc, acc);
     };
     if (n_chunks == 1) {
       if (working) {
@@ -601,9 +621,9 @@ relative_bwd_kv_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int3
   const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, l16 = lane % 16, g = lane / 16;
   const int64_t first = tile * kRows + (kSplit ? 0 : 16 * wave), j = first + l16;
   const bool live = j < L;
-  f32x4_t ak[G::kDt], av[G::kDt];
+  f32x4_t ak[G::kDt], av[G::kDt], ak_lo[G::kDt], av_lo[G::kDt];
 #pragma unroll
-  for (int dt = 0; dt < G::kDt; ++dt) ak[dt] = av[dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  for (int dt = 0; dt < G::kDt; ++dt) ak[dt] = av[dt] = ak_lo[dt] = av_lo[dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   ColumnScale<kHalf> cs;
   BucketSums<kColumns> sums(rel, dynamic);
   float* part_sums = kColumns ? partial_of(partial, rel, n_pa, heads, n_tiles, pos, a, tile) : nullptr;
@@ -691,9 +711,9 @@ relative_bwd_kv_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int3
 #pragma unroll
           for (int tt = 0; tt < 4; ++tt) p[tt] *= kPScale<kHalf>;
         }
-        accumulate_parts<kHalf, HD>(sg[buf], kWhole ? kTile : n, l16, g, p, av);
-        cs.apply(ds, ak);
-        accumulate_parts<kHalf, HD>(sq[buf], kWhole ? kTile : n, l16, g, ds, ak);
+        accumulate_parts<kHalf, HD>(sg[buf], kWhole ? kTile : n, l16, g, p, av, av_lo);
+        cs.apply(ds, ak, ak_lo);
+        accumulate_parts<kHalf, HD>(sq[buf], kWhole ? kTile : n, l16, g, ds, ak, ak_lo);
       }
       if (kSplit) wave_sync();
       if (!kColumns || kSplit) return;
@@ -707,6 +727,8 @@ relative_bwd_kv_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int3
     int64_t qb = kSplit ? wave * kTile : 0;
     for (; qb < last; qb += kSplit ? kBwdWaves * kTile : kTile) chunk(std::true_type{}, qb, kTile);
     if (qb == last) chunk(std::false_type{}, last, int(L - last));
+    join_parts(ak, ak_lo);
+    join_parts(av, av_lo);
     if constexpr (kSplit) {
       float x[8 * G::kDt];
 #pragma unroll

@@ -187,3 +187,31 @@ def test_a_compiled_step_takes_other_sizes(device):
             assert torch.equal(g, w), (name, positions, t)
     assert len(graphs) == 1
     torch._dynamo.reset()
+
+
+# ----------------------------------------------------------------- infinite operands
+
+
+@gpu
+@pytest.mark.parametrize("lens", [[1, 2, 3, 40, 128], [1, 2, 150], [200, 3, 1, 129] * 4])
+@pytest.mark.parametrize("d", [16, 32, 64])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_relative_attention_infinite_gradients_and_values(device, dtype, d, lens):
+    """An infinite entry gives infinities and NaNs where the formula does: an infinite incoming
+    gradient infinite dv, an infinite value infinite outputs and, where its row's signs agree, dk."""
+    q, k, v, bias, coords, buckets, sl, n_latents, grad = base.relative_case(lens, 4, d, dtype, 17, device=device)
+    for i, n in enumerate(lens):
+        grad[i, 1, n - 1, 3] = INF
+        grad[i, 2, n // 2, 5] = -INF
+        v[i, 3, n - 1, 2] = INF
+    case = (q, k, v, bias, coords, buckets, sl, n_latents, grad)
+    got = base._run_relative(case)
+    val, amp, score = base.relative_reference(*case)
+    tol = base._relative_tolerances(val, amp, score, dtype, q.shape[2], d, len(lens) * 4)
+    for name in got:
+        x, exp = got[name].detach().cpu().double(), val[name]
+        assert torch.equal(x.isnan(), exp.isnan()), name
+        assert torch.equal(x[exp.isinf()], exp[exp.isinf()]), name
+        base._within(got[name], exp, tol[name].nan_to_num(0.0), name)
+    assert (val["dv"] == INF).any() and (val["dv"] == -INF).any() and val["dk"].isinf().any()
+    assert val["out"].isinf().any() and not val["dv"][:, 0].isinf().any()
