@@ -19,16 +19,21 @@
 // times its gradient is no substitute: its rounding would stay in every ds of
 // the row and in the bias gradient's long sums).  Up to two chunks of keys (T <=
 // 128) keep p and dp in registers until delta is known.  Longer rows are met
-// once: dq = sum (p dp) k - delta sum p k, with two sums beside delta, and the
-// buckets' sums move to the key pass, which knows delta.  (A second sweep over
-// the keys instead: the two passes 511 + 285 us against 258 + 352 at two lines of 2,049-4,096 rows.)
+// once, with a reference r in delta's place, the mean of dp by the weights met so far:
+//   dq = sum p (dp - r) k - (delta - r) sum p k,
+// both sums brought to the new r after every chunk, and the buckets' sums move to the key
+// pass, which knows delta.  (A second sweep over the keys instead: the two passes 511 + 285 us
+// against 258 + 352 at two lines of 2,049-4,096 rows.  With r = 0 the passes take 3-5% less, but where
+// one key holds a row or dp has a mean of many deviations the terms cancel after
+// their cut to parts: a row with all but 5e-6 of its weight on one key lost 30% of dq.)
 //
 // Precision: scores and dp are exact products of 16-bit rows summed in fp32.
 // The probabilities and ds enter their products as two 16-bit parts, hi + lo:
 // bf16 beside bf16 rows (16 significant bits), beside fp16 rows fp16 parts of the
 // value times a power of two that follows the largest of its column (22
-// bits of that one).  What is cut is 2^-17 of a term, under the 2^-9 or 2^-12
-// that the outputs round.  (fp32 MFMAs with widened rows instead: the passes
+// bits of that one).  What is cut is 2^-17 of a term p (dp - delta) k, or p (dp - r) k, which is
+// of the same size: under the 2^-8 or 2^-11 that the outputs round unless terms of that size
+// cancel again, over keys that share a large mean.  (fp32 MFMAs with widened rows instead: the passes
 // 1,741 + 957 us where these parts took 619 + 337.)
 // dk and dv keep the sums of both parts apart until the end, where an infinite one is
 // the hi parts' alone (join_parts); any infinity that reaches dq is NaN by the formula.
@@ -224,6 +229,24 @@ struct ColumnScale {
   }
 };
 
+// A chunk's values in fp16 parts by themselves: x scaled so that the column's
+// largest lands in [2^13, 2^14), and what undoes it.
+__device__ __forceinline__ float chunk_scale(f32x4_t (&x)[4]) {
+  float m = 0.f;
+#pragma unroll
+  for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+    for (int t = 0; t < 4; ++t) m = fmaxf(m, fabsf(x[tt][t]));
+  m = max_xor32(max_xor16(m));
+  const int e = 267 - int(__float_as_uint(m) >> 23), in = e > 253 ? 253 : e;  // (12 for an infinity)
+  const float s = __uint_as_float(uint32_t(in) << 23);
+#pragma unroll
+  for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+    for (int t = 0; t < 4; ++t) x[tt][t] *= s;
+  return __uint_as_float(uint32_t(254 - in) << 23);
+}
+
 // Four adds of a lane to its own LDS words, all read before the first is
 // written: words named twice take the sum so far (merge4, before the reads'
 // answer where it can be: one set of comparisons serves every turn).
@@ -364,6 +387,7 @@ relative_bwd_q_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int32
   constexpr int kRows = kSplit ? 16 : kTile, kBufs = kSplit ? kBwdWaves : 2;
   __shared__ __attribute__((aligned(16))) uint16_t sk[kBufs][kTile * Tile::kPitch], sv[kBufs][kTile * Tile::kPitch];
   __shared__ __attribute__((aligned(16))) uint32_t sc[kBufs][kTile];
+  __shared__ float row_of[4][kSplit ? kBwdWaves : 1][16];  // r, weight, rest and sum p dp of a wavefront's rows
   extern __shared__ __attribute__((aligned(16))) char dynamic[];
   const int64_t n_tiles = (T + kRows - 1) / kRows;
   const Item item = item_of(n_pa, heads, n_tiles);
@@ -445,21 +469,30 @@ relative_bwd_q_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int32
       }
   };
   float dl = 0.f;
-  // (a chunk's terms among themselves first: fewer roundings of the long sum)
-  auto sum_delta = [&](const f32x4_t (&p)[4], const f32x4_t (&dp)[4]) {
-    float sum = 0.f;
+  // sums of p and p dp (a chunk's terms among themselves first: fewer roundings of the long sum)
+  auto sum_terms = [](const f32x4_t (&p)[4], const f32x4_t (&dp)[4], float& weight, float& sum) {
+    float w = 0.f, s = 0.f;
 #pragma unroll
     for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
-      for (int t = 0; t < 4; ++t) sum = fmaf(p[tt][t], dp[tt][t], sum);
-    dl += sum;
+      for (int t = 0; t < 4; ++t) {
+        w += p[tt][t];
+        s = fmaf(p[tt][t], dp[tt][t], s);
+      }
+    weight += w;
+    sum += s;
   };
+  auto row_sum = [](float x) { return sum_xor32(sum_xor16(x)); };
+  // A weighted mean of dp.  By the weights' own sum and not by 1: what log2 l and the exponentials
+  // round is common to a row, and where dp lies far from 0 that much of it would stay in every ds.
+  auto mean_of = [](float weight, float sum) { return weight == 0.f ? 0.f : sum / weight; };
   ColumnScale<kHalf> cs;
   f32x4_t p[4], dp[4];
   int at[4][4];
   const bool working = first < L;  // wavefront-uniform: a live row here
   const int tail = int(L - (n_chunks - 1) * kTile);  // rows of the last chunk
   if constexpr (kColumns > 0) {
+    float weight = 0.f;
     // ds (in p's place) into the buckets' sums and dq
     auto spread = [&](auto whole, int buf, int n, const int (&at)[4][4], f32x4_t (&p)[4], const f32x4_t (&dp)[4]) {
       constexpr bool kWhole = decltype(whole)::value;
@@ -480,8 +513,8 @@ relative_bwd_q_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int32
     if (n_chunks == 1) {
       if (working) {
         pairs(part, 0, 0, tail, at, p, dp);
-        sum_delta(p, dp);
-        dl = sum_xor32(sum_xor16(dl));
+        sum_terms(p, dp, weight, dl);
+        dl = mean_of(row_sum(weight), row_sum(dl));
         spread(part, 0, tail, at, p, dp);
       }
     } else {  // two
@@ -489,18 +522,28 @@ relative_bwd_q_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int32
       if (working) {
         int at1[4][4];
         pairs(full, 0, 0, kTile, at, p, dp);
-        sum_delta(p, dp);
+        sum_terms(p, dp, weight, dl);
         pairs(part, 1, 1, tail, at1, p1, dp1);
-        sum_delta(p1, dp1);
-        dl = sum_xor32(sum_xor16(dl));
+        sum_terms(p1, dp1, weight, dl);
+        dl = mean_of(row_sum(weight), row_sum(dl));
         spread(full, 0, kTile, at, p, dp);
         spread(part, 1, tail, at1, p1, dp1);
       }
     }
   } else {
-    f32x4_t plain[G::kDt];  // sum p k
+    // With r the row's mean of dp by the weights met so far: acc = sum p (dp - r) k, plain = sum p k,
+    // rest = sum p (dp - r); r moves after each chunk's sums, and acc and rest with it.
+    f32x4_t plain[G::kDt];
 #pragma unroll
     for (int dt = 0; dt < G::kDt; ++dt) plain[dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    float r = 0.f, weight = 0.f;             // of the row
+    float lane_weight = 0.f, rest = 0.f;     // of this lane's pairs
+    auto move = [&](float by) {  // r by `by`, already counted in the weights so far
+#pragma unroll
+      for (int dt = 0; dt < G::kDt; ++dt)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) acc[dt][t] = fmaf(by * (-1.f / kPScale<kHalf>), plain[dt][t], acc[dt][t]);
+    };
     auto step = [&](auto whole, int64_t c, int n) {
       const int buf = kSplit ? wave : int(c & 1);
       if (kSplit) {
@@ -510,14 +553,42 @@ relative_bwd_q_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int32
       }
       if (working) {
         pairs(whole, buf, c, n, at, p, dp);
-        sum_delta(p, dp);
+        float w = 0.f, s = 0.f;
+        sum_terms(p, dp, w, s);
+        dl += s;
+        const float chunk_weight = row_sum(w);
+        weight += chunk_weight;
+        // (any r will do, so a quick reciprocal; a row without a weight so far keeps 0)
+        const float next =
+            weight == 0.f ? 0.f : fmaf(fmaf(-r, chunk_weight, row_sum(s)), __builtin_amdgcn_rcpf(weight), r);
+        const float by = next - r;
+        r = next;
+        move(by);
+        rest = fmaf(-by, lane_weight, rest);
+        lane_weight += w;
 #pragma unroll
-        for (int tt = 0; tt < 4; ++tt) {
-          dp[tt] *= p[tt];
-          if (kHalf) p[tt] *= kPScale<kHalf>;
+        for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            dp[tt][t] = p[tt][t] * (dp[tt][t] - r);
+            rest += dp[tt][t];
+          }
+        const int rows = decltype(whole)::value ? kTile : n;
+        if constexpr (kHalf) {
+          const float undo = chunk_scale(dp);
+          f32x4_t chunk[G::kDt];
+#pragma unroll
+          for (int dt = 0; dt < G::kDt; ++dt) chunk[dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int tt = 0; tt < 4; ++tt) p[tt] *= kPScale<kHalf>;
+          accumulate_two<kHalf, HD>(sk[buf], rows, l16, g, dp, chunk, p, plain);
+#pragma unroll
+          for (int dt = 0; dt < G::kDt; ++dt)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) acc[dt][t] = fmaf(chunk[dt][t], undo, acc[dt][t]);
+        } else {
+          accumulate_two<kHalf, HD>(sk[buf], rows, l16, g, dp, acc, p, plain);
         }
-        cs.apply(dp, acc);
-        accumulate_two<kHalf, HD>(sk[buf], decltype(whole)::value ? kTile : n, l16, g, dp, acc, p, plain);
       }
       if (kSplit) {
         wave_sync();
@@ -532,30 +603,51 @@ relative_bwd_q_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int32
     int64_t c = kSplit ? wave : 0;
     for (; c + 1 < n_chunks; c += kSplit ? kBwdWaves : 1) step(full, c, kTile);
     if (c + 1 == n_chunks) step(part, c, tail);
-    dl = sum_xor32(sum_xor16(dl));
+    cs.s = 1.f;
+    rest = row_sum(rest);
+    dl = row_sum(dl);
     if constexpr (kSplit) {
+      // the wavefronts' sums brought to one r, the mean of all, and added up in their order
+      if (g == 0) {
+        row_of[0][wave][l16] = r;
+        row_of[1][wave][l16] = weight;
+        row_of[2][wave][l16] = rest;
+        row_of[3][wave][l16] = dl;
+      }
+      __syncthreads();
+      float all = 0.f, mean = 0.f;
+      dl = 0.f;
+#pragma unroll
+      for (int w = 0; w < kBwdWaves; ++w) {
+        dl += row_of[3][w][l16];
+        all += row_of[1][w][l16];
+        mean += fmaf(row_of[0][w][l16], row_of[1][w][l16], row_of[2][w][l16]);
+      }
+      mean = mean_of(all, mean);
+      move(mean - r);
       float x[8 * G::kDt + 1];
+      x[8 * G::kDt] = fmaf(r - mean, weight, rest);
 #pragma unroll
       for (int k = 0; k < 4 * G::kDt; ++k) {
-        x[k] = acc[k / 4][k % 4] / cs.s;
+        x[k] = acc[k / 4][k % 4];
         x[4 * G::kDt + k] = plain[k / 4][k % 4];
       }
-      x[8 * G::kDt] = dl;
       static_assert((kBwdWaves - 1) * sizeof(x) * 64 <= sizeof(sk), "the tiles' LDS holds them");
       join_waves(x, reinterpret_cast<float*>(sk));
       if (wave > 0) return;
-      cs.s = 1.f;
-      dl = x[8 * G::kDt];
+      r = mean;
+      weight = all;
+      rest = x[8 * G::kDt];
 #pragma unroll
       for (int k = 0; k < 4 * G::kDt; ++k) {
         acc[k / 4][k % 4] = x[k];
         plain[k / 4][k % 4] = x[4 * G::kDt + k];
       }
     }
-#pragma unroll
-    for (int dt = 0; dt < G::kDt; ++dt)
-#pragma unroll
-      for (int t = 0; t < 4; ++t) acc[dt][t] = fmaf(-dl / kPScale<kHalf> * cs.s, plain[dt][t], acc[dt][t]);
+    const float by = mean_of(weight, rest);
+    move(by);
+    // (where a dp is infinite, delta is the plain sum: r has met inf - inf)
+    dl = __builtin_isfinite(dl) ? r + by : dl;
   }
   if (i < T) {
     store_row<kHalf, HD, true>(dq.row(pos, a, i), g, acc, scale / cs.s, live);

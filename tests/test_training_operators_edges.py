@@ -215,3 +215,76 @@ def test_relative_attention_infinite_gradients_and_values(device, dtype, d, lens
         base._within(got[name], exp, tol[name].nan_to_num(0.0), name)
     assert (val["dv"] == INF).any() and (val["dv"] == -INF).any() and val["dk"].isinf().any()
     assert val["out"].isinf().any() and not val["dv"][:, 0].isinf().any()
+
+
+# ----------------------------------------------------------------- gradients whose terms cancel
+
+
+def _elementwise(q, k, v, bias, pair, grad, dtype):
+    """(dq, dk, p, dp - delta) of one position and head, the formula in ``dtype``."""
+    q, k, v, bias, grad = (x.to(dtype) for x in (q, k, v, bias, grad))
+    s = q @ k.T / math.sqrt(q.shape[1]) + bias[pair]
+    p = torch.exp(s - s.amax(1, keepdim=True))
+    p = p / p.sum(1, keepdim=True)
+    dp = grad @ v.T
+    off = dp - (p * dp).sum(1, keepdim=True)
+    ds = p * off
+    return ds @ k / math.sqrt(q.shape[1]), ds.T @ q / math.sqrt(q.shape[1]), p, off
+
+
+@gpu
+@pytest.mark.parametrize("lens,extra", [([100, 128, 65], 0), ([100, 128, 65], 40), ([300, 129, 512], 0),
+                                        ([300, 140, 512] * 6, 0)])
+@pytest.mark.parametrize("kind", ["peaked", "sharp", "offset", "twins"])
+@pytest.mark.parametrize("dtype,d", [(BF, 16), (BF, 32), (BF, 64), (HF, 32), (HF, 64)])
+def test_relative_attention_gradients_that_cancel(device, dtype, d, kind, lens, extra):
+    """dq and dk where dp - delta is far smaller than dp: rows that one key holds (all but 1e-3 or
+    1e-5 of the weight), keys and values with a mean of many deviations, equal keys.
+
+    In the 2-norm over a head, the error is at most the output's half step, three times the
+    error of the fp32 formula on the same inputs (the same roundings in another order), and the
+    cut of the parts: 2^-16 of the terms p |dp - delta| |k| and, for what r moves past, of their
+    row sums times sum p |k|."""
+    q, k, v, bias, coords, buckets, sl, _n, grad = base.relative_case(lens, 2, d, dtype, 23, n_latents=0, extra=extra,
+                                                                     device="cpu")
+    g = base._gen(3)
+    t = q.shape[2]
+    if kind in ("peaked", "sharp"):  # a row's own key stands out of the others by its score
+        gap = 10.0 if kind == "peaked" else 16.0
+        q = (torch.randn(q.shape, generator=g) * 0.5).to(dtype)
+        u = torch.nn.functional.normalize(torch.randn(len(lens), 2, t, d, generator=g), dim=3)
+        q, k = (u * gap).to(dtype), (u * math.sqrt(d)).to(dtype)
+        bias.zero_()
+    elif kind == "offset":
+        mean = 40.0 if dtype == HF else 160.0
+        k = (k.float() + mean * torch.randn(2, 1, d, generator=g).sign()).to(dtype)
+        v = (v.float() + mean * torch.randn(2, 1, d, generator=g).sign()).to(dtype)
+    else:  # two equal keys hold a row between them
+        u = torch.nn.functional.normalize(torch.randn(len(lens), 2, t, d, generator=g), dim=3)
+        u[:, :, 1::2] = u[:, :, 0:t - t % 2:2]
+        v = v.clone()
+        v[:, :, 1::2] = v[:, :, 0:t - t % 2:2]
+        q, k = (u * 14.0).to(dtype), (u * math.sqrt(d)).to(dtype)
+        bias.zero_()
+    case = [x.to(device) for x in (q, k, v, bias, coords, buckets, sl)] + [0, grad.to(device)]
+    got = base._run_relative(tuple(case))
+    u16 = base.HALF_STEP[dtype]
+    least = 2.0**-25 if dtype == HF else 0.0
+    for h in range(2):
+        sums = {n: [0.0] * 4 for n in ("dq", "dk")}
+        for i, n in enumerate(lens):
+            pair = base._pairs(coords[i], buckets, n, 0, bias.shape[1])
+            one = [x[i, h, :n] for x in (q, k, v)] + [bias[h], pair, grad[i, h, :n]]
+            dq, dk, p, off = _elementwise(*one, torch.float64)
+            dq32, dk32, _, _ = _elementwise(*one, torch.float32)
+            ka, qa = k[i, h, :n].double().abs(), q[i, h, :n].double().abs()
+            terms = p * off.abs()
+            cut = {"dq": terms @ ka + terms.sum(1, keepdim=True) * (p @ ka), "dk": terms.T @ qa}
+            for name, exp, low in (("dq", dq, dq32), ("dk", dk, dk32)):
+                x = got[name][i, h, :n].cpu().double()
+                for j, y in enumerate((x - exp, exp, low.double() - exp, cut[name] / math.sqrt(d))):
+                    sums[name][j] += float(y.square().sum())
+        for name, x in sums.items():
+            err, size, plain, cut = (math.sqrt(y) for y in x)
+            bound = u16 * size + 3 * plain + 2.0**-16 * cut + least * math.sqrt(sum(lens) * d)
+            assert err <= bound, (name, h, err / size, plain / size, bound / size)
