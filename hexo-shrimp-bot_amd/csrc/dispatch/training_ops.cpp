@@ -576,17 +576,8 @@ Tensor dropout_autograd(const Tensor& x, const optional<Tensor>& residual, const
 
 }  // namespace
 
+// (the operators' schemas are defined in mantisnet/library.py)
 TORCH_LIBRARY_FRAGMENT(mantisnet, m) {
-  m.def("fused_attention_relative(Tensor q, Tensor k, Tensor v, Tensor bias, Tensor coords, Tensor buckets, "
-        "Tensor seq_lens, int n_latents) -> (Tensor, Tensor, Tensor)");
-  m.def("fused_attention_relative_backward(Tensor q, Tensor k, Tensor v, Tensor bias, Tensor coords, Tensor buckets, "
-        "Tensor seq_lens, int n_latents, Tensor stats, Tensor grad_out) -> (Tensor, Tensor, Tensor, Tensor)");
-  m.def("policy_log_probs(Tensor logits, Tensor offsets, Tensor moves, int top) -> "
-        "(Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");
-  m.def("policy_log_probs_backward(Tensor logits, Tensor offsets, Tensor moves, Tensor top_moves, Tensor entropy, "
-        "Tensor norm, Tensor? grad_log_probs, Tensor? grad_entropy, Tensor? grad_lse, Tensor? grad_top) -> Tensor");
-  m.def("residual_dropout(Tensor x, Tensor? residual, Tensor rng, float p, int salt) -> Tensor");
-  m.def("residual_dropout_backward(Tensor grad_out, Tensor rng, float p, int salt, ScalarType dtype) -> Tensor");
   m.def("error_words(int device) -> Tensor?", error_words);
   m.def("set_error_words(Tensor words) -> ()", set_error_words);
 }

@@ -9,8 +9,9 @@ torch's dispatcher.
   (``csrc/dispatch/training_ops.cpp``).
 
 All are built in-tree by ``__graft_entry__.build()``.  There is no fallback:
-a missing library raises ``RuntimeError`` naming the file, so a GPU run can
-never silently take another path.
+what needs a missing library raises ``RuntimeError`` naming the file, so a GPU
+run can never silently take another path.  The package itself imports without
+the last two.
 """
 
 from __future__ import annotations
@@ -106,11 +107,28 @@ def hip() -> ctypes.CDLL:
     return _hip
 
 
-def load_operators() -> None:
-    """Register the natively written operators (once per process)."""
-    import torch
+_operators: bool | None = None
+_operators_error = ""
 
-    torch.ops.load_library(str(_built(TORCH_LIB)))
+
+def load_operators() -> bool:
+    """Load the natively written operators (once per process); False where they
+    cannot be: ``operators_error`` says why, and the operators raise it when called."""
+    global _operators, _operators_error
+    if _operators is None:
+        import torch
+
+        try:
+            torch.ops.load_library(str(_built(TORCH_LIB)))
+            _operators = True
+        except (RuntimeError, OSError) as err:  # not built, or against another torch
+            _operators_error = f"{TORCH_LIB.name} cannot be loaded: {err}"
+            _operators = False
+    return _operators
+
+
+def operators_error() -> str:
+    return _operators_error
 
 
 def check(status: int, err: ctypes.Array | None = None, what: str = "") -> None:

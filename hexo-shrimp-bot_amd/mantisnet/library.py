@@ -590,18 +590,40 @@ def _(window_pos, positions):
 # ----------------------------------------------------------------- training around the stone attention
 
 # fused_attention_relative, policy_log_probs, residual_dropout and their
-# backwards, registered natively (csrc/dispatch/training_ops.cpp): schemas,
-# kernels, fakes and gradients.
-#
-# fused_attention_relative(q, k, v, bias, coords, buckets, seq_lens, n_latents) -> (out, lse, stats):
-#   fused_attention with a learned bias by the two rows' relative position;
-#   differentiable in q, k, v and bias.
-# policy_log_probs(logits, offsets, moves, top) -> (log_probs, entropy, lse, top_log_probs, top_moves, norm):
-#   over each position's run of logits; differentiable in the logits through
-#   the first four.
-# residual_dropout(x, residual, rng, p, salt) -> out: residual + dropout(x), the
-#   mask drawn again in the backward; differentiable in x and residual.
-_native.load_operators()
+# backwards: schemas here, kernels, fakes and gradients native
+# (csrc/dispatch/training_ops.cpp).
+_TRAINING = torch.library.Library(_NS, "FRAGMENT")
+_TRAINING_SCHEMAS = {
+    # fused_attention with a learned bias by the two rows' relative position: (out, lse, stats);
+    # differentiable in q, k, v and bias
+    "fused_attention_relative":
+        "(Tensor q, Tensor k, Tensor v, Tensor bias, Tensor coords, Tensor buckets, Tensor seq_lens, int n_latents)"
+        " -> (Tensor, Tensor, Tensor)",
+    "fused_attention_relative_backward":
+        "(Tensor q, Tensor k, Tensor v, Tensor bias, Tensor coords, Tensor buckets, Tensor seq_lens, int n_latents,"
+        " Tensor stats, Tensor grad_out) -> (Tensor, Tensor, Tensor, Tensor)",
+    # over each position's run of logits: (log_probs, entropy, lse, top_log_probs, top_moves, norm);
+    # differentiable in the logits through the first four
+    "policy_log_probs":
+        "(Tensor logits, Tensor offsets, Tensor moves, int top) -> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)",
+    "policy_log_probs_backward":
+        "(Tensor logits, Tensor offsets, Tensor moves, Tensor top_moves, Tensor entropy, Tensor norm,"
+        " Tensor? grad_log_probs, Tensor? grad_entropy, Tensor? grad_lse, Tensor? grad_top) -> Tensor",
+    # residual + dropout(x), the mask drawn again in the backward; differentiable in x and residual
+    "residual_dropout": "(Tensor x, Tensor? residual, Tensor rng, float p, int salt) -> Tensor",
+    "residual_dropout_backward": "(Tensor grad_out, Tensor rng, float p, int salt, ScalarType dtype) -> Tensor",
+}
+for _name, _schema in _TRAINING_SCHEMAS.items():
+    _TRAINING.define(_name + _schema)
+
+
+def _not_loaded(*_args):
+    raise RuntimeError(_native.operators_error())
+
+
+if not _native.load_operators():
+    for _name in _TRAINING_SCHEMAS:
+        _TRAINING.impl(_name, _not_loaded, "CompositeExplicitAutograd")
 
 
 OPERATORS = (

@@ -166,10 +166,12 @@ def _flag_words(device: torch.device) -> Tensor:
     idx = device.index if device.index is not None else torch.cuda.current_device()
     f = _flags.get(idx)
     if f is None:
-        f = torch.ops.mantisnet.error_words(idx)  # (the dispatcher's operators may have made them)
+        native = _native.load_operators()
+        f = torch.ops.mantisnet.error_words(idx) if native else None  # (the dispatcher's operators may have made them)
         if f is None:
             f = torch.zeros(2, dtype=torch.int32, device=device)
-            torch.ops.mantisnet.set_error_words(f)
+            if native:
+                torch.ops.mantisnet.set_error_words(f)
         _flags[idx] = f
     return f
 
@@ -211,7 +213,7 @@ def raise_on_device_error(device: torch.device | None = None) -> None:
     """Raise if any kernel since the last check flagged bad indices."""
     devs = [device] if device is not None else [
         torch.device("cuda", i) for i in range(torch.cuda.device_count())
-        if i in _flags or torch.ops.mantisnet.error_words(i) is not None]
+        if i in _flags or (_native.load_operators() and torch.ops.mantisnet.error_words(i) is not None)]
     for d in devs:
         raise_on_bits(d, int(error_flag(d).item()))
 

@@ -8,10 +8,15 @@ The formulas in float64 and the tolerances are those of
 from __future__ import annotations
 
 import math
+import shutil
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
 
+import mantisnet
 from tests import test_training_operators as base
 
 OPS, INF, BF, HF = base.OPS, base.INF, base.BF, base.HF
@@ -288,3 +293,33 @@ def test_relative_attention_gradients_that_cancel(device, dtype, d, kind, lens, 
             err, size, plain, cut = (math.sqrt(y) for y in x)
             bound = u16 * size + 3 * plain + 2.0**-16 * cut + least * math.sqrt(sum(lens) * d)
             assert err <= bound, (name, h, err / size, plain / size, bound / size)
+
+
+# ----------------------------------------------------------------- without the GPU's libraries
+
+
+def test_the_package_imports_with_the_host_encoder_alone(tmp_path):
+    """Without libmantis_hip.so and libmantis_torch.so the package imports and a model is built; a
+    training operator raises, naming its library."""
+    root = Path(mantisnet.__file__).resolve().parents[1]
+    shutil.copytree(root / "mantisnet", tmp_path / "mantisnet", ignore=shutil.ignore_patterns("__pycache__"))
+    shutil.copy(root / "libhexo_encoder.so", tmp_path)
+    (tmp_path / "run.py").write_text(
+        "import torch, mantisnet\n"
+        "from mantisnet import ops\n"
+        "mantisnet.MantisNet(mantisnet.MantisConfig())\n"
+        "x, rng = torch.zeros(3, requires_grad=True), torch.zeros(2, dtype=torch.long)\n"
+        "for f in (torch.ops.mantisnet.residual_dropout, ops.residual_dropout):\n"
+        "    for y in (x, x.detach().to('meta')):\n"
+        "        try:\n"
+        "            f(y, None, rng.to(y.device), 0.5, 0)\n"
+        "        except RuntimeError as err:\n"
+        "            assert 'libmantis_torch.so' in str(err), err\n"
+        "        else:\n"
+        "            raise AssertionError('no error')\n"
+        "print('done')\n")
+    for broken in (False, True):  # not there; there, but not loadable
+        if broken:
+            (tmp_path / "libmantis_torch.so").write_bytes(b"no library")
+        run = subprocess.run([sys.executable, str(tmp_path / "run.py")], capture_output=True, text=True, timeout=300)
+        assert run.returncode == 0 and run.stdout.strip() == "done", run.stderr[-2000:]
