@@ -13,6 +13,8 @@
 // and recorded in the device's error words, which ops.raise_on_device_error reads.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
+#include <c10/hip/HIPGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime_api.h>
 #include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
@@ -20,6 +22,8 @@
 #include <torch/library.h>
 
 #include <array>
+#include <atomic>
+#include <memory>
 #include <mutex>
 #include <utility>
 
@@ -51,40 +55,38 @@ void* stream_of(at::Device dev) { return c10::hip::getCurrentHIPStream(dev.index
 // The devices' error words (ops.error_flag), held until the process ends.
 constexpr int kMaxDevices = 64;
 std::mutex words_lock;
-Tensor* words_of[kMaxDevices] = {};
+std::atomic<const Tensor*> words_of[kMaxDevices] = {};
 
-optional<Tensor> error_words(int64_t device) {
+// Made on the first use, filled, and only then seen by anyone else: another thread's or stream's
+// kernels write them next.  On a stream of their own and outside any capture, whose
+// memory would be the graph's, cleared by its replays.
+const Tensor& words(int64_t device) {
+  TORCH_CHECK(device >= 0 && device < kMaxDevices, "device index past ", kMaxDevices);
+  if (const Tensor* w = words_of[device].load(std::memory_order_acquire)) return *w;
   std::lock_guard<std::mutex> hold(words_lock);
-  if (device < 0 || device >= kMaxDevices || !words_of[device]) return std::nullopt;
-  return *words_of[device];
+  if (const Tensor* w = words_of[device].load(std::memory_order_acquire)) return *w;
+  const c10::impl::ExcludeDispatchKeyGuard no_modes(
+      c10::DispatchKeySet({c10::DispatchKey::Python, c10::DispatchKey::PythonTLSSnapshot}));
+  const c10::InferenceMode ordinary(false);  // (they are cleared outside of one too)
+  const at::Device dev(at::kCUDA, c10::DeviceIndex(device));
+  const c10::DeviceGuard on(dev);
+  const c10::hip::HIPStreamCaptureModeGuard apart(hipStreamCaptureModeRelaxed);
+  const c10::hip::HIPStream stream = c10::hip::getStreamFromPool(false, c10::DeviceIndex(device));
+  const c10::hip::HIPStreamGuard beside(stream);
+  auto made = std::make_unique<const Tensor>(at::zeros({2}, at::TensorOptions(at::kInt).device(dev)));
+  stream.synchronize();
+  words_of[device].store(made.get(), std::memory_order_release);
+  return *made.release();
 }
 
-void set_error_words(const Tensor& words) {
-  const int64_t device = words.get_device();
-  TORCH_CHECK_VALUE(device >= 0 && device < kMaxDevices && words.scalar_type() == at::kInt && words.numel() == 2,
-                    "error words are two int32 on a GPU");
-  std::lock_guard<std::mutex> hold(words_lock);
-  if (!words_of[device]) words_of[device] = new Tensor(words);
+// The words, made if need be or (make false) none where no one has asked for them.
+optional<Tensor> error_words(int64_t device, bool make) {
+  if (make) return words(device);
+  const Tensor* w = device >= 0 && device < kMaxDevices ? words_of[device].load(std::memory_order_acquire) : nullptr;
+  return w ? optional<Tensor>(*w) : std::nullopt;
 }
 
-int32_t* error_flag(at::Device dev) {
-  const int i = dev.index();
-  TORCH_CHECK(i < kMaxDevices, "device index past ", kMaxDevices);
-  {
-    std::lock_guard<std::mutex> hold(words_lock);
-    if (words_of[i]) return words_of[i]->data_ptr<int32_t>();
-  }
-  // made inside a capture their memory would be the graph's, cleared by replays only
-  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-  const bool asked = hipStreamIsCapturing(static_cast<hipStream_t>(stream_of(dev)), &status) == hipSuccess;
-  TORCH_CHECK(asked && status == hipStreamCaptureStatusNone,
-              "the device's error flag does not exist yet: run the operator once before capturing it");
-  set_error_words(at::zeros({2}, at::TensorOptions(at::kInt).device(dev)));
-  // (another stream's kernels may write them next)
-  TORCH_CHECK(hipStreamSynchronize(static_cast<hipStream_t>(stream_of(dev))) == hipSuccess, "the error flag's fill failed");
-  std::lock_guard<std::mutex> hold(words_lock);
-  return words_of[i]->data_ptr<int32_t>();
-}
+int32_t* error_flag(at::Device dev) { return words(dev.index()).data_ptr<int32_t>(); }
 
 void check_status(int32_t status, const char* what) {
   TORCH_CHECK_VALUE(status != MANTIS_E_ARG, what, ": unsupported shape, dtype, alignment or null input");
@@ -578,8 +580,7 @@ Tensor dropout_autograd(const Tensor& x, const optional<Tensor>& residual, const
 
 // (the operators' schemas are defined in mantisnet/library.py)
 TORCH_LIBRARY_FRAGMENT(mantisnet, m) {
-  m.def("error_words(int device) -> Tensor?", error_words);
-  m.def("set_error_words(Tensor words) -> ()", set_error_words);
+  m.def("error_words(int device, bool make) -> Tensor?", error_words);
 }
 
 namespace {

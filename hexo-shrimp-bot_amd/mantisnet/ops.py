@@ -11,6 +11,7 @@ is no CPU or PyTorch fallback: a CPU tensor is refused.
 from __future__ import annotations
 
 import ctypes
+import threading
 from typing import NamedTuple
 
 import torch
@@ -21,6 +22,7 @@ from . import _hip_api, _native
 F32, BF16, F16 = 0, 1, 2
 _FLAG_NAMES = {1: "an index was out of range", 2: "a CSR/run view was not ascending"}
 _flags: dict[int, Tensor] = {}
+_flags_lock = threading.Lock()
 
 
 def _lib():
@@ -166,12 +168,16 @@ def _flag_words(device: torch.device) -> Tensor:
     idx = device.index if device.index is not None else torch.cuda.current_device()
     f = _flags.get(idx)
     if f is None:
-        native = _native.load_operators()
-        f = torch.ops.mantisnet.error_words(idx) if native else None  # (the dispatcher's operators may have made them)
-        if f is None:
-            f = torch.zeros(2, dtype=torch.int32, device=device)
-            if native:
-                torch.ops.mantisnet.set_error_words(f)
+        if _native.load_operators():  # (one pair for these and for the dispatcher's own operators)
+            f = torch.ops.mantisnet.error_words(idx, True)
+        else:
+            with _flags_lock:
+                f = _flags.get(idx)
+                if f is None:
+                    f = torch.zeros(2, dtype=torch.int32, device=device)
+                    if not torch.cuda.is_current_stream_capturing():
+                        torch.cuda.current_stream(device).synchronize()  # (other streams write them next)
+                    _flags[idx] = f
         _flags[idx] = f
     return f
 
@@ -213,7 +219,7 @@ def raise_on_device_error(device: torch.device | None = None) -> None:
     """Raise if any kernel since the last check flagged bad indices."""
     devs = [device] if device is not None else [
         torch.device("cuda", i) for i in range(torch.cuda.device_count())
-        if i in _flags or (_native.load_operators() and torch.ops.mantisnet.error_words(i) is not None)]
+        if i in _flags or (_native.load_operators() and torch.ops.mantisnet.error_words(i, False) is not None)]
     for d in devs:
         raise_on_bits(d, int(error_flag(d).item()))
 

@@ -8,6 +8,7 @@ The formulas in float64 and the tolerances are those of
 from __future__ import annotations
 
 import math
+import os
 import shutil
 import subprocess
 import sys
@@ -323,3 +324,73 @@ def test_the_package_imports_with_the_host_encoder_alone(tmp_path):
             (tmp_path / "libmantis_torch.so").write_bytes(b"no library")
         run = subprocess.run([sys.executable, str(tmp_path / "run.py")], capture_output=True, text=True, timeout=300)
         assert run.returncode == 0 and run.stdout.strip() == "done", run.stderr[-2000:]
+
+
+# ----------------------------------------------------------------- the device's error words
+
+
+_FIRST_USE = """
+import sys, threading
+import torch, mantisnet
+from mantisnet import ops
+dev = torch.device("cuda:0")
+x = torch.randn(40, device=dev)
+offsets = torch.tensor([0, 40], device=dev)
+bad = torch.tensor([[40]], device=dev)  # one past the run
+torch.cuda.synchronize()
+
+def call():
+    return torch.ops.mantisnet.policy_log_probs(x, offsets, bad, 2)
+
+def flagged():
+    torch.cuda.synchronize()
+    try:
+        ops.raise_on_device_error()
+    except ValueError:
+        return True
+    return False
+
+def threads(first):
+    gate = threading.Barrier(8)
+    words = [None] * 8
+    def work(i):
+        with torch.cuda.stream(streams[i]):
+            gate.wait()
+            if i % 2 == first:
+                call()
+            else:
+                words[i] = ops.error_flag(dev).data_ptr()
+    streams = [torch.cuda.Stream() for _ in range(8)]
+    all_ = [threading.Thread(target=work, args=(i,)) for i in range(8)]
+    [t.start() for t in all_], [t.join() for t in all_]
+    assert {w for w in words if w} == {ops.error_flag(dev).data_ptr()}
+
+if sys.argv[1] == "threads":
+    threads(0)
+elif sys.argv[1] == "inference":
+    with torch.inference_mode():
+        call()
+        ops.error_flag(dev)
+else:
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = call()
+    assert not flagged()  # nothing has run yet
+    for _ in range(3):
+        graph.replay()
+        assert flagged() and not flagged()
+    graph.replay()
+assert flagged() and not flagged()
+call()
+assert flagged() and not flagged()
+print("done")
+"""
+
+
+@gpu
+@pytest.mark.parametrize("first", ["threads", "inference", "capture"])
+def test_error_words_are_there_before_anyone_writes_them(first):
+    """The first use of a process, by several threads and streams, in inference mode or in a capture."""
+    env = {**os.environ, "PYTHONPATH": str(Path(mantisnet.__file__).resolve().parents[1])}
+    run = subprocess.run([sys.executable, "-c", _FIRST_USE, first], capture_output=True, text=True, timeout=100, env=env)
+    assert run.returncode == 0 and run.stdout.strip().endswith("done"), run.stderr[-3000:]
