@@ -53,6 +53,7 @@
 // + key pass: 192 positions of 44-124 rows, 4 heads, 32 dims, 24 + 20 us; 16 of
 // 511-1,021 rows, 8 heads of 16 dims, 91 + 157; two lines of 2,049-4,096 rows, 8
 // heads of 64 dims, 244 + 329 (their products alone at the rate of a large matrix product: 118).
+#include <atomic>
 #include <type_traits>
 
 #include "attention_rows.hpp"
@@ -857,7 +858,7 @@ constexpr size_t static_lds(bool split) {
 // the dynamic LDS that a kernel may ask for, set once per kernel and device
 template <auto kKernel>
 bool allow_lds(size_t bytes) {
-  static bool done[64] = {};
+  static std::atomic<bool> done[64] = {};  // (threads may launch at once; setting it twice does no harm)
   int dev = 0;
   if (hipGetDevice(&dev) != hipSuccess || dev < 0) return false;
   if (dev < 64 && done[dev]) return true;

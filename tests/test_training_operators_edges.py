@@ -12,6 +12,7 @@ import os
 import shutil
 import subprocess
 import sys
+import threading
 from pathlib import Path
 
 import pytest
@@ -394,3 +395,28 @@ def test_error_words_are_there_before_anyone_writes_them(first):
     env = {**os.environ, "PYTHONPATH": str(Path(mantisnet.__file__).resolve().parents[1])}
     run = subprocess.run([sys.executable, "-c", _FIRST_USE, first], capture_output=True, text=True, timeout=100, env=env)
     assert run.returncode == 0 and run.stdout.strip().endswith("done"), run.stderr[-3000:]
+
+
+@gpu
+def test_threads_share_the_backward(device):
+    """Eight threads, a stream and a variant each, against the same calls one by one."""
+    cases = [base.relative_case([130, 64, 200][:1 + i % 3], 1 + i % 2, (16, 32, 64)[i % 3], (BF, HF)[i // 4], i,
+                                device=device) for i in range(8)]
+    want = [base._run_relative(c) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    gate, got = threading.Barrier(8), [None] * 8
+
+    def work(i):
+        with torch.cuda.stream(streams[i]):
+            gate.wait()
+            got[i] = [base._run_relative(cases[i]) for _ in range(5)]
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(8)]
+    for x in threads:
+        x.start()
+    for x in threads:
+        x.join()
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        assert all(torch.equal(one[n], w[n]) for one in g for n in w)
