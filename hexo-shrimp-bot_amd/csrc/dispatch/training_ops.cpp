@@ -105,7 +105,11 @@ T* ptr(const optional<Tensor>& t) {
   return t && t->defined() ? static_cast<T*>(t->data_ptr()) : nullptr;
 }
 
+// (a tangent would be lost below autograd)
 bool wants_grad(std::initializer_list<const Tensor*> tensors) {
+  for (const Tensor* t : tensors)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t || !t->defined() || !t->_fw_grad(/*level=*/0).defined(),
+                                "forward-mode differentiation of the MantisNet operators is not implemented");
   if (!at::GradMode::is_enabled()) return false;
   for (const Tensor* t : tensors)
     if (t && t->defined() && t->requires_grad()) return true;

@@ -420,3 +420,31 @@ def test_threads_share_the_backward(device):
     torch.cuda.synchronize()
     for g, w in zip(got, want):
         assert all(torch.equal(one[n], w[n]) for one in g for n in w)
+
+
+def test_forward_mode_is_refused():
+    """A tangent is an error, with and without gradients asked for, not a zero."""
+    import torch.autograd.forward_ad as fwad
+
+    new = lambda *s, dtype=torch.float32: torch.empty(s, dtype=dtype, device="meta")  # noqa: E731
+    i32, i64 = torch.int32, torch.int64
+    q = new(2, 4, 9, 32, dtype=BF)
+    rest = (new(4, 12), new(2, 9, 2, dtype=i32), new(5, 7, dtype=i32), new(2, dtype=i32), 4)
+    rng = new(2, dtype=i64)
+    calls = [
+        (lambda x: OPS.fused_attention_relative(x, q, q, *rest)[0], q),
+        (lambda x: OPS.fused_attention_relative(q, q, x, *rest)[0], q),
+        (lambda x: OPS.fused_attention_relative(q, q, q, x, *rest[1:])[0], rest[0]),
+        (lambda x: OPS.policy_log_probs(x, new(3, dtype=i64), new(2, 1, dtype=i64), 2)[0], new(10)),
+        (lambda x: OPS.residual_dropout(x, None, rng, 0.5, 0), new(10)),
+        (lambda x: OPS.residual_dropout(new(10), x, rng, 0.5, 0), new(10)),
+    ]
+    for call, x in calls:
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.func.jvp(call, (x,), (torch.empty_like(x),))
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(lambda y: torch.func.grad(lambda z: call(z).sum())(y), (x,), (torch.empty_like(x),))
+        for leaf in (x, x.clone().requires_grad_(True)):
+            with fwad.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
+                call(fwad.make_dual(leaf, torch.empty_like(x)))
+        call(x)
