@@ -101,7 +101,10 @@ __device__ __forceinline__ void products_onto(const uint16_t* s, int n, int l16,
   using FR = Frag<kHalf>;
 #pragma unroll
   for (int tt = 0; tt < 4; ++tt) {
-    if (16 * tt >= n) continue;  // uniform
+    if (16 * tt >= n) {  // uniform
+      around_products();
+      continue;
+    }
 #pragma unroll
     for (int ks = 0; ks < G::kKs; ++ks) {
       uint4 a = *reinterpret_cast<const uint4*>(s + (16 * tt + l16) * G::kPitch + G::kdim(ks, g));
@@ -126,7 +129,10 @@ __device__ __forceinline__ void accumulate(const uint16_t* st, int n, int l16, i
                                            f32x4_t (&acc)[Geom<kHalf, HD>::kDt]) {
 #pragma unroll
   for (int tt = 0; tt < 4; ++tt) {
-    if (16 * tt >= n) break;  // uniform
+    if (16 * tt >= n) {  // uniform
+      around_fp32_products();
+      continue;
+    }
     uint2 a[Geom<kHalf, HD>::kDt];
 #pragma unroll
     for (int dt = 0; dt < Geom<kHalf, HD>::kDt; ++dt)

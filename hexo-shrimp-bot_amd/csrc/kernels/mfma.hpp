@@ -34,6 +34,15 @@ __device__ __forceinline__ f32x4_t mfma16x16x32(f16x8_t a, f16x8_t b, f32x4_t c)
 }
 
 
+// The way around a block of products (`if (none) { around_products(); continue; }`, a block at a
+// time: out of a loop of them the compiler joins the ways).  A result is read eight wait states
+// after its instruction at the earliest (ten of an fp32 product), and the compiler counts them along the
+// way through the block and not along the branch that skips it.  Waited here and not at
+// the reader: where results live in accumulator registers the compiler copies them out
+// before anything that names them.
+__device__ __forceinline__ void around_products() { asm volatile("s_nop 7"); }
+__device__ __forceinline__ void around_fp32_products() { asm volatile("s_nop 9"); }
+
 // Element-type traits of the 16-bit MFMA operand formats.
 template <bool kHalf>
 struct Frag;

@@ -44,15 +44,6 @@ struct Operand {  // (P, A, T, hd): base and element strides
   int64_t sp, sa, st;
 };
 
-// Scores whose last matrix instruction may lie one branch back.  A result is
-// read eight wait states after its instruction at the earliest; where tiles
-// past the last key are left out, the compiler counts them along the way through
-// the next tile and not along the branch that skips it, and a row of up to 16 keys
-// took its reference point from the bias alone.
-__device__ __forceinline__ void settle(f32x4_t (&s)[4]) {
-  asm volatile("s_nop 7" : "+v"(s[0]), "+v"(s[1]), "+v"(s[2]), "+v"(s[3]));
-}
-
 // kSplit (kSub 1): an item has 16 queries, and its wavefronts every fourth chunk of keys each.
 template <bool kHalf, int HD, int kSub, bool kSplit>
 __global__ void __launch_bounds__(256)
@@ -212,7 +203,10 @@ relative_attention_kernel(Operand q, Operand k, Operand v, Relative rel, const i
       }
 #pragma unroll
       for (int tt = 0; tt < 4; ++tt) {
-        if (kMasked && 16 * tt >= n) break;
+        if (kMasked && 16 * tt >= n) {
+          around_products();
+          continue;
+        }
 #pragma unroll
         for (int ks = 0; ks < kKs; ++ks) {
           uint4 ku = *reinterpret_cast<const uint4*>(&sk[buf][(16 * tt + l16) * kKPitch + kdim(ks)]);
@@ -221,10 +215,6 @@ relative_attention_kernel(Operand q, Operand k, Operand v, Relative rel, const i
 #pragma unroll
           for (int j = 0; j < kNJ; ++j) s[j][tt] = mfma16x16x32(kf, qf[j][ks], s[j][tt]);
         }
-      }
-      if (kMasked) {
-#pragma unroll
-        for (int j = 0; j < kNJ; ++j) settle(s[j]);
       }
       typename FR::vec pf[kNJ][2];
 #pragma unroll
@@ -269,7 +259,10 @@ relative_attention_kernel(Operand q, Operand k, Operand v, Relative rel, const i
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        if (kMasked && 32 * h >= n) break;
+        if (kMasked && 32 * h >= n) {
+          around_products();
+          continue;
+        }
 #pragma unroll
         for (int dt = 0; dt < kDt; ++dt) {
           const typename FR::vec vf = FR::cast(transposed_frag<HD>(sv[buf], h, dt, l16, g));

@@ -136,7 +136,10 @@ __device__ __forceinline__ void accumulate_parts(const uint16_t* s, int n, int l
   using FR = Frag<kHalf>;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    if (32 * h >= n) break;  // uniform
+    if (32 * h >= n) {  // uniform
+      around_products();
+      continue;
+    }
     uint32_t hi[4], lo[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -171,7 +174,10 @@ __device__ __forceinline__ void accumulate_two(const uint16_t* s, int n, int l16
   using FR = Frag<kHalf>;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    if (32 * h >= n) break;  // uniform
+    if (32 * h >= n) {  // uniform
+      around_products();
+      continue;
+    }
     uint32_t xh[4], xl[4], yh[4], yl[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
