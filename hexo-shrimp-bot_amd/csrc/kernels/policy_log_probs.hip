@@ -441,8 +441,15 @@ policy_backward_kernel(const T* __restrict__ logits, int64_t stride, const int64
   float* add = reinterpret_cast<float*>(at + entries);  // (entries): its gradient
   __shared__ float sums[kWaves];
   const int64_t p = blockIdx.x / slices, sl = blockIdx.x % slices;
+  auto clear = [&](int64_t lo, int64_t hi) {  // this slice's share of [lo, hi)
+    for (int64_t i = lo + sl * kThreads + threadIdx.x; i < hi; i += int64_t(slices) * kThreads) narrow(dx[i], 0.f);
+  };
+  auto bound = [&](int64_t i) { return i < 0 ? 0 : i > n ? n : i; };
   int64_t a, b;
-  run_of(offsets, p, n, a, b, flag);
+  // what no run holds has no gradient: entries between offsets that are no run, before the first and after the last
+  if (!run_of(offsets, p, n, a, b, flag)) clear(bound(offsets[p]), bound(offsets[p + 1]));
+  if (p == 0) clear(0, bound(offsets[0]));
+  if (p == n_pos - 1) clear(bound(offsets[n_pos]), n);
   const int64_t len = b - a, from = len * sl / slices, to = len * (sl + 1) / slices;
   const float m = norm[2 * p], log_l = norm[2 * p + 1], h = entropy[p];
   const bool none = log_l == -INFINITY;
@@ -492,13 +499,6 @@ policy_backward_kernel(const T* __restrict__ logits, int64_t stride, const int64
   }
   for (int64_t i = from + threadIdx.x; i < body; i += kThreads) narrow(dx[a + i], none ? 0.f : base(i));
   for (int64_t i = tail + threadIdx.x; i < to; i += kThreads) narrow(dx[a + i], none ? 0.f : base(i));
-  // what no run holds has no gradient
-  const int64_t stop = p == 0 ? (offsets[0] < 0 ? 0 : offsets[0] > n ? n : offsets[0]) : 0;
-  for (int64_t i = sl * kThreads + threadIdx.x; i < stop; i += int64_t(slices) * kThreads) narrow(dx[i], 0.f);
-  if (p == n_pos - 1)
-    for (int64_t i = (offsets[n_pos] < 0 ? 0 : offsets[n_pos]) + sl * kThreads + threadIdx.x; i < n;
-         i += int64_t(slices) * kThreads)
-      narrow(dx[i], 0.f);
   if (none) return;
   __syncthreads();  // (orders the writes above before those of the same entries below)
   for (int e = threadIdx.x; e < entries; e += kThreads) {

@@ -19,6 +19,7 @@ import pytest
 import torch
 
 import mantisnet
+from mantisnet import ops
 from tests import test_training_operators as base
 
 OPS, INF, BF, HF = base.OPS, base.INF, base.BF, base.HF
@@ -448,3 +449,26 @@ def test_forward_mode_is_refused():
             with fwad.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
                 call(fwad.make_dual(leaf, torch.empty_like(x)))
         call(x)
+
+
+# ----------------------------------------------------------------- index tables that are none
+
+
+@gpu
+@pytest.mark.parametrize("n", [83, 30000])
+@pytest.mark.parametrize("bad", [[0, 2.0, 0.5, 0.8], [0.2, 0.1, 0.6, 0.6], [-1.0, 0.5, 0.7, 0.9], [2.0, 3.0, 2.5, 1.5],
+                                 [0.9, 0.1, 0.0, -1.0]])
+def test_policy_gradients_outside_every_run_are_zero_whatever_the_offsets(device, n, bad):
+    x = torch.randn(n, device=device, requires_grad=True)
+    offsets = [int(f * n) for f in bad]
+    moves = torch.full((3, 1), -1, device=device)
+    entropy, lse = OPS.policy_log_probs(x, torch.tensor(offsets, device=device), moves, 2)[1:3]
+    torch.full_like(x, math.nan)  # (its memory is the next result's)
+    (dx,) = torch.autograd.grad(entropy.sum() + lse.sum(), x)
+    with pytest.raises(ValueError, match="not ascending"):
+        ops.raise_on_device_error(device)
+    outside = torch.ones(n, dtype=torch.bool)
+    for a, b in zip(offsets, offsets[1:]):
+        if 0 <= a <= b <= n:
+            outside[a:b] = False
+    assert dx.isfinite().all() and not dx.cpu()[outside].any() and outside.any()
