@@ -354,8 +354,10 @@ relative_attention_kernel(Operand q, Operand k, Operand v, Relative rel, const i
       }
       if (g == 0) {
         const float m0 = m[j] == -INFINITY ? 0.f : m[j], log2l = log2f(lr);  // (an empty row's sum is 0)
-        // (a row of scores at the lowest finite value has that as its lse)
-        lp[qrow[j]] = !live ? 0.f : fabsf(m0) == kLargest ? m0 : fmaf(m0, 1.f / root_hd, log2l * 0.6931471805599453f);
+        // (a row of scores at the lowest finite value has that as its lse, unless a NaN is among them)
+        lp[qrow[j]] = !live                                 ? 0.f
+                      : fabsf(m0) == kLargest && lr == lr ? m0
+                                                          : fmaf(m0, 1.f / root_hd, log2l * 0.6931471805599453f);
         sp[qrow[j]] = live && lr != 0.f ? make_float2(m0, log2l) : make_float2(0.f, INFINITY);
       }
     }

@@ -472,3 +472,21 @@ def test_policy_gradients_outside_every_run_are_zero_whatever_the_offsets(device
         if 0 <= a <= b <= n:
             outside[a:b] = False
     assert dx.isfinite().all() and not dx.cpu()[outside].any() and outside.any()
+
+
+@gpu
+@pytest.mark.parametrize("lens", [[70, 20], [200, 20], [150] * 60])
+@pytest.mark.parametrize("bad", [math.nan, INF])
+def test_relative_attention_a_bad_key_beside_lowest_scores(device, lens, bad):
+    """A NaN (or infinite) score beside scores of the lowest finite value: its row is NaN, lse too."""
+    q, k, v, bias, coords, buckets, sl, _n, _grad = base.relative_case(lens, 2, 32, BF, 9, n_latents=0, device=device)
+    bias[:] = torch.finfo(torch.float32).min
+    q = q.abs()
+    k[0, 1, 5, 3] = bad
+    out, lse, _ = OPS.fused_attention_relative(q, k, v, bias, coords, buckets, sl, 0)
+    assert out[0, 1, :lens[0]].isnan().all()
+    if math.isnan(bad):
+        assert lse[0, 1, :lens[0]].isnan().all()
+    assert not out[0, 0].isnan().any() and not lse[0, 0].isnan().any() and not out[1:].isnan().any()
+    clean = lse[1, :, :lens[1]]
+    assert torch.equal(clean, torch.full_like(clean, torch.finfo(torch.float32).min))
