@@ -18,9 +18,11 @@
 // (bias * sqrt(hd) included), in fp32 and with the difference first, so a row
 // of scores at the type's lowest value is still uniform; m moves only when a
 // score passes it by more than 8 in log2 units.  The probabilities enter the
-// value product rounded to 16 bits (relative 2^-9 or 2^-12 of each, as their
-// output rounds once more); the output is divided by the sum of the rounded ones,
-// so a row of one key is that key's value, and lse is the log of the unrounded fp32 sum.
+// value product rounded to 16 bits, half a step of each as the output rounds once
+// more: 2^-8 of it in bf16, 2^-11 in fp16 and there, under 2^-14 beside a largest one of 1
+// to 2^8, 2^-25 outright (under that it counts as 0, beside an infinite value too).  The
+// output is divided by the sum of the rounded ones, so a row of one key is that key's
+// value, and lse is the log of the unrounded fp32 sum.
 //
 // Bound by the pairs' vector work (table offset, lookup, maximum, exp2, sum, pack:
 // some 20 instructions for each, against 4 hd matrix operations), not by memory.
