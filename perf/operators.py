@@ -192,8 +192,9 @@ def _operators():
 
 def _own_relative(st):
     q, k, v, bias = st["leaves"]
+    latents = min(st["latents"], q.shape[2])  # (a drawn batch may have fewer rows than latents)
     out, lse, _stats = _operators().fused_attention_relative(q, k, v, bias, st["coords"], st["buckets"], st["lens"],
-                                                            st["latents"])
+                                                            latents)
     if not st["train"]:
         return {"out": out, "lse": lse}
     grads = torch.autograd.grad(out, st["leaves"], st["grad"])
