@@ -571,15 +571,16 @@ relative_bwd_q_kernel(Rows q, Rows k, Rows v, Rows go, Relative rel, const int32
         const float by = next - r;
         r = next;
         move(by);
-        rest = fmaf(-by, lane_weight, rest);
-        lane_weight += w;
+        float terms = 0.f;  // (a chunk's among themselves first)
 #pragma unroll
         for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
           for (int t = 0; t < 4; ++t) {
             dp[tt][t] = p[tt][t] * (dp[tt][t] - r);
-            rest += dp[tt][t];
+            terms += dp[tt][t];
           }
+        rest = fmaf(-by, lane_weight, rest) + terms;
+        lane_weight += w;
         const int rows = decltype(whole)::value ? kTile : n;
         if constexpr (kHalf) {
           const float undo = chunk_scale(dp);
