@@ -37,7 +37,8 @@
 // 1,741 + 957 us where these parts took 619 + 337.)
 // dk and dv keep the sums of both parts apart until the end, where an infinite one is
 // the hi parts' alone (join_parts); any infinity that reaches dq is NaN by the formula.
-// (A position of 1,024 rows, 2 heads of 64 dims: backward 53.3 -> 55.9 us, wider grids the same.)
+// (That took the backward of one position of 1,024 rows, 2 heads of 64 dims, from 53.3 to
+// 55.9 us, and left wider grids as they were.)
 //
 // The bias gradient: every lane adds its ds to its own column of the
 // workgroup's LDS table (a row of 64 lanes per bucket and wavefront: no two
@@ -50,9 +51,9 @@
 // Bound by the pairs' vector and LDS work, not by memory or the matrix units: a
 // pair takes two products to recompute p and dp, exp2, the split into parts and,
 // in the pass with the bucket sums, two LDS accesses more.  Measured, query pass
-// + key pass: 192 positions of 44-124 rows, 4 heads, 32 dims, 24 + 20 us; 16 of
-// 511-1,021 rows, 8 heads of 16 dims, 91 + 157; two lines of 2,049-4,096 rows, 8
-// heads of 64 dims, 244 + 329 (their products alone at the rate of a large matrix product: 118).
+// + key pass: 192 positions of 44-124 rows, 4 heads, 32 dims, 25 + 20 us; 16 of
+// 511-1,021 rows, 8 heads of 16 dims, 101 + 156; two lines of 2,049-4,096 rows, 8
+// heads of 64 dims, 263 + 324 (their products alone at the rate of a large matrix product: 118).
 #include <atomic>
 #include <type_traits>
 

@@ -205,9 +205,9 @@ inline int64_t item_grid(int64_t n_pos, int heads, int64_t n_tiles) {
 // wavefronts.  Each stages its own, so the LDS grows with the head's width and at
 // 64 dims the few workgroups that fit a CU gain from this only when tiles are fewer
 // still.  The three passes of one position, 16 rows to a workgroup against 64: 2,000
-// rows of 4 heads, 32 dims (128 tiles of 64) 138 against 169 us, 16 dims 122 / 161;
-// 1,024 rows, 32 dims 54 / 93; 4,096 rows, 32 dims (256 tiles) 459 / 431, 16 dims 412 / 402;
-// 64 dims, 2 heads, 1,024 rows (32 tiles) 73 / 103, 2,048 rows (64 tiles) 226 / 200.
+// rows of 4 heads, 32 dims (128 tiles of 64) 133 against 161 us, 16 dims 121 / 160;
+// 1,024 rows, 32 dims 52 / 89; 4,096 rows, 32 dims (256 tiles) 427 / 402, 16 dims 398 / 388;
+// 64 dims, 2 heads, 1,024 rows (32 tiles) 74 / 100, 2,048 rows (64 tiles) 217 / 183.
 inline bool few_groups(int64_t n_pos, int64_t heads, int64_t t, int64_t hd) {
   return t > 128 && n_pos * heads * ((t + 63) / 64) <= (hd < 64 ? 128 : 32);
 }
