@@ -19,7 +19,7 @@ import pytest
 import torch
 
 import mantisnet
-from mantisnet import ops
+from mantisnet import ops, tables
 from tests import test_training_operators as base
 
 OPS, INF, BF, HF = base.OPS, base.INF, base.BF, base.HF
@@ -334,7 +334,7 @@ def test_the_package_imports_with_the_host_encoder_alone(tmp_path):
 _FIRST_USE = """
 import sys, threading
 import torch, mantisnet
-from mantisnet import ops
+from mantisnet import ops, tables
 dev = torch.device("cuda:0")
 x = torch.randn(40, device=dev)
 offsets = torch.tensor([0, 40], device=dev)
@@ -490,3 +490,29 @@ def test_relative_attention_a_bad_key_beside_lowest_scores(device, lens, bad):
     assert not out[0, 0].isnan().any() and not lse[0, 0].isnan().any() and not out[1:].isnan().any()
     clean = lse[1, :, :lens[1]]
     assert torch.equal(clean, torch.full_like(clean, torch.finfo(torch.float32).min))
+
+
+@gpu
+def test_relative_attention_bias_gradient_of_long_rows(device):
+    """dbias over 2,300 rows, most of whose pairs share a bucket: what stays of a row whose ds sum to
+    zero is delta's own rounding.  In the 2-norm over four heads and four batches at most sqrt(5) times
+    the fp32 formula's (summed up in float64): its roundings of scores, p and delta, and for each of the
+    fp32 sums, delta's and the buckets' columns, those of its terms and of the sum, all independent."""
+    n, heads, d = 2300, 4, 32
+    buckets, count = tables.relative_buckets(12)
+    err = low = 0.0
+    for seed in range(4):
+        q, k, v, _bias, coords, _b, lens, n_latents, grad = base.relative_case([n], heads, d, BF, seed, spread=26.0)
+        bias = 0.5 * torch.randn(heads, count, generator=base._gen(seed))
+        case = [x.to(device) for x in (q, k, v, bias, coords, buckets, lens)] + [n_latents, grad.to(device)]
+        got = base._run_relative(tuple(case))["dbias"].double()
+        pair = base._pairs(coords[0], buckets, n, n_latents, count).to(device)
+        for h in range(heads):
+            sums = []
+            for dtype in (torch.float64, torch.float32):
+                one = [x[0, h].to(device) for x in (q, k, v)] + [bias[h].to(device), pair, grad[0, h].to(device)]
+                _, _, p, off = _elementwise(*one, dtype)
+                sums.append(torch.bincount(pair.reshape(-1), (p * off).double().reshape(-1), minlength=count))
+            err += float((got[h] - sums[0]).square().sum())
+            low += float((sums[1] - sums[0]).square().sum())
+    assert err <= 5 * low, math.sqrt(err / low)
